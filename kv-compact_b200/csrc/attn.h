@@ -1,0 +1,205 @@
+// attn.h — what the attention kernels share: the launch arguments, the
+// sequences of a batch as the device sees them, the split of their keys over
+// the CTAs, and the stored elements.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "serve.h"
+
+#include "kv-compact-api.h"
+
+struct kvc_attn_args {
+    // queries: element (token, head, i) at q + token*q_stride + head*q_head + i
+    const void * q;
+    void * out;             // [n_total x Hq x dv]
+    float * lse;            // [n_total x Hq] or null
+    long long q_stride, q_head;
+    const int * cu_q;       // [n_seqs + 1]
+    int q_type;
+    int n_seqs, n_total, max_q;
+    int Hq, Hkv, g, dk, dv;
+    float scale;
+    // keys: row r, head h at K + r*k_rb + h*k_hb bytes
+    const uint8_t * K;
+    const uint8_t * V;
+    long long k_rb, k_hb, v_rb, v_hb;
+    int k_type, v_type;
+    // packed prompts (cu_k != null)
+    const int * cu_k;       // [n_seqs + 1]
+    int n_keys;
+    int causal;
+    // paged cache (seqs != null)
+    const int * seqs;
+    const int * table;
+    const int * seq_len;
+    const float * beta;     // [pages x Hkv x page] or null
+    const uint32_t * mask;
+    int mask_words;
+    int n_slots, n_pages, max_pages, page;
+    kvc_divisor by_page, by_group;
+    // the split: W workers per (KV head, row block)
+    int W;
+    float * part;           // partial results
+};
+
+// One sequence of a batch.
+struct kvc_attn_seq {
+    int q0, nq;             // rows of q
+    int ln;                 // keys
+    int k0;                 // packed: first key row
+    const int * table;      // paged: its table row
+};
+
+__device__ __forceinline__ kvc_attn_seq attn_seq(const kvc_attn_args & a, int s) {
+    kvc_attn_seq r;
+    r.q0 = min(max(a.cu_q[s], 0), a.n_total);
+    r.nq = min(min(max(a.cu_q[s + 1], r.q0), a.n_total) - r.q0, a.max_q);
+    r.k0 = 0;
+    r.ln = 0;
+    r.table = nullptr;
+    if (a.cu_k) {
+        r.k0 = min(max(a.cu_k[s], 0), a.n_keys);
+        r.ln = min(max(a.cu_k[s + 1], r.k0), a.n_keys) - r.k0;
+    } else {
+        const int slot = a.seqs[s];
+        if (slot >= 0 && slot < a.n_slots) {
+            r.table = a.table + (size_t)slot * a.max_pages;
+            r.ln = min(max(a.seq_len[slot], 0), a.max_pages * a.page);
+        }
+    }
+    return r;
+}
+
+// Row number of key j in K and V (and its page and place), or -1.
+__device__ __forceinline__ long long attn_row(const kvc_attn_args & a, const kvc_attn_seq & q, int j, int * page,
+                                              int * off) {
+    if (a.cu_k) return (long long)q.k0 + j;
+    const int b = (int)a.by_page.div((uint32_t)j);
+    const int p = q.table[b];
+    if (p < 0 || p >= a.n_pages) return -1;
+    *page = p;
+    *off = j - b * a.page;
+    return (long long)p * a.page + *off;
+}
+
+// Whether node / query i of a sequence sees key j (j < ln).
+__device__ __forceinline__ bool attn_sees(const kvc_attn_args & a, const kvc_attn_seq & q, int i, int j) {
+    if (a.cu_k) return !a.causal || j <= i + (q.ln - q.nq);
+    const int b = j - (q.ln - q.nq);
+    if (b < 0 || !a.mask) return true;
+    return (b >> 5) < a.mask_words && ((a.mask[(size_t)(q.q0 + i) * a.mask_words + (b >> 5)] >> (b & 31)) & 1u);
+}
+
+// ---- the split of the keys ---------------------------------------------------
+//
+// For one (KV head, row block of RB rows) the key tiles of all sequences that
+// have rows in the block are laid end to end, and worker w of W takes tiles
+// [w*T/W, (w+1)*T/W). Sequences of any lengths then load the workers evenly.
+// A worker's stretch meets at most two sequences that it does not cover whole:
+// the one it starts inside of (slot 0) and the one it ends inside of (slot 1);
+// their partial results go to those slots and are joined afterwards, in the
+// workers' order.
+
+template <int RB, int TILE>
+__device__ __forceinline__ int attn_tiles(const kvc_attn_args & a, int s, int qb) {
+    const kvc_attn_seq q = attn_seq(a, s);
+    if (qb * RB >= (long long)q.nq * a.g) return 0;
+    return (q.ln + TILE - 1) / TILE;
+}
+
+// Total tiles of row block qb, the same in every lane.
+template <int RB, int TILE>
+__device__ __forceinline__ long long attn_total(const kvc_attn_args & a, int qb) {
+    const int lane = threadIdx.x & 31;
+    long long t = 0;
+    for (int s = lane; s < a.n_seqs; s += 32) t += attn_tiles<RB, TILE>(a, s, qb);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(~0u, t, o);
+    return t;
+}
+
+// fn(s, lo, hi, slot) for every piece of worker w's stretch: tiles lo..hi-1 of
+// sequence s; slot -1 where that is all of them. Every warp of a CTA takes the
+// same steps.
+template <int RB, int TILE, typename F>
+__device__ __forceinline__ void attn_walk(const kvc_attn_args & a, int qb, int w, F && fn) {
+    const int lane = threadIdx.x & 31;
+    int mine0 = lane < a.n_seqs ? attn_tiles<RB, TILE>(a, lane, qb) : 0;
+    long long T = mine0;
+    for (int s = lane + 32; s < a.n_seqs; s += 32) T += attn_tiles<RB, TILE>(a, s, qb);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) T += __shfl_xor_sync(~0u, T, o);
+    const long long from = w * T / a.W, to = (w + 1) * T / a.W;
+    long long at = 0;
+    for (int s0 = 0; s0 < a.n_seqs && at < to; s0 += 32) {
+        const int s = s0 + lane;
+        const int t = s0 == 0 ? mine0 : (s < a.n_seqs ? attn_tiles<RB, TILE>(a, s, qb) : 0);
+        long long p = t;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(~0u, p, o);
+            if (lane >= o) p += u;
+        }
+        const long long end = __shfl_sync(~0u, p, 31);
+        p += at - t;
+        unsigned hit = __ballot_sync(~0u, t > 0 && p < to && p + t > from);
+        while (hit) {
+            const int l = __ffs(hit) - 1;
+            hit &= hit - 1;
+            const long long ps = __shfl_sync(~0u, p, l);
+            const int ts = __shfl_sync(~0u, t, l);
+            const int lo = (int)(max(from, ps) - ps), hi = (int)(min(to, ps + ts) - ps);
+            fn(s0 + l, lo, hi, lo == 0 && hi == ts ? -1 : (from > ps ? 0 : 1));
+        }
+        at += end;
+    }
+}
+
+// Worker that holds tile x of T.
+__device__ __forceinline__ int attn_worker(long long x, long long T, int W) {
+    return (int)(((x + 1) * W - 1) / T);
+}
+
+// Partial results of worker w, slot s: RB sums of d_v, then RB maxima, RB sums.
+template <int RB>
+__device__ __forceinline__ float * attn_part(const kvc_attn_args & a, int qb, int h, int w, int slot) {
+    return a.part + ((((size_t)qb * a.Hkv + h) * a.W + w) * 2 + slot) * ((size_t)RB * (a.dv + 2));
+}
+inline size_t kvc_attn_part_bytes(int rb, long long blocks, int W, int dv) {
+    return W > 1 ? (size_t)blocks * W * 2 * rb * (dv + 2) * sizeof(float) : 0;
+}
+
+// Joins the partial results and writes rows that no tile reached (attn_simt.cu).
+// RB and TILE are those of the kernel that ran.
+int kvc_launch_attn_join(const kvc_attn_args & a, int rb, int tile, cudaStream_t st);
+// The general kernel: every type, d <= 256, any strides (attn_simt.cu).
+int kvc_attn_simt_workers(const kvc_attn_args & a, int sms);
+int kvc_launch_attn_simt(const kvc_attn_args & a, cudaStream_t st);
+constexpr int KVC_SIMT_RB = 8, KVC_SIMT_TILE = 128;
+
+// ---- stored elements -----------------------------------------------------------
+// Element e of a row's head segment at p (block types: segments start on a block).
+__device__ __forceinline__ float attn_half(const uint8_t * p) {        // 2-byte aligned
+    return __half2float(*reinterpret_cast<const __half *>(p));
+}
+__device__ __forceinline__ float attn_elem(const uint8_t * p, int type, int e) {
+    switch (type) {
+    case KV_TYPE_F32: return reinterpret_cast<const float *>(p)[e];
+    case KV_TYPE_F16: return attn_half(p + 2 * e);
+    case KV_TYPE_Q8_0: {
+        const uint8_t * b = p + (e >> 5) * 34;
+        return attn_half(b) * (float)(int8_t)b[2 + (e & 31)];
+    }
+    case KV_TYPE_Q4_0: {
+        const uint8_t * b = p + (e >> 5) * 18;
+        const int q = b[2 + ((e & 31) >> 1)];
+        return attn_half(b) * ((float)((e & 1) ? q >> 4 : q & 15) - 8.0f);
+    }
+    default: {
+        const uint8_t * b = p + (e >> 5) * 20;
+        const int q = b[4 + ((e & 31) >> 1)];
+        return fmaf(attn_half(b), (float)((e & 1) ? q >> 4 : q & 15), attn_half(b + 2));
+    }
+    }
+}

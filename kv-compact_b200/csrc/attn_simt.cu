@@ -1,0 +1,315 @@
+// attn_simt.cu — the general attention kernel and the join of partial results
+// (include/kvc-attn.h). The tensor-core kernels (attn_tree.cu,
+// attn_prompt.cu) take the common types and shapes; this one takes the rest:
+// F32 rows, head sizes and strides that those do not read.
+//
+//   x_ij = scale q_i.k_j (+ beta_j),  m = max_j x_ij,  l = sum_j exp(x_ij - m),
+//   out_i = (sum_j exp(x_ij - m) v_j) / l,  lse_i = m + log l
+//
+// in one pass over the keys with a running m, l and sum (flash decoding).
+#include "attn.h"
+
+#include <math.h>
+
+namespace {
+
+constexpr int RB = KVC_SIMT_RB, TILE = KVC_SIMT_TILE;
+constexpr int WARPS = 4, THREADS = 32 * WARPS, WK = 32;
+static_assert(TILE == WARPS * WK, "a tile is one key per lane");
+
+// One CTA: 8 query rows of one KV head against its stretch of the keys. A
+// warp takes 32 keys of a tile, decodes their K rows into its own shared
+// memory, scores one key per lane, then does the same with V with one output
+// dimension per lane: no barrier inside the loop. Bound by the shared-memory
+// reads of the two products (9 words per 8 multiply-adds).
+template <int DV_LANES>
+__global__ void __launch_bounds__(THREADS) k_attn_simt(const __grid_constant__ kvc_attn_args a) {
+    extern __shared__ float sm[];
+    const int pitch = max(a.dk, a.dv) | 1;               // odd: a column read hits 32 banks
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float * qs = sm;                                     // [RB][dk]
+    float * ps = qs + RB * a.dk + warp * (RB * WK);      // [RB][32] of this warp
+    float * buf = qs + RB * a.dk + WARPS * RB * WK + (size_t)warp * WK * pitch;
+    float * joinO = qs + RB * a.dk + WARPS * RB * WK;    // reused after the loop: [WARPS][RB][dv] (dv <= pitch, RB <= 32)
+    __shared__ float s_m[WARPS][RB], s_l[WARPS][RB];
+    const int h = blockIdx.y % a.Hkv, w = blockIdx.x;
+    const int n_blocks = (int)(((long long)a.max_q * a.g + RB - 1) / RB);
+
+    for (int qb = blockIdx.y / a.Hkv; qb < n_blocks; qb += gridDim.y / a.Hkv) {
+    attn_walk<RB, TILE>(a, qb, w, [&](int s, int lo, int hi, int slot) {
+        const kvc_attn_seq q = attn_seq(a, s);
+        const int r0 = qb * RB;
+        const int nr = (int)min((long long)RB, (long long)q.nq * a.g - r0);
+        __syncthreads();
+        for (int e = threadIdx.x; e < RB * a.dk; e += THREADS) {
+            const int r = e / a.dk, d = e - r * a.dk;
+            float v = 0.0f;
+            if (r < nr) {
+                const int i = (int)a.by_group.div(r0 + r);
+                const long long at = (long long)(q.q0 + i) * a.q_stride + (long long)(h * a.g + (r0 + r - i * a.g)) * a.q_head + d;
+                v = a.q_type == KV_TYPE_F16 ? __half2float(reinterpret_cast<const __half *>(a.q)[at])
+                                            : reinterpret_cast<const float *>(a.q)[at];
+            }
+            qs[e] = v;
+        }
+        __syncthreads();
+        float m[RB], l[RB], o[RB][DV_LANES];
+#pragma unroll
+        for (int r = 0; r < RB; r++) {
+            m[r] = -INFINITY;
+            l[r] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < DV_LANES; c++) o[r][c] = 0.0f;
+        }
+        int last = q.ln;                                 // keys behind every row of the block are not read
+        if (a.cu_k && a.causal) {
+            const long long see = (long long)a.by_group.div(r0 + nr - 1) + (q.ln - q.nq) + 1;
+            last = (int)max(0LL, min((long long)q.ln, see));
+        }
+        for (int t = lo; t < hi; t++) {
+            const int j0 = t * TILE + warp * WK;
+            if (j0 >= last) continue;
+            const int j = j0 + lane;
+            int page = 0, off = 0;
+            const long long row = j < last ? attn_row(a, q, j, &page, &off) : -1;
+            float bias = 0.0f;
+            if (row >= 0 && a.beta) bias = a.beta[((size_t)page * a.Hkv + h) * a.page + off];
+            const bool there = row >= 0 && bias != -INFINITY;
+            const unsigned live = __ballot_sync(~0u, there);
+            if (!live) continue;
+            for (int k = 0; k < WK; k++) {
+                const long long rk = __shfl_sync(~0u, row, k);
+                const bool ok = (live >> k) & 1u;
+                const uint8_t * p = a.K + (ok ? rk : 0) * a.k_rb + (long long)h * a.k_hb;
+                for (int d = lane; d < a.dk; d += 32) buf[k * pitch + d] = ok ? attn_elem(p, a.k_type, d) : 0.0f;
+            }
+            __syncwarp();
+            float x[RB];
+#pragma unroll
+            for (int r = 0; r < RB; r++) x[r] = 0.0f;
+            for (int d = 0; d < a.dk; d++) {
+                const float kv = buf[lane * pitch + d];
+#pragma unroll
+                for (int r = 0; r < RB; r++) x[r] = fmaf(qs[r * a.dk + d], kv, x[r]);
+            }
+            __syncwarp();
+            for (int k = 0; k < WK; k++) {
+                const long long rk = __shfl_sync(~0u, row, k);
+                const bool ok = (live >> k) & 1u;
+                const uint8_t * p = a.V + (ok ? rk : 0) * a.v_rb + (long long)h * a.v_hb;
+                for (int d = lane; d < a.dv; d += 32) buf[k * pitch + d] = ok ? attn_elem(p, a.v_type, d) : 0.0f;
+            }
+#pragma unroll
+            for (int r = 0; r < RB; r++) {
+                const bool sees = there && r < nr && attn_sees(a, q, (int)a.by_group.div(r0 + r), j);
+                const float xr = sees ? fmaf(x[r], a.scale, bias) : -INFINITY;
+                float mt = xr;
+#pragma unroll
+                for (int o2 = 16; o2; o2 >>= 1) mt = fmaxf(mt, __shfl_xor_sync(~0u, mt, o2));
+                const float mn = fmaxf(m[r], mt);
+                const float base = mn == -INFINITY ? 0.0f : mn;
+                const float p = sees ? expf(xr - base) : 0.0f;
+                const float f = expf(m[r] - base);       // m = -inf: 0
+                m[r] = mn;
+                l[r] = l[r] * f + p;                     // per lane; summed over the lanes at the end
+#pragma unroll
+                for (int c = 0; c < DV_LANES; c++) o[r][c] *= f;
+                ps[r * WK + lane] = p;
+            }
+            __syncwarp();
+            for (int k = 0; k < WK; k++) {
+                float v[DV_LANES];
+#pragma unroll
+                for (int c = 0; c < DV_LANES; c++) v[c] = lane + 32 * c < a.dv ? buf[k * pitch + lane + 32 * c] : 0.0f;
+#pragma unroll
+                for (int r = 0; r < RB; r++) {
+                    const float p = ps[r * WK + k];
+                    if (p != 0.0f) {                     // a hidden row's V may be anything
+#pragma unroll
+                        for (int c = 0; c < DV_LANES; c++) o[r][c] = fmaf(p, v[c], o[r][c]);
+                    }
+                }
+            }
+            __syncwarp();
+        }
+        // join the warps
+#pragma unroll
+        for (int r = 0; r < RB; r++)
+#pragma unroll
+            for (int o2 = 16; o2; o2 >>= 1) l[r] += __shfl_xor_sync(~0u, l[r], o2);
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < RB; r++) {
+            if (lane == 0) {
+                s_m[warp][r] = m[r];
+                s_l[warp][r] = l[r];
+            }
+#pragma unroll
+            for (int c = 0; c < DV_LANES; c++)
+                if (lane + 32 * c < a.dv) joinO[((size_t)warp * RB + r) * a.dv + lane + 32 * c] = o[r][c];
+        }
+        __syncthreads();
+        float * part = slot >= 0 ? attn_part<RB>(a, qb, h, w, slot) : nullptr;
+        for (int e = threadIdx.x; e < nr * a.dv; e += THREADS) {
+            const int r = e / a.dv, d = e - r * a.dv;
+            float M = -INFINITY;
+            for (int u = 0; u < WARPS; u++) M = fmaxf(M, s_m[u][r]);
+            const float base = M == -INFINITY ? 0.0f : M;
+            float L = 0.0f, O = 0.0f;
+            for (int u = 0; u < WARPS; u++) {
+                const float f = expf(s_m[u][r] - base);
+                L = fmaf(f, s_l[u][r], L);
+                O = fmaf(f, joinO[((size_t)u * RB + r) * a.dv + d], O);
+            }
+            if (part) {
+                part[r * a.dv + d] = O;
+                if (d == 0) {
+                    part[RB * a.dv + r] = M;
+                    part[RB * a.dv + RB + r] = L;
+                }
+            } else {
+                const int i = (int)a.by_group.div(r0 + r);
+                const size_t row = (size_t)(q.q0 + i) * a.Hq + h * a.g + (r0 + r - i * a.g);
+                const float v = L > 0.0f ? O / L : (L == 0.0f ? 0.0f : L);
+                if (a.q_type == KV_TYPE_F16) reinterpret_cast<__half *>(a.out)[row * a.dv + d] = __float2half_rn(v);
+                else reinterpret_cast<float *>(a.out)[row * a.dv + d] = v;
+                if (d == 0 && a.lse) a.lse[row] = L == 0.0f ? -INFINITY : M + logf(L);
+            }
+        }
+    });
+    __syncthreads();
+    }
+}
+
+// One warp per (token, query head): the rows whose keys were split over
+// several workers, joined in the workers' order, and rows of sequences
+// without keys. Sequences that one worker covered are written already.
+template <int RBJ, int TILEJ>
+__global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ kvc_attn_args a) {
+    const int lane = threadIdx.x & 31;
+    const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int token = (int)(unit / a.Hq), hq = (int)(unit - (long long)token * a.Hq);
+    if (token >= a.n_total) return;
+    // the sequence of the token (the last one whose rows start at or before it)
+    int s = -1;
+    for (int s0 = 0; s0 < a.n_seqs && s < 0; s0 += 32) {
+        bool in = false;
+        if (s0 + lane < a.n_seqs) {
+            const int q0 = min(max(a.cu_q[s0 + lane], 0), a.n_total), q1 = min(max(a.cu_q[s0 + lane + 1], q0), a.n_total);
+            in = token >= q0 && token < q1;
+        }
+        const unsigned b = __ballot_sync(~0u, in);
+        if (b) s = s0 + __ffs(b) - 1;
+    }
+    if (s < 0) return;
+    const kvc_attn_seq q = attn_seq(a, s);
+    const int i = token - q.q0;
+    if (i >= q.nq) return;
+    const int h = hq / a.g;
+    const int rho = i * a.g + (hq - h * a.g);
+    const int qb = rho / RBJ, r = rho - qb * RBJ;
+    long long before = 0, T = 0;
+    for (int u = lane; u < a.n_seqs; u += 32) {
+        const int t = attn_tiles<RBJ, TILEJ>(a, u, qb);
+        T += t;
+        if (u < s) before += t;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        T += __shfl_xor_sync(~0u, T, o);
+        before += __shfl_xor_sync(~0u, before, o);
+    }
+    const int tiles = attn_tiles<RBJ, TILEJ>(a, s, qb);
+    const size_t row = (size_t)token * a.Hq + hq;
+    if (tiles == 0) {
+        for (int d = lane; d < a.dv; d += 32) {
+            if (a.q_type == KV_TYPE_F16) reinterpret_cast<__half *>(a.out)[row * a.dv + d] = __float2half_rn(0.0f);
+            else reinterpret_cast<float *>(a.out)[row * a.dv + d] = 0.0f;
+        }
+        if (lane == 0 && a.lse) a.lse[row] = -INFINITY;
+        return;
+    }
+    const int w0 = attn_worker(before, T, a.W), w1 = attn_worker(before + tiles - 1, T, a.W);
+    if (w0 == w1) return;
+    float M = -INFINITY;
+    for (int w = w0 + lane; w <= w1; w += 32) {
+        const int slot = (long long)w * T / a.W > before ? 0 : 1;
+        M = fmaxf(M, attn_part<RBJ>(a, qb, h, w, slot)[RBJ * a.dv + r]);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, o));
+    const float base = M == -INFINITY ? 0.0f : M;
+    float L = 0.0f, O[8];
+#pragma unroll
+    for (int c = 0; c < 8; c++) O[c] = 0.0f;
+    for (int w = w0; w <= w1; w++) {
+        const int slot = (long long)w * T / a.W > before ? 0 : 1;
+        const float * p = attn_part<RBJ>(a, qb, h, w, slot);
+        const float f = expf(p[RBJ * a.dv + r] - base);
+        L = fmaf(f, p[RBJ * a.dv + RBJ + r], L);
+#pragma unroll
+        for (int c = 0; c < 8; c++)
+            if (lane + 32 * c < a.dv) O[c] = fmaf(f, p[r * a.dv + lane + 32 * c], O[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < 8; c++) {
+        const int d = lane + 32 * c;
+        if (d < a.dv) {
+            const float v = L > 0.0f ? O[c] / L : (L == 0.0f ? 0.0f : L);
+            if (a.q_type == KV_TYPE_F16) reinterpret_cast<__half *>(a.out)[row * a.dv + d] = __float2half_rn(v);
+            else reinterpret_cast<float *>(a.out)[row * a.dv + d] = v;
+        }
+    }
+    if (lane == 0 && a.lse) a.lse[row] = L == 0.0f ? -INFINITY : M + logf(L);
+}
+
+size_t simt_smem(int dk, int dv) {
+    const int pitch = (dk > dv ? dk : dv) | 1;
+    return (size_t)(RB * dk + WARPS * RB * WK + WARPS * WK * pitch) * sizeof(float);
+}
+
+template <int C>
+int launch_simt(const kvc_attn_args & a, dim3 grid, cudaStream_t st) {
+    const size_t sm = simt_smem(a.dk, a.dv);
+    KVC_CUDA(cudaFuncSetAttribute(k_attn_simt<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm));
+    k_attn_simt<C><<<grid, THREADS, sm, st>>>(a);
+    g_serve_launches++;
+    KVC_CUDA(cudaGetLastError());
+    return KVC_OK;
+}
+
+template <int RBJ, int TILEJ>
+int launch_join(const kvc_attn_args & a, cudaStream_t st) {
+    const long long units = (long long)a.n_total * a.Hq;
+    if (units == 0) return KVC_OK;
+    k_attn_join<RBJ, TILEJ><<<(unsigned)((units + 3) / 4), 128, 0, st>>>(a);
+    g_serve_launches++;
+    KVC_CUDA(cudaGetLastError());
+    return KVC_OK;
+}
+
+}  // namespace
+
+int kvc_attn_simt_workers(const kvc_attn_args & a, int sms) {
+    // enough CTAs for four waves' worth of two per SM
+    const long long blocks = ((long long)a.max_q * a.g + RB - 1) / RB * a.Hkv;
+    const long long w = (8LL * sms + blocks - 1) / (blocks > 0 ? blocks : 1);
+    return (int)(w < 1 ? 1 : w);
+}
+
+int kvc_launch_attn_simt(const kvc_attn_args & a, cudaStream_t st) {
+    const long long blocks = ((long long)a.max_q * a.g + RB - 1) / RB;
+    if (blocks <= 0 || a.n_seqs == 0 || a.n_total == 0) return KVC_OK;
+    const long long cap = 65535 / a.Hkv;
+    const dim3 grid((unsigned)a.W, (unsigned)((blocks < cap ? blocks : cap) * a.Hkv));
+    int rc;
+    if (a.dv <= 64) rc = launch_simt<2>(a, grid, st);
+    else if (a.dv <= 128) rc = launch_simt<4>(a, grid, st);
+    else rc = launch_simt<8>(a, grid, st);
+    return rc ? rc : kvc_launch_attn_join(a, RB, TILE, st);
+}
+
+int kvc_launch_attn_join(const kvc_attn_args & a, int rb, int tile, cudaStream_t st) {
+    if (rb == 8 && tile == 128) return launch_join<8, 128>(a, st);
+    return KVC_ERR_SHAPE;
+}

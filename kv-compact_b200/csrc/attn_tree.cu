@@ -1,0 +1,108 @@
+// attn_tree.cu — attention of drafted tokens over the paged cache
+// (include/kvc-attn.h): argument checks and the choice of kernel.
+#include "attn.h"
+
+#include <limits.h>
+
+namespace {
+
+struct tree_plan {
+    kvc_attn_args a;
+    size_t bytes;
+};
+
+int head_bytes(int type, int d) {
+    return type == KV_TYPE_F32 ? 4 * d : type == KV_TYPE_F16 ? 2 * d : d / 32 * kvc_block_bytes(type);
+}
+
+int make_plan(const kvc_page_cache * c, const kvc_tree_desc * t, int sms, tree_plan * p) {
+    int rc = kvc_check_cache(c);
+    if (rc) return rc;
+    if (!t) return KVC_ERR_NULL;
+    if (t->n_seqs < 0 || t->total < 0 || t->max_nodes < 0 || t->n_head <= 0 || t->mask_words < 0 || t->layer < 0 ||
+        t->layer >= c->n_layers || t->n_head % c->n_head_kv != 0)
+        return KVC_ERR_DIMS;
+    if (t->q_type != KV_TYPE_F16 && t->q_type != KV_TYPE_F32) return KVC_ERR_DIMS;
+    if (t->n_seqs > 0 && t->total > 0 && (!t->q || !t->out || !t->cu || !t->seqs)) return KVC_ERR_NULL;
+    if (t->q_stride < (long long)t->n_head * c->d_k) return KVC_ERR_DIMS;
+    if (c->d_k > KVC_MAX_D || c->d_v > KVC_MAX_D) return KVC_ERR_SHAPE;
+    // a head's part of a row is whole blocks
+    for (int i = 0; i < 2; i++) {
+        const int type = i ? c->v_type : c->k_type, d = i ? c->d_v : c->d_k;
+        if (type != KV_TYPE_F32 && type != KV_TYPE_F16 && d % 32 != 0) return KVC_ERR_SHAPE;
+    }
+    const uintptr_t qa = t->q_type == KV_TYPE_F32 ? 3 : 1;
+    if (((uintptr_t)t->q & qa) || ((uintptr_t)t->out & qa)) return KVC_ERR_SHAPE;
+    if ((long long)t->total * t->n_head > INT_MAX || (long long)t->max_nodes * t->n_head > INT_MAX) return KVC_ERR_SHAPE;
+    kvc_attn_args & a = p->a;
+    a = kvc_attn_args{};
+    a.q = t->q;
+    a.out = t->out;
+    a.lse = t->lse;
+    a.q_stride = t->q_stride;
+    a.q_head = c->d_k;
+    a.cu_q = t->cu;
+    a.q_type = t->q_type;
+    a.n_seqs = t->n_seqs;
+    a.n_total = t->total;
+    a.max_q = t->max_nodes;
+    a.Hq = t->n_head;
+    a.Hkv = c->n_head_kv;
+    a.g = t->n_head / c->n_head_kv;
+    a.dk = c->d_k;
+    a.dv = c->d_v;
+    a.scale = t->scale;
+    const size_t rows = (size_t)c->n_pages * c->page_size;
+    a.K = c->K + (size_t)t->layer * rows * c->k_row_bytes;
+    a.V = c->V + (size_t)t->layer * rows * c->v_row_bytes;
+    a.k_rb = (long long)c->k_row_bytes;
+    a.v_rb = (long long)c->v_row_bytes;
+    a.k_hb = head_bytes(c->k_type, c->d_k);
+    a.v_hb = head_bytes(c->v_type, c->d_v);
+    a.k_type = c->k_type;
+    a.v_type = c->v_type;
+    a.seqs = t->seqs;
+    a.table = c->page_table;
+    a.seq_len = c->seq_len;
+    a.beta = c->beta ? c->beta + (size_t)t->layer * rows * c->n_head_kv : nullptr;
+    a.mask = t->mask;
+    a.mask_words = t->mask_words;
+    a.n_slots = c->n_slots;
+    a.n_pages = c->n_pages;
+    a.max_pages = c->max_pages;
+    a.page = c->page_size;
+    a.by_page = kvc_make_divisor((uint32_t)c->page_size);
+    a.by_group = kvc_make_divisor((uint32_t)a.g);
+    a.W = kvc_attn_simt_workers(a, sms);
+    const long long blocks = ((long long)a.max_q * a.g + KVC_SIMT_RB - 1) / KVC_SIMT_RB * a.Hkv;
+    p->bytes = kvc_attn_part_bytes(KVC_SIMT_RB, blocks, a.W, a.dv);
+    return KVC_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+KVC_EXPORT size_t kvc_attn_tree_workspace(const kvc_page_cache * cache, const kvc_tree_desc * desc, int * rc) {
+    tree_plan p;
+    int sms = kvc_serve_device();
+    int r = sms < 0 ? sms : make_plan(cache, desc, sms, &p);
+    if (rc) *rc = r;
+    return r ? 0 : p.bytes;
+}
+
+KVC_EXPORT int kvc_attn_tree(const kvc_page_cache * cache, const kvc_tree_desc * desc, void * workspace,
+                             size_t workspace_bytes, void * stream) {
+    tree_plan p;
+    const int sms = kvc_serve_device();
+    const int rc = make_plan(cache, desc, sms < 0 ? 1 : sms, &p);
+    if (rc) return rc;
+    if (sms < 0) return sms;
+    if (desc->n_seqs == 0 || desc->total == 0 || desc->max_nodes == 0) return KVC_OK;
+    if (p.bytes && !workspace) return KVC_ERR_NULL;
+    if (p.bytes > workspace_bytes || ((uintptr_t)workspace & 15)) return KVC_ERR_SHAPE;
+    p.a.part = static_cast<float *>(workspace);
+    return kvc_launch_attn_simt(p.a, (cudaStream_t)stream);
+}
+
+}  // extern "C"

@@ -8,6 +8,7 @@
 
 #include "../../include/kvc-batched.h"
 #include "engine.h"
+#include "serve.h"
 
 namespace {
 enum { SLOT_BATCH_KV = 3, SLOT_BATCH_IO = 5 };
@@ -41,7 +42,7 @@ extern "C" {
 KVC_EXPORT uint64_t kvc_launch_count(void) {
     int rc;
     kvc_ctx * ctx = kvc_get_ctx(&rc);
-    return ctx ? ctx->launches : 0;
+    return ctx ? ctx->launches + g_serve_launches.load() : 0;
 }
 
 KVC_EXPORT int kvc_profile(int enable, double * stage_ms, uint64_t * stage_launches, int n) {

@@ -1,0 +1,701 @@
+// pages.cu — the paged cache's operations (include/kvc-pages.h).
+//
+// A call that changes tables runs as three small launches: k_plan (one CTA:
+// per entry how many pages are shared and how many are new, then the lowest
+// free pages, found by scanning ref_count in order), k_move_rows (the row
+// copies of all layers, from the old table to the new pages) and k_commit
+// (tables, reference counts, lengths). The copies read the old table and only
+// write pages that were free, and k_commit runs after them, so no step can
+// see a half-made table; the counts change by integer additions, whose order
+// does not matter.
+#include "serve.h"
+
+#include "kv-compact-api.h"
+
+#include <limits.h>
+#include <stdlib.h>
+
+#include <initializer_list>
+
+std::atomic<uint64_t> g_serve_launches{0};
+
+int kvc_serve_device() {
+    static std::atomic<int> known[64];               // 0 unknown, else SM count + 1
+    const char * e = getenv("KVC_FAULT_INJECT");
+    if (e && strcmp(e, "nodev") == 0) return KVC_ERR_NODEV;
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+        cudaGetLastError();
+        return KVC_ERR_NODEV;
+    }
+    int v = known[dev].load(std::memory_order_relaxed);
+    if (v == 0) {
+        int major = 0, sms = 0;
+        if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess ||
+            cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || major < 10 || sms <= 0) {
+            cudaGetLastError();
+            fprintf(stderr, "[kvc] device %d cannot run sm_100a kernels\n", dev);
+            return KVC_ERR_NODEV;
+        }
+        v = sms + 1;
+        known[dev].store(v, std::memory_order_relaxed);
+    }
+    return v - 1;
+}
+
+int kvc_check_cache(const kvc_page_cache * c) {
+    if (!c || !c->K || !c->V || !c->page_table || !c->seq_len || !c->ref_count || !c->status) return KVC_ERR_NULL;
+    if (c->n_layers <= 0 || c->n_pages <= 0 || c->page_size <= 0 || c->n_slots <= 0 || c->max_pages <= 0 ||
+        c->n_head_kv <= 0 || c->d_k <= 0 || c->d_v <= 0)
+        return KVC_ERR_DIMS;
+    for (int t : {c->k_type, c->v_type})
+        if (t != KV_TYPE_F32 && t != KV_TYPE_F16 && t != KV_TYPE_Q4_0 && t != KV_TYPE_Q4_1 && t != KV_TYPE_Q8_0)
+            return KVC_ERR_DIMS;
+    if (c->n_layers > 65535 || c->n_head_kv > 65535) return KVC_ERR_SHAPE;
+    const long long ek = (long long)c->n_head_kv * c->d_k, ev = (long long)c->n_head_kv * c->d_v;
+    if (ek > INT_MAX / 4 || ev > INT_MAX / 4 || c->k_row_bytes > INT_MAX || c->v_row_bytes > INT_MAX) return KVC_ERR_SHAPE;
+    if (kvc_row_elements(c->k_type, c->k_row_bytes) != ek || kvc_row_bytes(c->k_type, (int)ek) != c->k_row_bytes ||
+        kvc_row_elements(c->v_type, c->v_row_bytes) != ev || kvc_row_bytes(c->v_type, (int)ev) != c->v_row_bytes)
+        return KVC_ERR_ROWSIZE;
+    // row numbers of the pool and of a sequence are 32-bit
+    if ((long long)c->n_pages * c->page_size > INT_MAX || (long long)c->max_pages * c->page_size > INT_MAX)
+        return KVC_ERR_SHAPE;
+    // the widest element of the type decides how rows may be addressed
+    const uintptr_t ka = c->k_type == KV_TYPE_F32 ? 4 : 2, va = c->v_type == KV_TYPE_F32 ? 4 : 2;
+    if ((uintptr_t)c->K % ka || (uintptr_t)c->V % va) return KVC_ERR_SHAPE;
+    return KVC_OK;
+}
+
+namespace {
+
+enum { OP_RESERVE, OP_FORK, OP_COMPACT, OP_FREE };
+
+// One entry of a planned call, as k_plan leaves it in the workspace.
+struct plan_item {
+    int whole;     // leading table entries of src that are shared
+    int need;      // new pages
+    int first;     // index of the first of them in the list of new pages
+    int length;    // rows of dst afterwards
+    int head;      // rows of src's page `whole` that go to the first new page
+    int kept;      // rows that the keep list adds
+};
+
+struct plan_ids {
+    int n;
+    int src[KVC_PAGES_MAX_SEQS];
+    int dst[KVC_PAGES_MAX_SEQS];
+};
+
+// Workspace: [0] 1 when the call may go on, then the items, then the new pages.
+constexpr size_t WS_HEAD = 256;
+constexpr size_t WS_ITEMS = WS_HEAD + KVC_PAGES_MAX_SEQS * sizeof(plan_item);
+
+struct cache_dev {
+    uint8_t * K;
+    uint8_t * V;
+    float * beta;
+    int * table;
+    int * seq_len;
+    int * ref;
+    int * status;
+    int n_layers, n_pages, page, max_pages, H;
+    kvc_divisor by_page;
+};
+
+cache_dev on_device(const kvc_page_cache * c) {
+    return {c->K,        c->V,       c->beta,      c->page_table, c->seq_len,
+            c->ref_count, c->status, c->n_layers,  c->n_pages,    c->page_size,
+            c->max_pages, c->n_head_kv, kvc_make_divisor((uint32_t)c->page_size)};
+}
+
+constexpr int PLAN_THREADS = 1024;
+constexpr int PLAN_PER = 16;          // counts per thread and scan step
+
+__device__ __forceinline__ int warp_scan(int v, int lane) {          // inclusive
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(~0u, v, o);
+        if (lane >= o) v += u;
+    }
+    return v;
+}
+
+// Exclusive scan over the CTA; every thread gets its prefix and the total.
+__device__ int block_scan(int v, int * sums, int * total) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int inc = warp_scan(v, lane);
+    __syncthreads();
+    if (lane == 31) sums[w] = inc;
+    __syncthreads();
+    if (w == 0) sums[lane] = warp_scan(sums[lane], lane);
+    __syncthreads();
+    *total = sums[31];
+    return inc - v + (w ? sums[w - 1] : 0);
+}
+
+// One CTA. Bound by latency: one pass over the entries, then the scan for free
+// pages, 16 counts per thread and step (four 16-byte loads in flight), which
+// stops as soon as enough were found.
+__global__ void __launch_bounds__(PLAN_THREADS) k_plan(cache_dev c, const __grid_constant__ plan_ids ids, int op,
+                                                       const int * __restrict__ base, const int * __restrict__ keep_n,
+                                                       const __grid_constant__ plan_ids counts, int keep_ld,
+                                                       int * __restrict__ ws) {
+    __shared__ int sums[32];
+    __shared__ int bad;
+    const int t = threadIdx.x;
+    if (t == 0) bad = 0;
+    plan_item it{};
+    if (t < ids.n) {
+        const int cap = c.max_pages * c.page;
+        const int len = min(max(c.seq_len[ids.src[t]], 0), cap);
+        long long length = len;
+        if (op == OP_RESERVE) {
+            it.whole = (len + c.page - 1) / c.page;
+            length = (long long)len + counts.src[t];
+        } else if (op == OP_FORK) {
+            it.whole = len / c.page;
+            it.head = len - it.whole * c.page;
+        } else {
+            const int b = min(max(base[t], 0), len);
+            it.kept = min(max(keep_n[t], 0), keep_ld);
+            it.whole = b / c.page;
+            it.head = b - it.whole * c.page;
+            length = (long long)b + it.kept;
+        }
+        if (length > cap) {
+            atomicOr(&bad, 1);
+        } else {
+            it.length = (int)length;
+            it.need = max((it.length + c.page - 1) / c.page - it.whole, 0);
+        }
+    }
+    int total;
+    it.first = block_scan(t < ids.n ? it.need : 0, sums, &total);
+    plan_item * items = reinterpret_cast<plan_item *>(reinterpret_cast<char *>(ws) + WS_HEAD);
+    if (t < ids.n) items[t] = it;
+    int * fresh = reinterpret_cast<int *>(reinterpret_cast<char *>(ws) + WS_ITEMS);
+    int found = 0;
+    __syncthreads();
+    const bool too_long = bad != 0;
+    if (!too_long) {
+        const bool wide = ((uintptr_t)c.ref & 15) == 0;
+        for (int at = 0; found < total && at < c.n_pages; at += PLAN_THREADS * PLAN_PER) {
+            const int p0 = at + t * PLAN_PER;
+            unsigned free_bits = 0;
+            if (wide && p0 + PLAN_PER <= c.n_pages) {
+                int4 r[PLAN_PER / 4];
+#pragma unroll
+                for (int i = 0; i < PLAN_PER / 4; i++) r[i] = reinterpret_cast<const int4 *>(c.ref + p0)[i];
+#pragma unroll
+                for (int i = 0; i < PLAN_PER / 4; i++) {
+                    free_bits |= (r[i].x == 0 ? 1u : 0u) << (4 * i);
+                    free_bits |= (r[i].y == 0 ? 2u : 0u) << (4 * i);
+                    free_bits |= (r[i].z == 0 ? 4u : 0u) << (4 * i);
+                    free_bits |= (r[i].w == 0 ? 8u : 0u) << (4 * i);
+                }
+            } else {
+                for (int i = 0; i < PLAN_PER; i++)
+                    if (p0 + i < c.n_pages && c.ref[p0 + i] == 0) free_bits |= 1u << i;
+            }
+            int step;
+            int k = found + block_scan(__popc(free_bits), sums, &step);
+            while (free_bits && k < total) {
+                const int i = __ffs(free_bits) - 1;
+                free_bits &= free_bits - 1;
+                fresh[k++] = p0 + i;
+            }
+            found += step;
+        }
+    }
+    if (t == 0) {
+        const bool ok = !too_long && found >= total;
+        ws[0] = ok;
+        if (!ok) *c.status = too_long ? KVC_ERR_SHAPE : KVC_ERR_OOM;
+    }
+}
+
+// Table entries, counts and lengths of every entry; one thread per entry of a
+// table row. Entry (dst, col) is read and written by its own thread alone, and
+// a source row is nobody's destination but its own, so nothing races.
+__global__ void __launch_bounds__(256) k_commit(cache_dev c, const __grid_constant__ plan_ids ids, int op,
+                                                const int * __restrict__ ws) {
+    const int i = blockIdx.y;
+    if (op != OP_FREE && ws[0] == 0) return;
+    const int col = blockIdx.x * 256 + threadIdx.x;
+    plan_item it{};
+    if (op != OP_FREE) it = reinterpret_cast<const plan_item *>(reinterpret_cast<const char *>(ws) + WS_HEAD)[i];
+    if (col == 0) c.seq_len[ids.dst[i]] = it.length;
+    if (col >= c.max_pages) return;
+    const int * fresh = reinterpret_cast<const int *>(reinterpret_cast<const char *>(ws) + WS_ITEMS);
+    int * at = c.table + (size_t)ids.dst[i] * c.max_pages + col;
+    const int old = *at;
+    int now = -1;
+    if (col < it.whole) now = c.table[(size_t)ids.src[i] * c.max_pages + col];
+    else if (col < it.whole + it.need) now = fresh[it.first + col - it.whole];
+    if (old == now) return;
+    if (old >= 0 && old < c.n_pages) atomicAdd(c.ref + old, -1);
+    if (now >= 0 && now < c.n_pages) atomicAdd(c.ref + now, 1);
+    *at = now;
+}
+
+// ---- row movement -----------------------------------------------------------
+//
+// A CTA moves MOVE_ROWS rows of one layer: their places are looked up once
+// into shared memory, then all threads copy the K bytes and the V bytes in
+// the widest pieces that the row sizes and base addresses allow (16 bytes for
+// the common shapes), MOVE_DEPTH loads in flight per thread. Bound by HBM.
+constexpr int MOVE_ROWS = 32;
+constexpr int MOVE_THREADS = 256;
+constexpr int MOVE_DEPTH = 4;
+
+enum { MV_PAGES, MV_FORK, MV_COMPACT, MV_WRITE, MV_READ };
+
+struct move_args {
+    cache_dev c;
+    int mode;
+    long long krb, vrb;             // bytes per row
+    int rows;                       // rows per entry (MV_PAGES, MV_FORK, MV_COMPACT) or in all (MV_WRITE / MV_READ)
+    kvc_divisor kdiv, vdiv;         // pieces per row
+    const int * ws;
+    const int * src_pages;          // MV_PAGES
+    const int * dst_pages;
+    const int * keep;               // MV_COMPACT
+    int keep_ld;
+    long long keep_layer;
+    int n;
+    uint8_t * k_rows;               // packed rows (MV_WRITE / MV_READ), or replacements (MV_COMPACT: V and beta)
+    uint8_t * v_rows;
+    float * b_rows;
+};
+
+template <typename T>
+__device__ __forceinline__ void copy_pieces(const long long * src, const long long * dst, const uint8_t * from,
+                                            uint8_t * to, kvc_divisor per, long long rb, int rows) {
+    const uint32_t n = (uint32_t)rows * per.d;
+    for (uint32_t p0 = threadIdx.x; p0 < n; p0 += MOVE_THREADS * MOVE_DEPTH) {
+        T v[MOVE_DEPTH];
+        long long out[MOVE_DEPTH];
+#pragma unroll
+        for (int i = 0; i < MOVE_DEPTH; i++) {
+            const uint32_t p = p0 + i * MOVE_THREADS;
+            out[i] = -1;
+            if (p < n) {
+                const uint32_t r = per.div(p), q = p - r * per.d;
+                if (src[r] >= 0 && dst[r] >= 0) {
+                    v[i] = *reinterpret_cast<const T *>(from + src[r] * rb + (long long)q * sizeof(T));
+                    out[i] = dst[r] * rb + (long long)q * sizeof(T);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < MOVE_DEPTH; i++)
+            if (out[i] >= 0) *reinterpret_cast<T *>(to + out[i]) = v[i];
+    }
+}
+
+// Row numbers count rows of one layer's pool, or of a packed array; -1 = none.
+template <typename TK, typename TV>
+__global__ void __launch_bounds__(MOVE_THREADS) k_move_rows(const __grid_constant__ move_args a,
+                                                            const __grid_constant__ plan_ids ids,
+                                                            const __grid_constant__ plan_ids span) {
+    __shared__ long long s_src[MOVE_ROWS], s_dst[MOVE_ROWS], s_vsrc[MOVE_ROWS];
+    const cache_dev & c = a.c;
+    const int layer = blockIdx.y, item = blockIdx.z;
+    const bool planned = a.mode == MV_FORK || a.mode == MV_COMPACT;
+    if (planned && a.ws[0] == 0) return;
+    const long long pool = (long long)c.n_pages * c.page;
+    plan_item it{};
+    int count = a.rows;
+    if (planned) {
+        it = reinterpret_cast<const plan_item *>(reinterpret_cast<const char *>(a.ws) + WS_HEAD)[item];
+        count = it.head + it.kept;
+    }
+    const int * fresh = reinterpret_cast<const int *>(reinterpret_cast<const char *>(a.ws) + WS_ITEMS);
+    const uint8_t * v_from = c.V + (long long)layer * pool * a.vrb;
+    uint8_t * v_to = c.V + (long long)layer * pool * a.vrb;
+    const uint8_t * k_from = c.K + (long long)layer * pool * a.krb;
+    uint8_t * k_to = c.K + (long long)layer * pool * a.krb;
+    if (a.mode == MV_WRITE) {
+        k_from = a.k_rows + (long long)layer * a.rows * a.krb;
+        v_from = a.v_rows + (long long)layer * a.rows * a.vrb;
+    } else if (a.mode == MV_READ) {
+        k_to = a.k_rows + (long long)layer * a.rows * a.krb;
+        v_to = a.v_rows + (long long)layer * a.rows * a.vrb;
+    }
+    const bool new_v = a.mode == MV_COMPACT && a.v_rows != nullptr;
+    const uint8_t * new_v_from = new_v ? a.v_rows + ((long long)layer * a.n + item) * a.keep_ld * a.vrb : nullptr;
+    for (long long j0 = (long long)blockIdx.x * MOVE_ROWS; j0 < count; j0 += (long long)gridDim.x * MOVE_ROWS) {
+        const int rows = (int)min((long long)MOVE_ROWS, count - j0);
+        __syncthreads();
+        if (threadIdx.x < rows) {
+            const int j = (int)j0 + threadIdx.x;
+            long long src = -1, dst = -1, vsrc;
+            bool replaced = false;
+            if (a.mode == MV_PAGES) {
+                const int e = (int)c.by_page.div(j), off = j - e * c.page;
+                const int ps = a.src_pages[e], pd = a.dst_pages[e];
+                if (ps >= 0 && ps < c.n_pages && pd >= 0 && pd < c.n_pages && ps != pd) {
+                    src = (long long)ps * c.page + off;
+                    dst = (long long)pd * c.page + off;
+                }
+                vsrc = src;
+            } else if (planned) {
+                const int * table = c.table + (size_t)ids.src[item] * c.max_pages;
+                int row;
+                if (j < it.head) {
+                    row = it.whole * c.page + j;
+                } else {
+                    row = a.keep[(long long)layer * a.keep_layer + (long long)item * a.keep_ld + (j - it.head)];
+                    replaced = true;
+                }
+                const int len = min(max(c.seq_len[ids.src[item]], 0), c.max_pages * c.page);
+                if (row >= 0 && row < len) {
+                    const int e = (int)c.by_page.div(row), p = table[e];
+                    if (p >= 0 && p < c.n_pages) src = (long long)p * c.page + (row - e * c.page);
+                }
+                const int e = (int)c.by_page.div(j);
+                dst = (long long)fresh[it.first + e] * c.page + (j - e * c.page);
+                vsrc = src;
+                if (new_v && replaced && src >= 0) vsrc = -2 - (j - it.head);      // a replacement row
+            } else {
+                // packed rows: the entry that row j belongs to (few entries: a linear walk)
+                int e = 0, at = 0;
+                while (e < ids.n - 1 && j >= at + span.dst[e]) at += span.dst[e++];
+                const int row = span.src[e] + (j - at);
+                const int slot = ids.src[e];
+                const int len = min(max(c.seq_len[slot], 0), c.max_pages * c.page);
+                long long there = -1;
+                if (row < len) {
+                    const int b = (int)c.by_page.div(row), p = c.table[(size_t)slot * c.max_pages + b];
+                    if (p >= 0 && p < c.n_pages) {
+                        there = (long long)p * c.page + (row - b * c.page);
+                        if (a.mode == MV_WRITE && c.ref[p] > 1) {
+                            there = -1;
+                            *c.status = KVC_ERR_DIMS;
+                        }
+                    }
+                }
+                src = a.mode == MV_WRITE ? j : there;
+                dst = a.mode == MV_WRITE ? there : j;
+                vsrc = src;
+            }
+            s_src[threadIdx.x] = src;
+            s_dst[threadIdx.x] = dst;
+            s_vsrc[threadIdx.x] = vsrc;
+        }
+        __syncthreads();
+        if (a.mode < MV_WRITE || a.k_rows) copy_pieces<TK>(s_src, s_dst, k_from, k_to, a.kdiv, a.krb, rows);
+        if (!new_v) {
+            if (a.mode < MV_WRITE || a.v_rows) copy_pieces<TV>(s_src, s_dst, v_from, v_to, a.vdiv, a.vrb, rows);
+        } else {
+            const uint32_t n = (uint32_t)rows * a.vdiv.d;
+            for (uint32_t p0 = threadIdx.x; p0 < n; p0 += MOVE_THREADS * MOVE_DEPTH) {
+                TV v[MOVE_DEPTH];
+                long long out[MOVE_DEPTH];
+#pragma unroll
+                for (int i = 0; i < MOVE_DEPTH; i++) {
+                    const uint32_t p = p0 + i * MOVE_THREADS;
+                    out[i] = -1;
+                    if (p < n) {
+                        const uint32_t r = a.vdiv.div(p), q = p - r * a.vdiv.d;
+                        const long long vs = s_vsrc[r];
+                        if (vs != -1) {
+                            const uint8_t * f = vs >= 0 ? v_from + vs * a.vrb : new_v_from + (-2 - vs) * a.vrb;
+                            v[i] = *reinterpret_cast<const TV *>(f + (long long)q * sizeof(TV));
+                            out[i] = s_dst[r] * a.vrb + (long long)q * sizeof(TV);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < MOVE_DEPTH; i++)
+                    if (out[i] >= 0) *reinterpret_cast<TV *>(v_to + out[i]) = v[i];
+            }
+        }
+        // beta: [page][head][row in page]; neighbouring threads take
+        // neighbouring rows, which lie side by side in a page
+        if (c.beta && (a.mode < MV_WRITE || a.b_rows)) {
+            float * pool_b = c.beta + (long long)layer * pool * c.H;
+            for (int p = threadIdx.x; p < rows * c.H; p += MOVE_THREADS) {
+                const int h = p / rows, r = p - h * rows;
+                const long long src = s_src[r], dst = s_dst[r];
+                if (dst < 0) continue;
+                auto place = [&](long long row) {
+                    const uint32_t pg = c.by_page.div((uint32_t)row);
+                    return ((long long)pg * c.H + h) * c.page + (row - (long long)pg * c.page);
+                };
+                if (a.mode == MV_WRITE) {
+                    pool_b[place(dst)] = a.b_rows[((long long)layer * c.H + h) * a.rows + src];
+                } else if (a.mode == MV_READ) {
+                    if (src >= 0) a.b_rows[((long long)layer * c.H + h) * a.rows + dst] = pool_b[place(src)];
+                } else {
+                    const int kept = (int)(j0 + r) - it.head;
+                    if (src < 0) continue;
+                    if (a.mode == MV_COMPACT && a.b_rows && kept >= 0)
+                        pool_b[place(dst)] = a.b_rows[(((long long)layer * a.n + item) * c.H + h) * a.keep_ld + kept];
+                    else
+                        pool_b[place(dst)] = pool_b[place(src)];
+                }
+            }
+        }
+    }
+}
+
+// The widest piece (16, 8, 4 or 2 bytes) that divides the row size and every base address.
+int piece(size_t rb, std::initializer_list<const void *> bases) {
+    uintptr_t m = rb;
+    for (const void * b : bases) m |= (uintptr_t)b;
+    return (m & 15) == 0 ? 16 : (m & 7) == 0 ? 8 : (m & 3) == 0 ? 4 : (m & 1) == 0 ? 2 : 1;
+}
+
+template <typename TK>
+int launch_move_v(const move_args & a, int vp, const plan_ids & ids, const plan_ids & span, dim3 grid, cudaStream_t st) {
+    switch (vp) {
+    case 16: k_move_rows<TK, int4><<<grid, MOVE_THREADS, 0, st>>>(a, ids, span); break;
+    case 8: k_move_rows<TK, int2><<<grid, MOVE_THREADS, 0, st>>>(a, ids, span); break;
+    case 4: k_move_rows<TK, int><<<grid, MOVE_THREADS, 0, st>>>(a, ids, span); break;
+    case 2: k_move_rows<TK, short><<<grid, MOVE_THREADS, 0, st>>>(a, ids, span); break;
+    default: k_move_rows<TK, char><<<grid, MOVE_THREADS, 0, st>>>(a, ids, span); break;
+    }
+    g_serve_launches++;
+    KVC_CUDA(cudaGetLastError());
+    return KVC_OK;
+}
+
+// most: rows of the longest entry. Enough CTAs to fill the machine several
+// times over, each looping when there are more rows.
+int launch_move(move_args & a, const kvc_page_cache * c, const plan_ids & ids, const plan_ids & span, int items,
+                long long most, int sms, cudaStream_t st) {
+    if (most <= 0 || items <= 0) return KVC_OK;
+    const bool packed = a.mode == MV_WRITE || a.mode == MV_READ;
+    const int kp = piece(c->k_row_bytes, {c->K, packed ? a.k_rows : nullptr});
+    const int vp = piece(c->v_row_bytes, {c->V, a.v_rows});
+    a.krb = (long long)c->k_row_bytes;
+    a.vrb = (long long)c->v_row_bytes;
+    a.kdiv = kvc_make_divisor((uint32_t)(c->k_row_bytes / kp));
+    a.vdiv = kvc_make_divisor((uint32_t)(c->v_row_bytes / vp));
+    const long long tiles = (most + MOVE_ROWS - 1) / MOVE_ROWS;
+    const long long want = (16LL * sms * 8 + (long long)items * c->n_layers - 1) / ((long long)items * c->n_layers);
+    const dim3 grid((unsigned)(tiles < want ? tiles : want), (unsigned)c->n_layers, (unsigned)items);
+    switch (kp) {
+    case 16: return launch_move_v<int4>(a, vp, ids, span, grid, st);
+    case 8: return launch_move_v<int2>(a, vp, ids, span, grid, st);
+    case 4: return launch_move_v<int>(a, vp, ids, span, grid, st);
+    case 2: return launch_move_v<short>(a, vp, ids, span, grid, st);
+    default: return launch_move_v<char>(a, vp, ids, span, grid, st);
+    }
+}
+
+int check_ids(const kvc_page_cache * c, const int * src, const int * dst, int n, plan_ids * ids) {
+    if (n < 0 || n > KVC_PAGES_MAX_SEQS) return KVC_ERR_DIMS;
+    if (n > 0 && (!src || !dst)) return KVC_ERR_NULL;
+    ids->n = n;
+    for (int i = 0; i < n; i++) {
+        if (src[i] < 0 || src[i] >= c->n_slots || dst[i] < 0 || dst[i] >= c->n_slots) return KVC_ERR_DIMS;
+        ids->src[i] = src[i];
+        ids->dst[i] = dst[i];
+    }
+    for (int i = 0; i < n; i++)
+        for (int j = 0; j < n; j++)
+            if (i != j && (dst[i] == dst[j] || dst[i] == src[j])) return KVC_ERR_DIMS;
+    return KVC_OK;
+}
+
+int check_ws(const kvc_page_cache * c, const void * ws, size_t bytes) {
+    if (!ws) return KVC_ERR_NULL;
+    if (bytes < kvc_pages_workspace(c) || ((uintptr_t)ws & 15)) return KVC_ERR_SHAPE;
+    return KVC_OK;
+}
+
+int launch_commit(const cache_dev & c, const plan_ids & ids, int op, const int * ws, cudaStream_t st) {
+    k_commit<<<dim3((c.max_pages + 255) / 256, ids.n), 256, 0, st>>>(c, ids, op, ws);
+    g_serve_launches++;
+    KVC_CUDA(cudaGetLastError());
+    return KVC_OK;
+}
+
+int launch_plan(const cache_dev & c, const plan_ids & ids, int op, const int * base, const int * keep_n,
+                const plan_ids & counts, int keep_ld, int * ws, cudaStream_t st) {
+    k_plan<<<1, PLAN_THREADS, 0, st>>>(c, ids, op, base, keep_n, counts, keep_ld, ws);
+    g_serve_launches++;
+    KVC_CUDA(cudaGetLastError());
+    return KVC_OK;
+}
+
+// Rows of the packed forms: starts and counts of the entries, their sum.
+int check_spans(const kvc_page_cache * c, const int * seqs, const int * first, const int * count, int n, plan_ids * ids,
+                plan_ids * span, long long * total) {
+    if (n < 0 || n > KVC_PAGES_MAX_SEQS) return KVC_ERR_DIMS;
+    if (n > 0 && (!seqs || !first || !count)) return KVC_ERR_NULL;
+    ids->n = span->n = n;
+    *total = 0;
+    for (int i = 0; i < n; i++) {
+        if (seqs[i] < 0 || seqs[i] >= c->n_slots || first[i] < 0 || count[i] < 0 ||
+            (long long)first[i] + count[i] > INT_MAX)
+            return KVC_ERR_DIMS;
+        ids->src[i] = seqs[i];
+        span->src[i] = first[i];
+        span->dst[i] = count[i];
+        *total += count[i];
+    }
+    return *total > INT_MAX - 65536 ? KVC_ERR_SHAPE : KVC_OK;
+}
+
+int packed_move(int mode, const kvc_page_cache * cache, const int * seqs, const int * first, const int * count, int n,
+                uint8_t * k_rows, uint8_t * v_rows, float * b_rows, cudaStream_t st) {
+    int rc = kvc_check_cache(cache);
+    if (rc) return rc;
+    plan_ids ids, span;
+    long long total;
+    if ((rc = check_spans(cache, seqs, first, count, n, &ids, &span, &total))) return rc;
+    if (b_rows && !cache->beta) return KVC_ERR_NULL;
+    if (mode == MV_WRITE)               // two entries that write one row would race
+        for (int i = 0; i < n; i++)
+            for (int j = 0; j < i; j++)
+                if (seqs[i] == seqs[j] && count[i] > 0 && count[j] > 0 && first[i] < first[j] + count[j] &&
+                    first[j] < first[i] + count[i])
+                    return KVC_ERR_DIMS;
+    const int sms = kvc_serve_device();
+    if (sms < 0) return sms;
+    if (!k_rows && !v_rows && !b_rows) return KVC_OK;
+    move_args a{};
+    a.c = on_device(cache);
+    a.mode = mode;
+    a.rows = (int)total;
+    a.k_rows = k_rows;
+    a.v_rows = v_rows;
+    a.b_rows = b_rows;
+    a.n = n;
+    return launch_move(a, cache, ids, span, 1, total, sms, st);
+}
+
+}  // namespace
+
+extern "C" {
+
+KVC_EXPORT size_t kvc_pages_workspace(const kvc_page_cache * cache) {
+    if (kvc_check_cache(cache)) return 0;
+    return (WS_ITEMS + (size_t)cache->n_pages * 4 + 255) & ~(size_t)255;
+}
+
+KVC_EXPORT int kvc_pages_reserve(const kvc_page_cache * cache, const int * seqs, const int * add, int n, void * ws,
+                                 size_t ws_bytes, void * stream) {
+    int rc = kvc_check_cache(cache);
+    if (rc) return rc;
+    plan_ids ids, counts{};
+    if ((rc = check_ids(cache, seqs, seqs, n, &ids))) return rc;
+    if (n > 0 && !add) return KVC_ERR_NULL;
+    for (int i = 0; i < n; i++) {
+        if (add[i] < 0) return KVC_ERR_DIMS;
+        counts.src[i] = add[i];
+    }
+    if ((rc = check_ws(cache, ws, ws_bytes))) return rc;
+    const int sms = kvc_serve_device();
+    if (sms < 0) return sms;
+    if (n == 0) return KVC_OK;
+    const cache_dev c = on_device(cache);
+    if ((rc = launch_plan(c, ids, OP_RESERVE, nullptr, nullptr, counts, 0, (int *)ws, (cudaStream_t)stream))) return rc;
+    return launch_commit(c, ids, OP_RESERVE, (const int *)ws, (cudaStream_t)stream);
+}
+
+KVC_EXPORT int kvc_pages_write(const kvc_page_cache * cache, const int * seqs, const int * first, const int * count,
+                               int n, const uint8_t * k_rows, const uint8_t * v_rows, const float * beta_rows,
+                               void * stream) {
+    return packed_move(MV_WRITE, cache, seqs, first, count, n, const_cast<uint8_t *>(k_rows),
+                       const_cast<uint8_t *>(v_rows), const_cast<float *>(beta_rows), (cudaStream_t)stream);
+}
+
+KVC_EXPORT int kvc_pages_read(const kvc_page_cache * cache, const int * seqs, const int * first, const int * count,
+                              int n, uint8_t * k_rows, uint8_t * v_rows, float * beta_rows, void * stream) {
+    return packed_move(MV_READ, cache, seqs, first, count, n, k_rows, v_rows, beta_rows, (cudaStream_t)stream);
+}
+
+KVC_EXPORT int kvc_pages_copy(const kvc_page_cache * cache, const int * src, const int * dst, int n, void * stream) {
+    int rc = kvc_check_cache(cache);
+    if (rc) return rc;
+    if (n < 0 || (long long)n * cache->page_size > INT_MAX - 65536) return KVC_ERR_DIMS;
+    if (n > 0 && (!src || !dst)) return KVC_ERR_NULL;
+    const int sms = kvc_serve_device();
+    if (sms < 0) return sms;
+    move_args a{};
+    a.c = on_device(cache);
+    a.mode = MV_PAGES;
+    a.rows = n * cache->page_size;
+    a.src_pages = src;
+    a.dst_pages = dst;
+    static const plan_ids none{};
+    return launch_move(a, cache, none, none, 1, a.rows, sms, (cudaStream_t)stream);
+}
+
+KVC_EXPORT int kvc_pages_fork(const kvc_page_cache * cache, const int * src, const int * dst, int n, void * ws,
+                              size_t ws_bytes, void * stream) {
+    int rc = kvc_check_cache(cache);
+    if (rc) return rc;
+    plan_ids ids;
+    if ((rc = check_ids(cache, src, dst, n, &ids))) return rc;
+    for (int i = 0; i < n; i++)
+        if (src[i] == dst[i]) return KVC_ERR_DIMS;
+    if ((rc = check_ws(cache, ws, ws_bytes))) return rc;
+    const int sms = kvc_serve_device();
+    if (sms < 0) return sms;
+    if (n == 0) return KVC_OK;
+    const cache_dev c = on_device(cache);
+    cudaStream_t st = (cudaStream_t)stream;
+    static const plan_ids none{};
+    if ((rc = launch_plan(c, ids, OP_FORK, nullptr, nullptr, none, 0, (int *)ws, st))) return rc;
+    move_args a{};
+    a.c = c;
+    a.mode = MV_FORK;
+    a.n = n;
+    a.ws = (const int *)ws;
+    if ((rc = launch_move(a, cache, ids, none, n, cache->page_size - 1, sms, st))) return rc;
+    return launch_commit(c, ids, OP_FORK, (const int *)ws, st);
+}
+
+KVC_EXPORT int kvc_pages_compact(const kvc_page_cache * cache, const int * src, const int * dst, int n,
+                                 const int * base, const int * keep_n, const int * keep, int keep_ld,
+                                 size_t keep_layer_stride, const uint8_t * v_rows, const float * beta_rows, void * ws,
+                                 size_t ws_bytes, void * stream) {
+    int rc = kvc_check_cache(cache);
+    if (rc) return rc;
+    plan_ids ids;
+    if ((rc = check_ids(cache, src, dst, n, &ids))) return rc;
+    if (keep_ld < 0) return KVC_ERR_DIMS;
+    if (n > 0 && (!base || !keep_n || (!keep && keep_ld > 0))) return KVC_ERR_NULL;
+    if (beta_rows && !cache->beta) return KVC_ERR_NULL;
+    if ((rc = check_ws(cache, ws, ws_bytes))) return rc;
+    const int sms = kvc_serve_device();
+    if (sms < 0) return sms;
+    if (n == 0) return KVC_OK;
+    const cache_dev c = on_device(cache);
+    cudaStream_t st = (cudaStream_t)stream;
+    static const plan_ids none{};
+    if ((rc = launch_plan(c, ids, OP_COMPACT, base, keep_n, none, keep_ld, (int *)ws, st))) return rc;
+    move_args a{};
+    a.c = c;
+    a.mode = MV_COMPACT;
+    a.n = n;
+    a.ws = (const int *)ws;
+    a.keep = keep;
+    a.keep_ld = keep_ld;
+    a.keep_layer = (long long)keep_layer_stride;
+    a.v_rows = const_cast<uint8_t *>(v_rows);
+    a.b_rows = const_cast<float *>(beta_rows);
+    const long long most = (long long)cache->page_size - 1 + keep_ld;
+    if ((rc = launch_move(a, cache, ids, none, n, most, sms, st))) return rc;
+    return launch_commit(c, ids, OP_COMPACT, (const int *)ws, st);
+}
+
+KVC_EXPORT int kvc_pages_free(const kvc_page_cache * cache, const int * seqs, int n, void * ws, size_t ws_bytes,
+                              void * stream) {
+    int rc = kvc_check_cache(cache);
+    if (rc) return rc;
+    plan_ids ids;
+    if ((rc = check_ids(cache, seqs, seqs, n, &ids))) return rc;
+    if ((rc = check_ws(cache, ws, ws_bytes))) return rc;
+    const int sms = kvc_serve_device();
+    if (sms < 0) return sms;
+    if (n == 0) return KVC_OK;
+    return launch_commit(on_device(cache), ids, OP_FREE, (const int *)ws, (cudaStream_t)stream);
+}
+
+}  // extern "C"

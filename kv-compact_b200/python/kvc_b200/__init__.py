@@ -3,6 +3,8 @@
 ``abi``       ctypes mirror of the drop-in C ABI (include/kv-compact-api.h)
 ``lib``       loader for libkvc.so and wrappers over its entry points
 ``workloads`` seeded synthetic caches for the benchmark configurations
+``pages``     paged cache of stored rows (include/kvc-pages.h)
+``attn``      attention over prompts and paged caches (include/kvc-attn.h)
 """
 import os
 

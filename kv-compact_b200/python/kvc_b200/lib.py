@@ -24,6 +24,9 @@ BATCHED_SYMBOLS = ["kvc_plan_layers", "kvc_compact_layers_dev", "kvc_launch_coun
                    "kvc_quantize_rows_dev", "kvc_dequantize_rows_dev"]
 PEER_SYMBOLS = ["kvc_peer_alloc", "kvc_peer_free", "kvc_peer_open", "kvc_peer_close", "kvc_copy_async",
                 "kvc_copy2d_async", "kvc_place_slice"]
+PAGES_SYMBOLS = ["kvc_pages_workspace", "kvc_pages_reserve", "kvc_pages_write", "kvc_pages_read", "kvc_pages_copy",
+                 "kvc_pages_fork", "kvc_pages_compact", "kvc_pages_free"]
+ATTN_SYMBOLS = ["kvc_attn_prompt", "kvc_attn_tree_workspace", "kvc_attn_tree"]
 STAGES = ["decode", "score", "softmax_importance", "select", "refit_target", "beta", "x_build", "ls_gram",
           "refine", "metrics", "requant", "ls_factor", "ls_out"]
 
@@ -96,6 +99,21 @@ def load(path=None):
     lib.kvc_copy2d_async.argtypes = [c_void_p, c_size_t, c_void_p, c_size_t, c_size_t, c_size_t, c_void_p]
     lib.kvc_place_slice.restype = c_int
     lib.kvc_place_slice.argtypes = [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p]
+    P = c_void_p                                    # structs, device pointers and host id arrays
+    for name, res, args in (
+            ("kvc_pages_workspace", c_size_t, [P]),
+            ("kvc_pages_reserve", c_int, [P, P, P, c_int, P, c_size_t, P]),
+            ("kvc_pages_write", c_int, [P, P, P, P, c_int, P, P, P, P]),
+            ("kvc_pages_read", c_int, [P, P, P, P, c_int, P, P, P, P]),
+            ("kvc_pages_copy", c_int, [P, P, P, c_int, P]),
+            ("kvc_pages_fork", c_int, [P, P, P, c_int, P, c_size_t, P]),
+            ("kvc_pages_compact", c_int, [P, P, P, c_int, P, P, P, c_int, c_size_t, P, P, P, c_size_t, P]),
+            ("kvc_pages_free", c_int, [P, P, c_int, P, c_size_t, P]),
+            ("kvc_attn_prompt", c_int, [P, P]),
+            ("kvc_attn_tree_workspace", c_size_t, [P, P, P]),
+            ("kvc_attn_tree", c_int, [P, P, P, c_size_t, P])):
+        getattr(lib, name).restype = res
+        getattr(lib, name).argtypes = args
     fns["_lib"] = lib
     fns["_path"] = path
     if path == LIB_PATH or _LIB is None:
