@@ -311,5 +311,8 @@ int kvc_launch_attn_simt(const kvc_attn_args & a, cudaStream_t st) {
 
 int kvc_launch_attn_join(const kvc_attn_args & a, int rb, int tile, cudaStream_t st) {
     if (rb == 8 && tile == 128) return launch_join<8, 128>(a, st);
+    if (rb == 8 && tile == 64) return launch_join<8, 64>(a, st);
+    if (rb == 16 && tile == 64) return launch_join<16, 64>(a, st);
+    if (rb == 32 && tile == 64) return launch_join<32, 64>(a, st);
     return KVC_ERR_SHAPE;
 }

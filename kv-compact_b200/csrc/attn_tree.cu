@@ -1,6 +1,7 @@
 // attn_tree.cu — attention of drafted tokens over the paged cache
 // (include/kvc-attn.h): argument checks and the choice of kernel.
 #include "attn.h"
+#include "attn_tree.h"
 
 #include <limits.h>
 
@@ -8,6 +9,8 @@ namespace {
 
 struct tree_plan {
     kvc_attn_args a;
+    kvc_tree_mma_plan mma;
+    bool use_mma;
     size_t bytes;
 };
 
@@ -34,6 +37,7 @@ int make_plan(const kvc_page_cache * c, const kvc_tree_desc * t, int sms, tree_p
     const uintptr_t qa = t->q_type == KV_TYPE_F32 ? 3 : 1;
     if (((uintptr_t)t->q & qa) || ((uintptr_t)t->out & qa)) return KVC_ERR_SHAPE;
     if ((long long)t->total * t->n_head > INT_MAX || (long long)t->max_nodes * t->n_head > INT_MAX) return KVC_ERR_SHAPE;
+    if (sms < 0) return sms;                             // no device: after the argument checks
     kvc_attn_args & a = p->a;
     a = kvc_attn_args{};
     a.q = t->q;
@@ -73,6 +77,15 @@ int make_plan(const kvc_page_cache * c, const kvc_tree_desc * t, int sms, tree_p
     a.page = c->page_size;
     a.by_page = kvc_make_divisor((uint32_t)c->page_size);
     a.by_group = kvc_make_divisor((uint32_t)a.g);
+    if (t->n_seqs == 0 || t->total == 0 || t->max_nodes == 0) {
+        p->bytes = 0;
+        return KVC_OK;
+    }
+    p->use_mma = kvc_attn_tree_mma_plan(&a, sms, &p->mma);
+    if (p->use_mma) {
+        p->bytes = kvc_attn_part_bytes(p->mma.rb, p->mma.blocks * a.Hkv, a.W, a.dv);
+        return KVC_OK;
+    }
     a.W = kvc_attn_simt_workers(a, sms);
     const long long blocks = ((long long)a.max_q * a.g + KVC_SIMT_RB - 1) / KVC_SIMT_RB * a.Hkv;
     p->bytes = kvc_attn_part_bytes(KVC_SIMT_RB, blocks, a.W, a.dv);
@@ -85,8 +98,7 @@ extern "C" {
 
 KVC_EXPORT size_t kvc_attn_tree_workspace(const kvc_page_cache * cache, const kvc_tree_desc * desc, int * rc) {
     tree_plan p;
-    int sms = kvc_serve_device();
-    int r = sms < 0 ? sms : make_plan(cache, desc, sms, &p);
+    const int r = make_plan(cache, desc, kvc_serve_device(), &p);
     if (rc) *rc = r;
     return r ? 0 : p.bytes;
 }
@@ -95,13 +107,13 @@ KVC_EXPORT int kvc_attn_tree(const kvc_page_cache * cache, const kvc_tree_desc *
                              size_t workspace_bytes, void * stream) {
     tree_plan p;
     const int sms = kvc_serve_device();
-    const int rc = make_plan(cache, desc, sms < 0 ? 1 : sms, &p);
+    const int rc = make_plan(cache, desc, sms, &p);
     if (rc) return rc;
-    if (sms < 0) return sms;
     if (desc->n_seqs == 0 || desc->total == 0 || desc->max_nodes == 0) return KVC_OK;
     if (p.bytes && !workspace) return KVC_ERR_NULL;
     if (p.bytes > workspace_bytes || ((uintptr_t)workspace & 15)) return KVC_ERR_SHAPE;
     p.a.part = static_cast<float *>(workspace);
+    if (p.use_mma) return kvc_launch_attn_tree_mma(p.a, p.mma, (cudaStream_t)stream);
     return kvc_launch_attn_simt(p.a, (cudaStream_t)stream);
 }
 
