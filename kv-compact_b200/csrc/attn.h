@@ -4,6 +4,7 @@
 #pragma once
 
 #include <cuda_fp16.h>
+#include <math.h>
 
 #include "serve.h"
 
@@ -38,9 +39,12 @@ struct kvc_attn_args {
     int mask_words;
     int n_slots, n_pages, max_pages, page;
     kvc_divisor by_page, by_group;
-    // the split: W workers per (KV head, row block)
-    int W;
+    // the split: blocks of rb query rows, tiles of `tile` keys, W workers per
+    // (KV head, row block)
+    int rb, tile, W;
+    kvc_divisor by_tile;
     float * part;           // partial results
+    int * status;           // set to KVC_ERR_CUDA by a device wait that ran out (or null)
 };
 
 // One sequence of a batch.
@@ -93,7 +97,7 @@ __device__ __forceinline__ bool attn_sees(const kvc_attn_args & a, const kvc_att
 
 // ---- the split of the keys ---------------------------------------------------
 //
-// For one (KV head, row block of RB rows) the key tiles of all sequences that
+// For one (KV head, row block) the key tiles of all sequences that
 // have rows in the block are laid end to end, and worker w of W takes tiles
 // [w*T/W, (w+1)*T/W). Sequences of any lengths then load the workers evenly.
 // A worker's stretch meets at most two sequences that it does not cover whole:
@@ -101,40 +105,29 @@ __device__ __forceinline__ bool attn_sees(const kvc_attn_args & a, const kvc_att
 // their partial results go to those slots and are joined afterwards, in the
 // workers' order.
 
-template <int RB, int TILE>
+// Key tiles of sequence s in row block qb (blocks of a.rb rows, tiles of a.tile keys).
 __device__ __forceinline__ int attn_tiles(const kvc_attn_args & a, int s, int qb) {
     const kvc_attn_seq q = attn_seq(a, s);
-    if (qb * RB >= (long long)q.nq * a.g) return 0;
-    return (q.ln + TILE - 1) / TILE;
-}
-
-// Total tiles of row block qb, the same in every lane.
-template <int RB, int TILE>
-__device__ __forceinline__ long long attn_total(const kvc_attn_args & a, int qb) {
-    const int lane = threadIdx.x & 31;
-    long long t = 0;
-    for (int s = lane; s < a.n_seqs; s += 32) t += attn_tiles<RB, TILE>(a, s, qb);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(~0u, t, o);
-    return t;
+    if ((long long)qb * a.rb >= (long long)q.nq * a.g) return 0;
+    return q.ln ? (int)a.by_tile.div((uint32_t)q.ln - 1u) + 1 : 0;
 }
 
 // fn(s, lo, hi, slot) for every piece of worker w's stretch: tiles lo..hi-1 of
 // sequence s; slot -1 where that is all of them. Every warp of a CTA takes the
 // same steps.
-template <int RB, int TILE, typename F>
+template <typename F>
 __device__ __forceinline__ void attn_walk(const kvc_attn_args & a, int qb, int w, F && fn) {
     const int lane = threadIdx.x & 31;
-    int mine0 = lane < a.n_seqs ? attn_tiles<RB, TILE>(a, lane, qb) : 0;
+    const int mine0 = lane < a.n_seqs ? attn_tiles(a, lane, qb) : 0;
     long long T = mine0;
-    for (int s = lane + 32; s < a.n_seqs; s += 32) T += attn_tiles<RB, TILE>(a, s, qb);
+    for (int s = lane + 32; s < a.n_seqs; s += 32) T += attn_tiles(a, s, qb);
 #pragma unroll
     for (int o = 16; o; o >>= 1) T += __shfl_xor_sync(~0u, T, o);
     const long long from = w * T / a.W, to = (w + 1) * T / a.W;
     long long at = 0;
     for (int s0 = 0; s0 < a.n_seqs && at < to; s0 += 32) {
         const int s = s0 + lane;
-        const int t = s0 == 0 ? mine0 : (s < a.n_seqs ? attn_tiles<RB, TILE>(a, s, qb) : 0);
+        const int t = s0 == 0 ? mine0 : (s < a.n_seqs ? attn_tiles(a, s, qb) : 0);
         long long p = t;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -161,22 +154,29 @@ __device__ __forceinline__ int attn_worker(long long x, long long T, int W) {
     return (int)(((x + 1) * W - 1) / T);
 }
 
-// Partial results of worker w, slot s: RB sums of d_v, then RB maxima, RB sums.
-template <int RB>
+// Partial results of worker w, slot s: rb sums of d_v, then rb maxima, rb sums.
 __device__ __forceinline__ float * attn_part(const kvc_attn_args & a, int qb, int h, int w, int slot) {
-    return a.part + ((((size_t)qb * a.Hkv + h) * a.W + w) * 2 + slot) * ((size_t)RB * (a.dv + 2));
+    return a.part + ((((size_t)qb * a.Hkv + h) * a.W + w) * 2 + slot) * ((size_t)a.rb * (a.dv + 2));
 }
-inline size_t kvc_attn_part_bytes(int rb, long long blocks, int W, int dv) {
-    return W > 1 ? (size_t)blocks * W * 2 * rb * (dv + 2) * sizeof(float) : 0;
+inline size_t kvc_attn_part_bytes(const kvc_attn_args & a, long long blocks) {
+    return a.W > 1 ? (size_t)blocks * a.Hkv * a.W * 2 * a.rb * (a.dv + 2) * sizeof(float) : 0;
+}
+
+// Output row (token, head) from its sum and statistics.
+__device__ __forceinline__ void attn_store(const kvc_attn_args & a, size_t row, int d, float o, float M, float L) {
+    const float v = L > 0.0f ? o / L : (L == 0.0f ? 0.0f : L);       // no key seen: 0; NaN stays NaN
+    if (a.q_type == KV_TYPE_F16) reinterpret_cast<__half *>(a.out)[row * a.dv + d] = __float2half_rn(v);
+    else reinterpret_cast<float *>(a.out)[row * a.dv + d] = v;
+    if (d == 0 && a.lse) a.lse[row] = L == 0.0f ? -INFINITY : M + logf(L);
 }
 
 // Joins the partial results and writes rows that no tile reached (attn_simt.cu).
-// RB and TILE are those of the kernel that ran.
-int kvc_launch_attn_join(const kvc_attn_args & a, int rb, int tile, cudaStream_t st);
+// `overlap`: the kernel that ran lets its successor start early.
+int kvc_launch_attn_join(const kvc_attn_args & a, bool overlap, cudaStream_t st);
 // The general kernel: every type, d <= 256, any strides (attn_simt.cu).
-int kvc_attn_simt_workers(const kvc_attn_args & a, int sms);
+// Sets the split for it; `whole`: one worker per row block (no partial results).
+void kvc_attn_simt_split(kvc_attn_args * a, int sms, bool whole);
 int kvc_launch_attn_simt(const kvc_attn_args & a, cudaStream_t st);
-constexpr int KVC_SIMT_RB = 8, KVC_SIMT_TILE = 128;
 
 // ---- stored elements -----------------------------------------------------------
 // Element e of a row's head segment at p (block types: segments start on a block).

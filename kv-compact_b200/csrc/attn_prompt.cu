@@ -54,7 +54,7 @@ KVC_EXPORT int kvc_attn_prompt(const kvc_prompt_desc * t, void * stream) {
     a.page = 1;
     a.by_page = kvc_make_divisor(1);
     a.by_group = kvc_make_divisor((uint32_t)a.g);
-    a.W = 1;
+    kvc_attn_simt_split(&a, sms, true);
     return kvc_launch_attn_simt(a, (cudaStream_t)stream);
 }
 

@@ -13,7 +13,7 @@
 
 namespace {
 
-constexpr int RB = KVC_SIMT_RB, TILE = KVC_SIMT_TILE;
+constexpr int RB = 8, TILE = 128;        // query rows and keys per CTA and step
 constexpr int WARPS = 4, THREADS = 32 * WARPS, WK = 32;
 static_assert(TILE == WARPS * WK, "a tile is one key per lane");
 
@@ -36,7 +36,7 @@ __global__ void __launch_bounds__(THREADS) k_attn_simt(const __grid_constant__ k
     const int n_blocks = (int)(((long long)a.max_q * a.g + RB - 1) / RB);
 
     for (int qb = blockIdx.y / a.Hkv; qb < n_blocks; qb += gridDim.y / a.Hkv) {
-    attn_walk<RB, TILE>(a, qb, w, [&](int s, int lo, int hi, int slot) {
+    attn_walk(a, qb, w, [&](int s, int lo, int hi, int slot) {
         const kvc_attn_seq q = attn_seq(a, s);
         const int r0 = qb * RB;
         const int nr = (int)min((long long)RB, (long long)q.nq * a.g - r0);
@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(THREADS) k_attn_simt(const __grid_constant__ k
                 if (lane + 32 * c < a.dv) joinO[((size_t)warp * RB + r) * a.dv + lane + 32 * c] = o[r][c];
         }
         __syncthreads();
-        float * part = slot >= 0 ? attn_part<RB>(a, qb, h, w, slot) : nullptr;
+        float * part = slot >= 0 ? attn_part(a, qb, h, w, slot) : nullptr;
         for (int e = threadIdx.x; e < nr * a.dv; e += THREADS) {
             const int r = e / a.dv, d = e - r * a.dv;
             float M = -INFINITY;
@@ -169,11 +169,7 @@ __global__ void __launch_bounds__(THREADS) k_attn_simt(const __grid_constant__ k
                 }
             } else {
                 const int i = (int)a.by_group.div(r0 + r);
-                const size_t row = (size_t)(q.q0 + i) * a.Hq + h * a.g + (r0 + r - i * a.g);
-                const float v = L > 0.0f ? O / L : (L == 0.0f ? 0.0f : L);
-                if (a.q_type == KV_TYPE_F16) reinterpret_cast<__half *>(a.out)[row * a.dv + d] = __float2half_rn(v);
-                else reinterpret_cast<float *>(a.out)[row * a.dv + d] = v;
-                if (d == 0 && a.lse) a.lse[row] = L == 0.0f ? -INFINITY : M + logf(L);
+                attn_store(a, (size_t)(q.q0 + i) * a.Hq + h * a.g + (r0 + r - i * a.g), d, O, M, L);
             }
         }
     });
@@ -181,16 +177,17 @@ __global__ void __launch_bounds__(THREADS) k_attn_simt(const __grid_constant__ k
     }
 }
 
-// One warp per (token, query head): the rows whose keys were split over
-// several workers, joined in the workers' order, and rows of sequences
-// without keys. Sequences that one worker covered are written already.
-template <int RBJ, int TILEJ>
+// One CTA per (token, query head): the rows whose keys were split over several
+// workers, joined in the workers' order, and rows of sequences without keys.
+// Sequences that one worker covered are written already. The four warps take
+// every fourth partial result each, several in flight; bound by the latency of
+// those reads. What does not depend on the kernel before is done first, while
+// that one still runs.
 __global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ kvc_attn_args a) {
-    const int lane = threadIdx.x & 31;
-    const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int token = (int)(unit / a.Hq), hq = (int)(unit - (long long)token * a.Hq);
-    if (token >= a.n_total) return;
-    // the sequence of the token (the last one whose rows start at or before it)
+    __shared__ float s_l[4], s_o[4][KVC_MAX_D];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int token = (int)(blockIdx.x / (unsigned)a.Hq), hq = (int)(blockIdx.x - (unsigned)token * (unsigned)a.Hq);
+    // the sequence of the token
     int s = -1;
     for (int s0 = 0; s0 < a.n_seqs && s < 0; s0 += 32) {
         bool in = false;
@@ -201,16 +198,18 @@ __global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ kvc_a
         const unsigned b = __ballot_sync(~0u, in);
         if (b) s = s0 + __ffs(b) - 1;
     }
-    if (s < 0) return;
+    if (s < 0 || token - min(max(a.cu_q[s], 0), a.n_total) >= a.max_q) {
+        cudaGridDependencySynchronize();     // on every path: what follows in the stream relies on it
+        return;
+    }
     const kvc_attn_seq q = attn_seq(a, s);
     const int i = token - q.q0;
-    if (i >= q.nq) return;
     const int h = hq / a.g;
     const int rho = i * a.g + (hq - h * a.g);
-    const int qb = rho / RBJ, r = rho - qb * RBJ;
+    const int qb = rho / a.rb, r = rho - qb * a.rb;
     long long before = 0, T = 0;
     for (int u = lane; u < a.n_seqs; u += 32) {
-        const int t = attn_tiles<RBJ, TILEJ>(a, u, qb);
+        const int t = attn_tiles(a, u, qb);
         T += t;
         if (u < s) before += t;
     }
@@ -219,48 +218,50 @@ __global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ kvc_a
         T += __shfl_xor_sync(~0u, T, o);
         before += __shfl_xor_sync(~0u, before, o);
     }
-    const int tiles = attn_tiles<RBJ, TILEJ>(a, s, qb);
+    const int tiles = attn_tiles(a, s, qb);
     const size_t row = (size_t)token * a.Hq + hq;
+    cudaGridDependencySynchronize();
     if (tiles == 0) {
-        for (int d = lane; d < a.dv; d += 32) {
-            if (a.q_type == KV_TYPE_F16) reinterpret_cast<__half *>(a.out)[row * a.dv + d] = __float2half_rn(0.0f);
-            else reinterpret_cast<float *>(a.out)[row * a.dv + d] = 0.0f;
-        }
-        if (lane == 0 && a.lse) a.lse[row] = -INFINITY;
+        for (int d = threadIdx.x; d < a.dv; d += 128) attn_store(a, row, d, 0.0f, 0.0f, 0.0f);
         return;
     }
     const int w0 = attn_worker(before, T, a.W), w1 = attn_worker(before + tiles - 1, T, a.W);
     if (w0 == w1) return;
+    const size_t step = 2 * (size_t)a.rb * (a.dv + 2);
+    // slot 1 of the first worker where the sequence starts inside its stretch
+    const int slot0 = (long long)w0 * T / a.W > before ? 0 : 1;
+    const float * base_p = attn_part(a, qb, h, w0, 0);
+    const float * first_p = attn_part(a, qb, h, w0, slot0);
+    auto at = [&](int w) {
+        // a later worker's stretch starts inside the sequence, or with it (w*T/W == before)
+        const bool inside = (long long)w * T / a.W > before;
+        return w == w0 ? first_p : base_p + (size_t)(w - w0) * step + (inside ? 0 : step / 2);
+    };
     float M = -INFINITY;
-    for (int w = w0 + lane; w <= w1; w += 32) {
-        const int slot = (long long)w * T / a.W > before ? 0 : 1;
-        M = fmaxf(M, attn_part<RBJ>(a, qb, h, w, slot)[RBJ * a.dv + r]);
-    }
+    for (int w = w0 + lane; w <= w1; w += 32) M = fmaxf(M, at(w)[a.rb * a.dv + r]);
 #pragma unroll
     for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, o));
     const float base = M == -INFINITY ? 0.0f : M;
-    float L = 0.0f, O[8];
+    float L = 0.0f, O[KVC_MAX_D / 32];
 #pragma unroll
-    for (int c = 0; c < 8; c++) O[c] = 0.0f;
-    for (int w = w0; w <= w1; w++) {
-        const int slot = (long long)w * T / a.W > before ? 0 : 1;
-        const float * p = attn_part<RBJ>(a, qb, h, w, slot);
-        const float f = expf(p[RBJ * a.dv + r] - base);
-        L = fmaf(f, p[RBJ * a.dv + RBJ + r], L);
+    for (int c = 0; c < KVC_MAX_D / 32; c++) O[c] = 0.0f;
+#pragma unroll 4
+    for (int w = w0 + warp; w <= w1; w += 4) {
+        const float * p = at(w);
+        const float f = expf(p[a.rb * a.dv + r] - base);
+        L = fmaf(f, p[a.rb * a.dv + a.rb + r], L);
 #pragma unroll
-        for (int c = 0; c < 8; c++)
+        for (int c = 0; c < KVC_MAX_D / 32; c++)
             if (lane + 32 * c < a.dv) O[c] = fmaf(f, p[r * a.dv + lane + 32 * c], O[c]);
     }
+    if (lane == 0) s_l[warp] = L;
 #pragma unroll
-    for (int c = 0; c < 8; c++) {
-        const int d = lane + 32 * c;
-        if (d < a.dv) {
-            const float v = L > 0.0f ? O[c] / L : (L == 0.0f ? 0.0f : L);
-            if (a.q_type == KV_TYPE_F16) reinterpret_cast<__half *>(a.out)[row * a.dv + d] = __float2half_rn(v);
-            else reinterpret_cast<float *>(a.out)[row * a.dv + d] = v;
-        }
-    }
-    if (lane == 0 && a.lse) a.lse[row] = L == 0.0f ? -INFINITY : M + logf(L);
+    for (int c = 0; c < KVC_MAX_D / 32; c++)
+        if (lane + 32 * c < a.dv) s_o[warp][lane + 32 * c] = O[c];
+    __syncthreads();
+    L = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
+    for (int d = threadIdx.x; d < a.dv; d += 128)
+        attn_store(a, row, d, (s_o[0][d] + s_o[1][d]) + (s_o[2][d] + s_o[3][d]), M, L);
 }
 
 size_t simt_smem(int dk, int dv) {
@@ -278,23 +279,16 @@ int launch_simt(const kvc_attn_args & a, dim3 grid, cudaStream_t st) {
     return KVC_OK;
 }
 
-template <int RBJ, int TILEJ>
-int launch_join(const kvc_attn_args & a, cudaStream_t st) {
-    const long long units = (long long)a.n_total * a.Hq;
-    if (units == 0) return KVC_OK;
-    k_attn_join<RBJ, TILEJ><<<(unsigned)((units + 3) / 4), 128, 0, st>>>(a);
-    g_serve_launches++;
-    KVC_CUDA(cudaGetLastError());
-    return KVC_OK;
-}
-
 }  // namespace
 
-int kvc_attn_simt_workers(const kvc_attn_args & a, int sms) {
+void kvc_attn_simt_split(kvc_attn_args * a, int sms, bool whole) {
+    a->rb = RB;
+    a->tile = TILE;
+    a->by_tile = kvc_make_divisor(TILE);
     // enough CTAs for four waves' worth of two per SM
-    const long long blocks = ((long long)a.max_q * a.g + RB - 1) / RB * a.Hkv;
-    const long long w = (8LL * sms + blocks - 1) / (blocks > 0 ? blocks : 1);
-    return (int)(w < 1 ? 1 : w);
+    const long long blocks = ((long long)a->max_q * a->g + RB - 1) / RB * a->Hkv;
+    const long long w = whole || blocks <= 0 ? 1 : (8LL * sms + blocks - 1) / blocks;
+    a->W = (int)(w < 1 ? 1 : w);
 }
 
 int kvc_launch_attn_simt(const kvc_attn_args & a, cudaStream_t st) {
@@ -306,13 +300,22 @@ int kvc_launch_attn_simt(const kvc_attn_args & a, cudaStream_t st) {
     if (a.dv <= 64) rc = launch_simt<2>(a, grid, st);
     else if (a.dv <= 128) rc = launch_simt<4>(a, grid, st);
     else rc = launch_simt<8>(a, grid, st);
-    return rc ? rc : kvc_launch_attn_join(a, RB, TILE, st);
+    return rc ? rc : kvc_launch_attn_join(a, false, st);
 }
 
-int kvc_launch_attn_join(const kvc_attn_args & a, int rb, int tile, cudaStream_t st) {
-    if (rb == 8 && tile == 128) return launch_join<8, 128>(a, st);
-    if (rb == 8 && tile == 64) return launch_join<8, 64>(a, st);
-    if (rb == 16 && tile == 64) return launch_join<16, 64>(a, st);
-    if (rb == 32 && tile == 64) return launch_join<32, 64>(a, st);
-    return KVC_ERR_SHAPE;
+int kvc_launch_attn_join(const kvc_attn_args & a, bool overlap, cudaStream_t st) {
+    const long long units = (long long)a.n_total * a.Hq;
+    if (units == 0) return KVC_OK;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)units);
+    cfg.blockDim = dim3(128);
+    cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = overlap ? 1 : 0;
+    KVC_CUDA(cudaLaunchKernelEx(&cfg, k_attn_join, a));
+    g_serve_launches++;
+    return KVC_OK;
 }

@@ -9,7 +9,6 @@ namespace {
 
 struct tree_plan {
     kvc_attn_args a;
-    kvc_tree_mma_plan mma;
     bool use_mma;
     size_t bytes;
 };
@@ -71,6 +70,7 @@ int make_plan(const kvc_page_cache * c, const kvc_tree_desc * t, int sms, tree_p
     a.beta = c->beta ? c->beta + (size_t)t->layer * rows * c->n_head_kv : nullptr;
     a.mask = t->mask;
     a.mask_words = t->mask_words;
+    a.status = c->status;
     a.n_slots = c->n_slots;
     a.n_pages = c->n_pages;
     a.max_pages = c->max_pages;
@@ -81,14 +81,13 @@ int make_plan(const kvc_page_cache * c, const kvc_tree_desc * t, int sms, tree_p
         p->bytes = 0;
         return KVC_OK;
     }
-    p->use_mma = kvc_attn_tree_mma_plan(&a, sms, &p->mma);
-    if (p->use_mma) {
-        p->bytes = kvc_attn_part_bytes(p->mma.rb, p->mma.blocks * a.Hkv, a.W, a.dv);
-        return KVC_OK;
+    long long blocks = 0;
+    p->use_mma = kvc_attn_tree_mma_plan(&a, sms, &blocks);
+    if (!p->use_mma) {
+        kvc_attn_simt_split(&a, sms, false);
+        blocks = ((long long)a.max_q * a.g + a.rb - 1) / a.rb;
     }
-    a.W = kvc_attn_simt_workers(a, sms);
-    const long long blocks = ((long long)a.max_q * a.g + KVC_SIMT_RB - 1) / KVC_SIMT_RB * a.Hkv;
-    p->bytes = kvc_attn_part_bytes(KVC_SIMT_RB, blocks, a.W, a.dv);
+    p->bytes = kvc_attn_part_bytes(a, blocks);
     return KVC_OK;
 }
 
@@ -113,7 +112,7 @@ KVC_EXPORT int kvc_attn_tree(const kvc_page_cache * cache, const kvc_tree_desc *
     if (p.bytes && !workspace) return KVC_ERR_NULL;
     if (p.bytes > workspace_bytes || ((uintptr_t)workspace & 15)) return KVC_ERR_SHAPE;
     p.a.part = static_cast<float *>(workspace);
-    if (p.use_mma) return kvc_launch_attn_tree_mma(p.a, p.mma, (cudaStream_t)stream);
+    if (p.use_mma) return kvc_launch_attn_tree_mma(p.a, (cudaStream_t)stream);
     return kvc_launch_attn_simt(p.a, (cudaStream_t)stream);
 }
 

@@ -13,33 +13,57 @@
 //
 // The codes of the block formats are small integers, exact in fp16; a block's
 // scale is applied to its 32-value partial score on one side and to the
-// probabilities on the other, in fp32. With F32 queries both Q (times a power
-// of two per row) and P dV (times a power of two, kept per warp) enter as two
-// fp16 pieces, 22 bits together; with F16 queries as one. Q4_1's minima add
-// m[key][b] (sum of Q over b) and a product of P m with ones.
+// probabilities on the other. With F32 queries both Q (times a power of two
+// per row) and P dV (times a power of two, kept per warp) enter as two fp16
+// pieces, 22 bits together; with F16 queries Q enters as it is and P dV is
+// rounded once to fp16, as the output is. Q4_1's minima add m[key][b] (sum of
+// Q over b) to the scores and a product of P m with ones to the output.
 //
-// A warp works alone: 16 keys per step through its own ring of asynchronous
-// copies, its own running maximum, sum and output, no barrier in the loop; the
-// four warps of a CTA and the CTAs of a sequence are joined at the end.
+// One CTA per SM (16 or 8 warps) runs through its stretch of the keys with a
+// ring of stages, each `tile` whole rows: the part of every row that belongs to
+// the CTA's heads, loaded by TMA in boxes of as many rows as lie side by side
+// in a page. The box is up to 31 bytes wider than that part, so that rows lie an
+// odd number of 16 bytes apart and fragment reads meet no bank conflict. Warp
+// 0 refills the ring between its own steps, two tiles behind the fastest reader.
+// A warp owns one KV head and one block of query rows for a sequence, takes
+// every nsub-th group of 16 keys, and keeps its own maximum, sum and output;
+// the warps of a head are joined at the end of the CTA's stretch of a
+// sequence, the CTAs afterwards (k_attn_join). Rows or pages that TMA cannot
+// read (row sizes that are no multiple of 16 bytes, pages without 8 rows side
+// by side) are copied by all warps with cp.async instead.
 #include "attn.h"
 #include "attn_tree.h"
+#include "tc_sm100.h"
 
-#include <math.h>
+#include <cuda.h>
 
 namespace {
 
-constexpr int WARPS = 4, THREADS = 128, KEYS = 16;
-constexpr int TILE = WARPS * KEYS;
+constexpr int KEYS = 16;                  // keys of one MMA step
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int P_SHIFT = 13;               // P dV enters as P dV 2^(13 - R), R >= exponent of the largest dV so far
+constexpr int P_SHIFT = 10;               // P dV enters as P dV 2^(10 - R), R >= exponent of the largest dV so far
+constexpr int MAX_STAGES = 8, MAX_TILE = 256, MAX_SEGS = 64;
+constexpr uint32_t POLLS = 1u << 22;      // bound of every wait
 
 struct mma_geom {
+    int nw;                     // warps
+    int hc, ngh;                // KV heads per CTA, groups of them
+    int rc;                     // blocks of 8*NB query rows per CTA
     int kp, vp;                 // ring bytes per K / V row (16 * odd: no bank conflicts)
-    int kseg, vseg;             // bytes of a head's part of a row
-    int kg, vg;                 // copy piece: 16, 8 or 4 bytes
-    int stages;
-    int ring;                   // bytes of the rings (and of the join's buffer)
+    int kg, vg;                 // cp.async piece: 16, 8 or 4 bytes
+    int run;                    // rows per TMA box; 0: cp.async
+    int bbox;                   // floats between the beta of two boxes
+    int stages, stage_bytes;
     int nbk, nbv;               // 32-value blocks per head
+    int qvec;                   // rows of q may be read four elements at a time
+    kvc_divisor by_run;
+};
+
+// A piece of the CTA's stretch: key tiles lo .. hi-1 of one sequence.
+struct segment {
+    int lo, hi, slot;
+    int q0, nq, ln;
+    int table;                  // table row
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void * p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -96,6 +120,12 @@ __device__ __forceinline__ uint32_t lds32(const uint8_t * p) {
     if (ALIGNED) return *reinterpret_cast<const uint32_t *>(p);
     return lds16(p) | (lds16(p + 2) << 16);
 }
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t pair16(uint32_t lo, uint32_t hi) { return __byte_perm(lo, hi, 0x5410); }
 __device__ __forceinline__ float half_bits(uint32_t h) { return __half2float(__ushort_as_half((unsigned short)h)); }
 
 // Two signed bytes (b0, b1 of v after v ^= 0x80808080) as fp16: 0x6400 | u is
@@ -159,7 +189,8 @@ __device__ __forceinline__ void k_frag(uint32_t a[2][4], const uint8_t * r0, con
 
 // A fragments of the output product for a block: dimensions 4g .. 4g+3 (two
 // m-tiles) of keys 2t, 2t+1, 2t+8, 2t+9, whose rows start at `r` + key * vp.
-template <int VT, bool ODD>
+// CENTRE: Q4_1 codes minus 8.
+template <int VT, bool ODD, bool CENTRE>
 __device__ __forceinline__ void v_frag(uint32_t a[2][4], const uint8_t * r, int vp, uint32_t ld_addr, int g) {
     if (VT == KV_TYPE_F16) {
         ldmatrix4_trans(a[0], ld_addr);
@@ -177,7 +208,7 @@ __device__ __forceinline__ void v_frag(uint32_t a[2][4], const uint8_t * r, int 
         }
     } else {
         constexpr int HEAD = VT == KV_TYPE_Q4_0 ? 2 : 4;
-        constexpr int BIAS = VT == KV_TYPE_Q4_0 ? 8 : 0;
+        constexpr int BIAS = VT == KV_TYPE_Q4_0 || CENTRE ? 8 : 0;
 #pragma unroll
         for (int s = 0; s < 2; s++) {
             const uint32_t w = lds16(r + (8 * s) * vp + HEAD + 2 * g) | (lds16(r + (8 * s + 1) * vp + HEAD + 2 * g) << 16);
@@ -190,129 +221,302 @@ __device__ __forceinline__ void v_frag(uint32_t a[2][4], const uint8_t * r, int 
 }
 
 template <int BYTES>
-__device__ __forceinline__ void copy_async(uint32_t dst, const uint8_t * src, bool real) {
-    const int n = real ? BYTES : 0;
-    if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(n) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" :: "r"(dst), "l"(src), "n"(BYTES), "r"(n) : "memory");
+__device__ __forceinline__ void copy_async(uint32_t dst, const uint8_t * src) {
+    if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(dst), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" :: "r"(dst), "l"(src), "n"(BYTES) : "memory");
+}
+// One row's part, by a warp.
+__device__ __forceinline__ void copy_row(uint32_t dst, const uint8_t * src, int g, int bytes, int lane) {
+    if (g == 16) for (int o = 16 * lane; o < bytes; o += 512) copy_async<16>(dst + o, src + o);
+    else if (g == 8) for (int o = 8 * lane; o < bytes; o += 256) copy_async<8>(dst + o, src + o);
+    else for (int o = 4 * lane; o < bytes; o += 128) copy_async<4>(dst + o, src + o);
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void * map, int x, int y, int z, uint64_t * bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 :: "r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar)) : "memory");
 }
 
-// One row's part for one head: `pieces` pieces of g bytes, four lanes side by side.
-__device__ __forceinline__ void copy_row(uint32_t dst, const uint8_t * src, bool real, int g, int bytes, int t) {
-    if (g == 16) {
-        for (int o = 16 * t; o < bytes; o += 64) copy_async<16>(dst + o, src + o, real);
-    } else if (g == 8) {
-        for (int o = 8 * t; o < bytes; o += 32) copy_async<8>(dst + o, src + o, real);
-    } else {
-        for (int o = 4 * t; o < bytes; o += 16) copy_async<4>(dst + o, src + o, real);
-    }
-}
-
+// Bytes of the region that holds the query fragments (two pieces) in the loop and
+// the outputs that are joined after it.
 template <int DB, int NB, int NP>
-__global__ void __launch_bounds__(THREADS) k_tree_mma(const __grid_constant__ kvc_attn_args a,
-                                                      const __grid_constant__ mma_geom G) {
-    constexpr int RB = 8 * NB;
-    constexpr bool QREG = NB == 1 && DB <= 4;            // query fragments stay in registers
-    extern __shared__ __align__(16) uint8_t sm[];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int h = blockIdx.y % a.Hkv, qb = blockIdx.y / a.Hkv, w = blockIdx.x;
-    uint2 * qf = reinterpret_cast<uint2 *>(sm);          // [DB][2][NP][NB][32 lanes] query fragments
-    float * qsum = reinterpret_cast<float *>(qf + DB * 2 * NP * NB * 32);   // [DB][RB] sums of Q over a block
-    float * qmul = qsum + DB * RB;                       // [RB] scale / power of two of the row
-    float * jm = qmul + RB;                              // [WARPS][RB] maxima, [WARPS][RB] sums (join)
-    float * jl = jm + WARPS * RB;
-    uint8_t * ring_all = reinterpret_cast<uint8_t *>(jl + WARPS * RB);
-    const int stage_bytes = KEYS * (G.kp + G.vp) + KEYS * 4;
-    uint8_t * ring = ring_all + (size_t)warp * G.stages * stage_bytes;
-    // where the head's part of a row starts, and from where it is copied
-    const long long k_at = (long long)h * a.k_hb, v_at = (long long)h * a.v_hb;
-    const int k_off = G.kg == 16 ? (int)(k_at & 15) : 0, v_off = G.vg == 16 ? (int)(v_at & 15) : 0;
-    const int k_copy = G.kg == 16 ? (k_off + G.kseg + 15) & ~15 : G.kseg;
-    const int v_copy = G.vg == 16 ? (v_off + G.vseg + 15) & ~15 : G.vseg;
-    const uint8_t * Kh = a.K + (k_at - k_off);
-    const uint8_t * Vh = a.V + (v_at - v_off);
-    const int kt = a.k_type, vt = a.v_type;
+__host__ __device__ constexpr int join_dims() { return DB == 2 ? 64 : 64; }
+template <int DB, int NB, int NP>
+__host__ __device__ inline int shared_region(int nw, int units) {
+    const int frags = NP == 2 ? units * DB * 2 * NB * 32 * 16 : 0;
+    const int join = nw * 8 * NB * (join_dims<DB, NB, NP>() + 4) * 4;
+    return frags > join ? frags : join;
+}
 
-    attn_walk<RB, TILE>(a, qb, w, [&](int s, int lo, int hi, int slot) {
-        const kvc_attn_seq q = attn_seq(a, s);
-        const int r0 = qb * RB;
-        const int nr = (int)min((long long)RB, (long long)q.nq * a.g - r0);
-        const int first_own = q.ln - q.nq;               // rows from here on are the nodes' own
+template <int DB, int NB, int NP, int MAXW>
+__global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant__ kvc_attn_args a,
+                                                           const __grid_constant__ mma_geom G,
+                                                           const __grid_constant__ CUtensorMap k_map,
+                                                           const __grid_constant__ CUtensorMap v_map,
+                                                           const __grid_constant__ CUtensorMap b_map) {
+    using namespace kvc_tc;
+    constexpr int RW = 8 * NB;                           // query rows of a warp
+    constexpr bool QS = NP == 2;                         // query fragments in shared memory
+    constexpr int JD = join_dims<DB, NB, NP>(), JP = JD + 4;
+    extern __shared__ __align__(128) uint8_t sm[];
+    const int NW = G.nw, KT = a.tile;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const bool tma = G.run != 0;
+    uint8_t * ring = sm;
+    uint8_t * fixed = sm + (size_t)G.stages * G.stage_bytes;
+    uint64_t * full = reinterpret_cast<uint64_t *>(fixed);
+    uint64_t * empty = full + MAX_STAGES;
+    uint32_t * bad = reinterpret_cast<uint32_t *>(empty + MAX_STAGES);       // [stages] boxes without a page
+    int * n_segs = reinterpret_cast<int *>(bad + MAX_STAGES);                // [2]: of this batch, of all
+    segment * segs = reinterpret_cast<segment *>(n_segs + 8);
+    float * qsum_all = reinterpret_cast<float *>(segs + MAX_SEGS);           // [NW][DB][RW]
+    float * jm = qsum_all + NW * DB * RW;                                    // [NW][RW] maxima, sums; of the units
+    float * jl = jm + NW * RW;
+    float * uM = jl + NW * RW;
+    float * uL = uM + NW * RW;
+    uint4 * qs_all = reinterpret_cast<uint4 *>(uL + NW * RW);                // [units][DB][2][NB][32] (two pieces)
+    float * jo = reinterpret_cast<float *>(qs_all);                          // [NW][RW][JP], after the loop
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < G.stages; i++) {
+            mbar_init(full + i, tma ? 1 : 64 * NW);
+            mbar_init(empty + i, NW);
+        }
+        mbar_init_fence();
+    }
+    cudaTriggerProgrammaticLaunchCompletion();           // the join may set up meanwhile; it waits for this grid
+
+    const int hg = blockIdx.y % G.ngh, qb = blockIdx.y / G.ngh, w = blockIdx.x;
+    const int h0 = hg * G.hc, nh = min(G.hc, a.Hkv - h0);
+    // the heads' part of a row: where it starts, and from where it is copied
+    const int k_at = h0 * (int)a.k_hb, v_at = h0 * (int)a.v_hb;
+    const int k_off = tma || G.kg == 16 ? k_at & 15 : 0, v_off = tma || G.vg == 16 ? v_at & 15 : 0;
+    const int kt = a.k_type, vt = a.v_type;
+    const bool has_bias = !tma || a.beta != nullptr;
+    float * qsum = qsum_all + warp * DB * RW;
+    bool dead = false;                                   // a wait ran out: no more waits, the status says so
+    auto await = [&](uint64_t * bar, uint32_t parity) {
+        if (!dead && !mbar_wait(bar, parity, POLLS)) {
+            dead = true;
+            if (a.status) *a.status = KVC_ERR_CUDA;
+        }
+    };
+    int p_stage = 0, c_stage = 0;                        // next stage to fill / to read
+    uint32_t p_phase = 1, c_phase = 0;
+    auto step = [&](int & st, uint32_t & ph) {
+        if (++st == G.stages) {
+            st = 0;
+            ph ^= 1;
+        }
+    };
+
+    for (int batch = 0;; batch += MAX_SEGS) {
+        // ---- the pieces of this CTA's stretch, MAX_SEGS at a time
         __syncthreads();
-        // query fragments: a warp takes rows warp, warp + 4, ...
-        for (int r = warp; r < RB; r += WARPS) {
-            float v[DB];
-            float top = 0.0f;
+        if (warp == 0) {
+            int n = 0;
+            attn_walk(a, qb, w, [&](int s, int lo, int hi, int slot) {
+                if (n >= batch && n < batch + MAX_SEGS && lane == 0) {
+                    const kvc_attn_seq q = attn_seq(a, s);
+                    segs[n - batch] = segment{lo, hi, slot, q.q0, q.nq, q.ln, (int)((q.table - a.table) / a.max_pages)};
+                }
+                n++;
+            });
+            if (lane == 0) {
+                n_segs[0] = min(n - batch, MAX_SEGS);
+                n_segs[1] = n;
+            }
+        }
+        __syncthreads();
+        const int ns = n_segs[0];
+
+        // ---- filling: the next tile of the batch, in order
+        int p_seg = 0, p_tile = ns > 0 ? segs[0].lo : 0;
+        int p_page = -1;                                 // TMA: page of box `lane` of that tile, read ahead
+        auto look = [&]() {
+            p_page = -1;
+            if (p_seg < ns) {
+                const segment & S = segs[p_seg];
+                const long long j = (long long)p_tile * KT + lane * G.run;
+                if (lane * G.run < KT && j < S.ln) p_page = a.table[(size_t)S.table * a.max_pages + a.by_page.div((uint32_t)j)];
+            }
+        };
+        auto fill = [&]() {
+            if (p_seg >= ns) return;
+            const segment & S = segs[p_seg];
+            await(empty + p_stage, p_phase);
+            uint8_t * st = ring + (size_t)p_stage * G.stage_bytes;
+            uint8_t * sv = st + KT * G.kp;
+            float * sb = reinterpret_cast<float *>(sv + KT * G.vp);
+            uint64_t * bar = full + p_stage;
+            if (tma) {
+                const int k = lane * G.run;
+                const long long j = (long long)p_tile * KT + k;
+                const bool want = k < KT && j < S.ln;
+                const bool have = want && p_page >= 0 && p_page < a.n_pages && !dead;
+                const uint32_t boxes = __ballot_sync(~0u, have), missing = __ballot_sync(~0u, want && !have);
+                if (lane == 0) {
+                    bad[p_stage] = missing;
+                    const uint32_t bytes = (uint32_t)G.run * (uint32_t)(G.kp + G.vp + (a.beta ? 4 * G.hc : 0));
+                    mbar_arrive_expect_tx(bar, bytes * (uint32_t)__popc(boxes));
+                }
+                __syncwarp();
+                if (have) {
+                    const int off = (int)(j - (long long)a.by_page.div((uint32_t)j) * a.page);
+                    const int row = p_page * a.page + off;
+                    tma_load_2d(st + k * G.kp, &k_map, (k_at - k_off) >> 3, row, bar);
+                    tma_load_2d(sv + k * G.vp, &v_map, (v_at - v_off) >> 3, row, bar);
+                    if (a.beta) tma_load_3d(smem_addr(sb + lane * G.bbox), &b_map, off, h0, p_page, bar);
+                }
+            } else {
+                // rows warp, warp + NW, ...; lane r knows the place of the r-th of them
+                const int k0 = warp + NW * lane;
+                const long long j = (long long)p_tile * KT + k0;
+                int row = -1;
+                if (k0 < KT && j < S.ln) {
+                    const int b = (int)a.by_page.div((uint32_t)j);
+                    const int p = a.table[(size_t)S.table * a.max_pages + b];
+                    if (p >= 0 && p < a.n_pages) row = p * a.page + (int)(j - (long long)b * a.page);
+                }
+                for (int r = 0; warp + NW * r < KT; r++) {
+                    const int k = warp + NW * r;
+                    const long long at = __shfl_sync(~0u, row, r);
+                    for (int hh = lane; hh < nh; hh += 32) {
+                        float b = at < 0 ? -INFINITY : 0.0f;
+                        if (at >= 0 && a.beta) {
+                            const uint32_t p = a.by_page.div((uint32_t)at);
+                            b = a.beta[((size_t)p * a.Hkv + h0 + hh) * a.page + (at - (long long)p * a.page)];
+                        }
+                        sb[hh * KT + k] = b;
+                    }
+                    if (at < 0 || dead) continue;
+                    copy_row(smem_addr(st + k * G.kp), a.K + at * a.k_rb + (k_at - k_off), G.kg,
+                             (k_off + nh * (int)a.k_hb + G.kg - 1) & ~(G.kg - 1), lane);
+                    copy_row(smem_addr(sv + k * G.vp), a.V + at * a.v_rb + (v_at - v_off), G.vg,
+                             (v_off + nh * (int)a.v_hb + G.vg - 1) & ~(G.vg - 1), lane);
+                }
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(smem_addr(bar)) : "memory");
+                mbar_arrive(bar);
+            }
+            step(p_stage, p_phase);
+            if (++p_tile == S.hi) {
+                if (++p_seg < ns) p_tile = segs[p_seg].lo;
+            }
+            if (tma) look();
+        };
+        if (!tma || warp == 0) {
+            if (tma) look();
+            for (int i = 0; i < G.stages - 1; i++) fill();
+        }
+
+    for (int seg = 0; seg < ns; seg++) {
+        const int lo = segs[seg].lo, hi = segs[seg].hi, slot = segs[seg].slot;
+        kvc_attn_seq q;
+        q.q0 = segs[seg].q0;
+        q.nq = segs[seg].nq;
+        q.ln = segs[seg].ln;
+        // this warp's KV head, block of query rows and share of the keys
+        const int rows_here = (int)min((long long)a.rb, (long long)q.nq * a.g - (long long)qb * a.rb);
+        const int units = nh * ((rows_here + RW - 1) / RW);
+        const int nsub = NW / units;
+        const int sub = warp / units, unit = warp - sub * units;
+        const bool active = sub < nsub;
+        const int hc = unit % nh, h = h0 + hc;
+        const int r0 = qb * a.rb + unit / nh * RW;
+        const int nr = min(RW, rows_here - unit / nh * RW);
+        const int first_own = q.ln - q.nq;               // rows from here on are the nodes' own
+
+        // query fragments: lane (g, t) holds, of row g of each block of 8, the
+        // elements that the k-steps of its K type ask of it; two pieces lie in
+        // shared memory (32 registers less in the loop), written by a unit's
+        // first warp
+        uint32_t qf[QS ? 1 : DB][2][NB][2];
+        uint4 * qs = qs_all + (size_t)(active ? unit : 0) * (DB * 2 * NB * 32) + lane;
+        float mul[NB][2];
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++) {
+            const int r = 8 * nb + g;
             const int i = (int)a.by_group.div(r0 + r);
             const long long at = (long long)(q.q0 + i) * a.q_stride + (long long)(h * a.g + (r0 + r - i * a.g)) * a.q_head;
+            const bool there = active && r < nr;
+            float x[DB][8];                              // in the order [k-step][element] of the fragments
 #pragma unroll
             for (int b = 0; b < DB; b++) {
-                v[b] = 0.0f;
-                if (r < nr && b < G.nbk) {
-                    const long long e = at + 32 * b + lane;
-                    v[b] = a.q_type == KV_TYPE_F16 ? __half2float(reinterpret_cast<const __half *>(a.q)[e])
-                                                   : reinterpret_cast<const float *>(a.q)[e];
-                }
-                top = fmaxf(top, fabsf(v[b]));
-            }
-            float up = 1.0f, mul = a.scale;
-            if (NP == 2) {
 #pragma unroll
-                for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+                for (int u = 0; u < 4; u++) {            // pairs of neighbouring elements
+                    const int d = 32 * b + (kt == KV_TYPE_F16 ? 2 * t + 8 * u
+                                            : kt == KV_TYPE_Q8_0 ? 4 * t + 2 * (u & 1) + 16 * (u >> 1) : 8 * t + 2 * u);
+                    float2 v = make_float2(0.0f, 0.0f);
+                    if (there && b < G.nbk) {
+                        if (a.q_type == KV_TYPE_F16) {
+                            const __half * p = reinterpret_cast<const __half *>(a.q) + at + d;
+                            v = G.qvec ? __half22float2(*reinterpret_cast<const __half2 *>(p))
+                                       : make_float2(__half2float(p[0]), __half2float(p[1]));
+                        } else {
+                            const float * p = reinterpret_cast<const float *>(a.q) + at + d;
+                            v = G.qvec ? *reinterpret_cast<const float2 *>(p) : make_float2(p[0], p[1]);
+                        }
+                    }
+                    x[b][2 * u] = v.x;
+                    x[b][2 * u + 1] = v.y;
+                }
+                if (kt == KV_TYPE_Q4_0 || kt == KV_TYPE_Q4_1) {
+                    // dimension i of the lane's eight is element e of step ks: i = 2 ks + (e >> 1) + 4 (e & 1)
+                    const float y1 = x[b][1], y2 = x[b][2], y3 = x[b][3], y4 = x[b][4], y5 = x[b][5], y6 = x[b][6];
+                    x[b][1] = y4;
+                    x[b][2] = y1;
+                    x[b][3] = y5;
+                    x[b][4] = y2;
+                    x[b][5] = y6;
+                    x[b][6] = y3;
+                }
+            }
+            float up = 1.0f, m = a.scale;
+            if (NP == 2) {
+                float top = 0.0f;
+#pragma unroll
+                for (int b = 0; b < DB; b++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[b][e]));
+                top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
                 // largest value of the row in [2^13, 2^14): both pieces normal numbers
                 if (top > 0.0f && top < INFINITY) {
                     const int e = min(max(13 - ilogbf(top), -100), 100);
                     up = scalbnf(1.0f, e);
-                    mul = a.scale * scalbnf(1.0f, -e);
+                    m = a.scale * scalbnf(1.0f, -e);
                 }
             }
-            if (lane == 0) qmul[r] = mul;
+            mul[nb][0] = __shfl_sync(~0u, m, 8 * t);     // of rows 2t and 2t + 1
+            mul[nb][1] = __shfl_sync(~0u, m, 8 * t + 4);
 #pragma unroll
             for (int b = 0; b < DB; b++) {
-                const float x = v[b] * up;
-                float sum = x;
+                float sum = 0.0f;
 #pragma unroll
-                for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-                if (lane == 0) qsum[b * RB + r] = sum;
-                // element `lane` of the block goes to the fragment that reads it
-                int fs, ft, fe;
-                if (kt == KV_TYPE_F16) {
-                    fs = lane >> 4;
-                    ft = (lane & 7) >> 1;
-                    fe = (lane & 1) + 2 * ((lane >> 3) & 1);
-                } else if (kt == KV_TYPE_Q8_0) {
-                    fs = lane >> 4;
-                    ft = (lane & 15) >> 2;
-                    fe = lane & 3;
-                } else {
-                    ft = lane >> 3;
-                    fs = (lane >> 1) & 1;
-                    fe = 2 * (lane & 1) + ((lane >> 2) & 1);
+                for (int ks = 0; ks < 2; ks++) {
+                    uint32_t f[2], rest[2];
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        const float y0 = x[b][4 * ks + 2 * u] * up, y1 = x[b][4 * ks + 2 * u + 1] * up;
+                        sum += y0 + y1;
+                        f[u] = pack(y0, y1);
+                        const float2 z = unpack(f[u]);
+                        rest[u] = pack(y0 - z.x, y1 - z.y);
+                    }
+                    if (QS) {
+                        if (sub == 0) qs[((b * 2 + ks) * NB + nb) * 32] = make_uint4(f[0], f[1], rest[0], rest[1]);
+                    } else {
+                        qf[QS ? 0 : b][ks][nb][0] = f[0];
+                        qf[QS ? 0 : b][ks][nb][1] = f[1];
+                    }
                 }
-                __half * f = reinterpret_cast<__half *>(qf);
-                const int nb = r >> 3, n = r & 7;
-                const __half hi16 = __float2half_rn(x);
-                f[((((b * 2 + fs) * NP + 0) * NB + nb) * 32 + n * 4 + ft) * 4 + fe] = hi16;
-                if (NP == 2)
-                    f[((((b * 2 + fs) * NP + 1) * NB + nb) * 32 + n * 4 + ft) * 4 + fe] =
-                        __float2half_rn(x - __half2float(hi16));
+                if (kt == KV_TYPE_Q4_1) {
+                    sum += __shfl_xor_sync(~0u, sum, 1);
+                    sum += __shfl_xor_sync(~0u, sum, 2);
+                    if (t == 0) qsum[b * RW + r] = sum;
+                }
             }
         }
-        __syncthreads();
-        uint2 qr[QREG ? DB : 1][2][NP];
-        if (QREG) {
-#pragma unroll
-            for (int b = 0; b < DB; b++)
-#pragma unroll
-                for (int st = 0; st < 2; st++)
-#pragma unroll
-                    for (int p = 0; p < NP; p++) qr[QREG ? b : 0][st][p] = qf[((b * 2 + st) * NP + p) * NB * 32 + lane];
-        }
-        float mul[NB][2];
-#pragma unroll
-        for (int nb = 0; nb < NB; nb++) {
-            mul[nb][0] = qmul[8 * nb + 2 * t];
-            mul[nb][1] = qmul[8 * nb + 2 * t + 1];
-        }
+        if (QS) __syncthreads();
+        else __syncwarp();
         float m[NB][2], l[NB][2], O[DB][2][NB][4];
 #pragma unroll
         for (int nb = 0; nb < NB; nb++) {
@@ -325,90 +529,47 @@ __global__ void __launch_bounds__(THREADS) k_tree_mma(const __grid_constant__ kv
 #pragma unroll
                     for (int e = 0; e < 4; e++) O[b][mt][nb][e] = 0.0f;
         }
-        int R = -1000;                                   // exponent that P dV is scaled by; none yet
-        if (vt == KV_TYPE_F16) R = 0;
+        int R = vt == KV_TYPE_F16 ? 0 : -1000;           // exponent that P dV is scaled by; -1000: none yet
 
-        // ---- the ring: steps of 16 keys, table entries two steps ahead, beta one
-        const int end = min(hi * TILE, q.ln);
-        const int j00 = (lo * WARPS + warp) * KEYS;
-        const int steps = j00 < end ? (end - j00 + TILE - 1) / TILE : 0;
-        int pg[2];
-        long long row[2];
-        float bias[2];
-        auto fetch_table = [&](int i) {
-#pragma unroll
-            for (int r = 0; r < 2; r++) {
-                const int j = j00 + i * TILE + g + 8 * r;
-                pg[r] = i < steps && j < end ? q.table[a.by_page.div((uint32_t)j)] : -1;
-            }
-        };
-        auto fetch_bias = [&](int i) {
-#pragma unroll
-            for (int r = 0; r < 2; r++) {
-                const int j = j00 + i * TILE + g + 8 * r;
-                row[r] = -1;
-                bias[r] = -INFINITY;
-                if (pg[r] >= 0 && pg[r] < a.n_pages) {
-                    const int off = j - (int)a.by_page.div((uint32_t)j) * a.page;
-                    row[r] = (long long)pg[r] * a.page + off;
-                    bias[r] = a.beta ? a.beta[((size_t)pg[r] * a.Hkv + h) * a.page + off] : 0.0f;
-                }
-            }
-        };
-        auto issue = [&](int i) {
-            if (i < steps) {
-                uint8_t * st = ring + (i % G.stages) * stage_bytes;
-#pragma unroll
-                for (int r = 0; r < 2; r++) {
-                    const bool real = row[r] >= 0 && bias[r] != -INFINITY;   // rows that nobody sees are read as zeros
-                    const long long at = real ? row[r] : 0;
-                    copy_row(smem_addr(st + (g + 8 * r) * G.kp), Kh + at * a.k_rb, real, G.kg, k_copy, t);
-                    copy_row(smem_addr(st + KEYS * G.kp + (g + 8 * r) * G.vp), Vh + at * a.v_rb, real, G.vg, v_copy, t);
-                    if (t == 0) reinterpret_cast<float *>(st + KEYS * (G.kp + G.vp))[g + 8 * r] = bias[r];
-                }
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            fetch_bias(i + 1);
-            fetch_table(i + 2);
-        };
-        fetch_table(0);
-        fetch_bias(0);
-        fetch_table(1);
-        for (int i = 0; i < G.stages - 1; i++) issue(i);
-
-        for (int i = 0; i < steps; i++) {
-            if (G.stages == 4) asm volatile("cp.async.wait_group 2;" ::: "memory");
-            else if (G.stages == 3) asm volatile("cp.async.wait_group 1;" ::: "memory");
-            else asm volatile("cp.async.wait_group 0;" ::: "memory");
-            __syncwarp();
-            issue(i + G.stages - 1);
-            const uint8_t * st = ring + (i % G.stages) * stage_bytes;
-            const uint8_t * kr0 = st + g * G.kp + k_off;
+        // 16 keys from j0 on, the k0-th of their tile; rows at ks / vs, the head's beta at sb
+        auto group = [&](int j0, int k0, const uint8_t * ks, const uint8_t * vs, const float * sb, uint32_t missing) {
+            const uint8_t * kr0 = ks + g * G.kp;
             const uint8_t * kr1 = kr0 + 8 * G.kp;
-            const float * sb = reinterpret_cast<const float *>(st + KEYS * (G.kp + G.vp));
-            const float b0 = sb[g], b1 = sb[g + 8];
+            // bias of key k of the group; -inf: not there, or hidden from the head
+            auto key_bias = [&](int k) {
+                if (j0 + k >= q.ln) return -INFINITY;
+                if (!tma) return sb[hc * KT + k0 + k];
+                float b = 0.0f;
+                if (has_bias || missing) {
+                    const int box = (int)G.by_run.div((uint32_t)(k0 + k));
+                    if (has_bias) b = sb[box * G.bbox + hc * G.run + (k0 + k - box * G.run)];
+                    if ((missing >> box) & 1u) b = -INFINITY;
+                }
+                return b;
+            };
+            const float b0 = key_bias(g), b1 = key_bias(g + 8);
 
-            // ---- scores of 16 keys x RB rows: S[nb] = {(g, 2t), (g, 2t+1), (g+8, 2t), (g+8, 2t+1)}
+            // ---- scores of 16 keys x RW rows: S[nb] = {(g, 2t), (g, 2t+1), (g+8, 2t), (g+8, 2t+1)}
             float S[NB][4];
 #pragma unroll
             for (int nb = 0; nb < NB; nb++) S[nb][0] = S[nb][1] = S[nb][2] = S[nb][3] = 0.0f;
-            const uint32_t k_ld = smem_addr(st + ((lane & 7) + 8 * ((lane >> 3) & 1)) * G.kp + k_off + 16 * (lane >> 4));
+            const uint32_t k_ld = smem_addr(ks + ((lane & 7) + 8 * ((lane >> 3) & 1)) * G.kp + 16 * (lane >> 4));
             auto scores = [&](auto type) {
-                constexpr int KT = decltype(type)::value;
+                constexpr int KT_ = decltype(type)::value;
 #pragma unroll
                 for (int b = 0; b < DB; b++) {
                     if (b < G.nbk) {
                         uint32_t fa[2][4];
-                        const uint8_t * p0 = kr0 + b * block_bytes(KT);
-                        const uint8_t * p1 = kr1 + b * block_bytes(KT);
-                        if (b & 1) k_frag<KT, true>(fa, p0, p1, k_ld + 64 * b, t);
-                        else k_frag<KT, false>(fa, p0, p1, k_ld + 64 * b, t);
+                        const uint8_t * p0 = kr0 + b * block_bytes(KT_);
+                        const uint8_t * p1 = kr1 + b * block_bytes(KT_);
+                        if (b & 1) k_frag<KT_, true>(fa, p0, p1, k_ld + 64 * b, t);
+                        else k_frag<KT_, false>(fa, p0, p1, k_ld + 64 * b, t);
                         float d0 = 1.0f, d1 = 1.0f, m0 = 0.0f, m1 = 0.0f;
-                        if (KT != KV_TYPE_F16) {
+                        if (KT_ != KV_TYPE_F16) {
                             d0 = half_bits(lds16(p0));
                             d1 = half_bits(lds16(p1));
                         }
-                        if (KT == KV_TYPE_Q4_1) {
+                        if (KT_ == KV_TYPE_Q4_1) {
                             m0 = half_bits(lds16(p0 + 2));
                             m1 = half_bits(lds16(p1 + 2));
                         }
@@ -416,19 +577,21 @@ __global__ void __launch_bounds__(THREADS) k_tree_mma(const __grid_constant__ kv
                         for (int nb = 0; nb < NB; nb++) {
                             float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                            for (int p = NP - 1; p >= 0; p--)          // the small pieces first
-#pragma unroll
-                                for (int ks = 0; ks < 2; ks++) {
-                                    const uint2 f = QREG ? qr[QREG ? b : 0][ks][p]
-                                                         : qf[(((b * 2 + ks) * NP + p) * NB + nb) * 32 + lane];
-                                    mma(c, fa[ks], f.x, f.y, c);
+                            for (int u = 0; u < 2; u++) {
+                                if (QS) {                              // the small piece first
+                                    const uint4 f = qs[((b * 2 + u) * NB + nb) * 32];
+                                    mma(c, fa[u], f.z, f.w, c);
+                                    mma(c, fa[u], f.x, f.y, c);
+                                } else {
+                                    mma(c, fa[u], qf[QS ? 0 : b][u][nb][0], qf[QS ? 0 : b][u][nb][1], c);
                                 }
-                            if (KT == KV_TYPE_Q4_1) {
-                                const float s0 = qsum[b * RB + 8 * nb + 2 * t], s1 = qsum[b * RB + 8 * nb + 2 * t + 1];
-                                S[nb][0] = fmaf(m0, s0, S[nb][0]);
-                                S[nb][1] = fmaf(m0, s1, S[nb][1]);
-                                S[nb][2] = fmaf(m1, s0, S[nb][2]);
-                                S[nb][3] = fmaf(m1, s1, S[nb][3]);
+                            }
+                            if (KT_ == KV_TYPE_Q4_1) {
+                                const float2 s2 = *reinterpret_cast<const float2 *>(qsum + b * RW + 8 * nb + 2 * t);
+                                S[nb][0] = fmaf(m0, s2.x, S[nb][0]);
+                                S[nb][1] = fmaf(m0, s2.y, S[nb][1]);
+                                S[nb][2] = fmaf(m1, s2.x, S[nb][2]);
+                                S[nb][3] = fmaf(m1, s2.y, S[nb][3]);
                             }
                             S[nb][0] = fmaf(d0, c[0], S[nb][0]);
                             S[nb][1] = fmaf(d0, c[1], S[nb][1]);
@@ -446,21 +609,24 @@ __global__ void __launch_bounds__(THREADS) k_tree_mma(const __grid_constant__ kv
             }
 
             // ---- softmax: running maximum per row (the 8 lane groups hold the keys), probabilities
-            const int j0 = j00 + i * TILE;
-            const bool own = a.mask && j0 + KEYS > first_own;      // the step holds rows that the mask decides on
+            const bool own = a.mask && j0 + KEYS > first_own;          // the group holds rows that the mask decides on
+            const bool hidden = __any_sync(~0u, b0 == -INFINITY || b1 == -INFINITY);
             bool moved = false;
             float f[NB][2];
 #pragma unroll
             for (int nb = 0; nb < NB; nb++) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float b = e < 2 ? b0 : b1;
-                    bool sees = b != -INFINITY;
-                    if (own && sees) {
-                        const int rr = r0 + 8 * nb + 2 * t + (e & 1);
-                        sees = rr < r0 + nr && attn_sees(a, q, (int)a.by_group.div(rr), j0 + g + (e < 2 ? 0 : 8));
+                for (int e = 0; e < 4; e++) S[nb][e] = fmaf(S[nb][e], mul[nb][e & 1], e < 2 ? b0 : b1);
+                if (own || hidden) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        bool sees = (e < 2 ? b0 : b1) != -INFINITY;
+                        if (own && sees) {
+                            const int rr = r0 + 8 * nb + 2 * t + (e & 1);
+                            sees = rr < r0 + nr && attn_sees(a, q, (int)a.by_group.div(rr), j0 + g + (e < 2 ? 0 : 8));
+                        }
+                        if (!sees) S[nb][e] = -INFINITY;
                     }
-                    S[nb][e] = sees ? fmaf(S[nb][e], mul[nb][e & 1], b) : -INFINITY;
                 }
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
@@ -489,27 +655,71 @@ __global__ void __launch_bounds__(THREADS) k_tree_mma(const __grid_constant__ kv
             }
 
             // ---- output
-            const uint8_t * vst = st + KEYS * G.kp + v_off;
-            const uint32_t v_ld = smem_addr(vst + ((lane & 7) + 8 * (lane >> 4)) * G.vp + 16 * ((lane >> 3) & 1));
+            // A key that some queries see and others do not may hold infinities or NaN: then value by value.
+            auto by_value = [&]() {
+                if (R == -1000) R = 0;
+                const float up = scalbnf(1.0f, P_SHIFT - R);
+                for (int k = 0; k < KEYS; k++) {
+#pragma unroll
+                    for (int nb = 0; nb < NB; nb++) {
+                        const int from = (k & 7) * 4 + t;
+                        const float x0 = __shfl_sync(~0u, S[nb][0], from), x1 = __shfl_sync(~0u, S[nb][1], from);
+                        const float x2 = __shfl_sync(~0u, S[nb][2], from), x3 = __shfl_sync(~0u, S[nb][3], from);
+                        const float p0 = (k < 8 ? x0 : x2) * up, p1 = (k < 8 ? x1 : x3) * up;
+#pragma unroll
+                        for (int b = 0; b < DB; b++)
+#pragma unroll
+                            for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+                                for (int r8 = 0; r8 < 2; r8++) {
+                                    if (b < G.nbv) {
+                                        const float v = attn_elem(vs + k * G.vp, vt, 32 * b + v_dim(vt, mt, g, r8));
+                                        if (p0 != 0.0f) O[b][mt][nb][2 * r8] = fmaf(p0, v, O[b][mt][nb][2 * r8]);
+                                        if (p1 != 0.0f) O[b][mt][nb][2 * r8 + 1] = fmaf(p1, v, O[b][mt][nb][2 * r8 + 1]);
+                                    }
+                                }
+                    }
+                }
+            };
+            const uint32_t v_ld = smem_addr(vs + ((lane & 7) + 8 * (lane >> 4)) * G.vp + 16 * ((lane >> 3) & 1));
+            const uint8_t * vk = vs + 2 * t * G.vp;      // keys 2t, 2t+1, 2t+8, 2t+9 are this lane's in the product
             auto product = [&](auto type) {
                 constexpr int VT = decltype(type)::value;
-                bool odd_values = false;                 // a scale that is no finite number
-                float c13 = 8192.0f;                     // 2^(13 - R)
-                if (VT != KV_TYPE_F16) {
+                constexpr bool BLOCK = VT != KV_TYPE_F16;
+                constexpr bool TWO = NP == 2 || BLOCK;   // P in two pieces
+                // Q4_1 with one piece: codes minus 8 and m + 8 d, which nearly cancel no more
+                constexpr bool CENTRE = VT == KV_TYPE_Q4_1 && NP == 1;
+                uint32_t dl[DB], dh[DB];
+                uint32_t live_l = ~0u, live_h = ~0u;     // rows hidden from the whole head: scales of 0
+                uint32_t rs = 0x3C003C00u;               // 2^-R
+                if (BLOCK) {
+                    if (hidden) {
+                        live_l = (key_bias(2 * t) == -INFINITY ? 0u : 0xFFFFu) |
+                                 (key_bias(2 * t + 1) == -INFINITY ? 0u : 0xFFFF0000u);
+                        live_h = (key_bias(2 * t + 8) == -INFINITY ? 0u : 0xFFFFu) |
+                                 (key_bias(2 * t + 9) == -INFINITY ? 0u : 0xFFFF0000u);
+                    }
                     uint32_t top = 0;
 #pragma unroll
-                    for (int b = 0; b < DB; b++)
+                    for (int b = 0; b < DB; b++) {
+                        dl[b] = dh[b] = 0;
                         if (b < G.nbv) {
-#pragma unroll
-                            for (int u = 0; u < (VT == KV_TYPE_Q4_1 ? 2 : 1); u++) {
-                                const uint32_t x = lds16(vst + g * G.vp + b * block_bytes(VT) + 2 * u) & 0x7FFFu;
-                                const uint32_t y = lds16(vst + (g + 8) * G.vp + b * block_bytes(VT) + 2 * u) & 0x7FFFu;
-                                odd_values |= x >= 0x7C00u || y >= 0x7C00u;
-                                top = max(top, max(x < 0x7C00u ? x : 0u, y < 0x7C00u ? y : 0u));
+                            const uint8_t * p = vk + b * block_bytes(VT);
+                            dl[b] = pair16(lds16(p), lds16(p + G.vp)) & live_l;
+                            dh[b] = pair16(lds16(p + 8 * G.vp), lds16(p + 9 * G.vp)) & live_h;
+                            top = __vmaxu2(top, __vmaxu2(dl[b] & 0x7FFF7FFFu, dh[b] & 0x7FFF7FFFu));
+                            if (VT == KV_TYPE_Q4_1) {
+                                const uint32_t x = pair16(lds16(p + 2), lds16(p + G.vp + 2)) & live_l;
+                                const uint32_t y = pair16(lds16(p + 8 * G.vp + 2), lds16(p + 9 * G.vp + 2)) & live_h;
+                                top = __vmaxu2(top, __vmaxu2(x & 0x7FFF7FFFu, y & 0x7FFF7FFFu));
                             }
                         }
-                    odd_values = __any_sync(~0u, odd_values);
-                    top = __reduce_max_sync(~0u, top);
+                    }
+                    top = __reduce_max_sync(~0u, max(top & 0xFFFFu, top >> 16));
+                    if (top >= 0x7C00u) {
+                        by_value();
+                        return;
+                    }
                     const int e = top ? max((int)(top >> 10), 1) - 15 : -14;    // |scale| < 2^(e+1)
                     if (e > R) {
                         if (R > -1000) {
@@ -525,30 +735,41 @@ __global__ void __launch_bounds__(THREADS) k_tree_mma(const __grid_constant__ kv
                         }
                         R = e;
                     }
-                    c13 = __int_as_float((127 + P_SHIFT - R) << 23);
+                    rs = pack(__int_as_float((127 - R) << 23), __int_as_float((127 - R) << 23));
                 }
-                // B fragments of P times a factor per key (f0: key g, f1: key g + 8)
-                auto probs = [&](int nb, float f0, float f1, uint32_t bf[NP][2]) {
-                    float x[4] = {S[nb][0] * f0, S[nb][1] * f0, S[nb][2] * f1, S[nb][3] * f1};
-                    if (VT != KV_TYPE_F16 && odd_values) {
+                // P 2^10 as B fragments: [nb][piece][keys 2t.. | 2t+8..]
+                uint32_t pf[NB][2][2];
 #pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            if (S[nb][e] == 0.0f) x[e] = 0.0f;
-                    }
+                for (int nb = 0; nb < NB; nb++)
 #pragma unroll
                     for (int u = 0; u < 2; u++) {
-                        const uint32_t hi2 = pack(x[2 * u], x[2 * u + 1]);
-                        bf[0][u] = transpose8(hi2);
+                        const float x = S[nb][2 * u] * 1024.0f, y = S[nb][2 * u + 1] * 1024.0f;
+                        const uint32_t hi2 = pack(x, y);
+                        pf[nb][0][u] = transpose8(hi2);
+                        if (TWO) {
+                            const float2 k = unpack(hi2);
+                            pf[nb][1][u] = transpose8(pack(x - k.x, y - k.y));
+                        }
+                    }
+                // pieces of P times a factor per key (f: keys 2t, 2t+1 and 2t+8, 2t+9): the product's rounding
+                // error is exact in fp16 (22 bits in all)
+                auto times = [&](int nb, uint32_t fl, uint32_t fh, uint32_t bf[NP][2]) {
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        const uint32_t d = u ? fh : fl;
                         if (NP == 2) {
-                            const float2 b = unpack(hi2);
-                            bf[NP - 1][u] = transpose8(pack(x[2 * u] - b.x, x[2 * u + 1] - b.y));
+                            const uint32_t r = hmul2(pf[nb][0][u], d);
+                            bf[0][u] = r;
+                            bf[NP - 1][u] = hfma2(pf[nb][1][u], d, hfma2(pf[nb][0][u], d, r ^ 0x80008000u));
+                        } else {
+                            bf[0][u] = hfma2(pf[nb][0][u], d, hmul2(pf[nb][1][u], d));
                         }
                     }
                 };
                 auto add = [&](int b, int mt, int nb, const uint32_t * fa, const uint32_t bf[NP][2]) {
                     if (NP == 1) {
                         mma(O[b][mt][nb], fa, bf[0][0], bf[0][1], O[b][mt][nb]);
-                    } else {                             // a step's sum apart, so that the running sum rounds to nearest
+                    } else {                             // the group's sum apart, so that the running sum rounds to nearest
                         float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                         mma(c, fa, bf[NP - 1][0], bf[NP - 1][1], c);
                         mma(c, fa, bf[0][0], bf[0][1], c);
@@ -556,251 +777,340 @@ __global__ void __launch_bounds__(THREADS) k_tree_mma(const __grid_constant__ kv
                         for (int e = 0; e < 4; e++) O[b][mt][nb][e] += c[e];
                     }
                 };
-                uint32_t bf[NB][NP][2];
-                if (VT == KV_TYPE_F16) {
-#pragma unroll
-                    for (int nb = 0; nb < NB; nb++) probs(nb, 8192.0f, 8192.0f, bf[nb]);
-                }
 #pragma unroll
                 for (int b = 0; b < DB; b++) {
                     if (b < G.nbv) {
                         uint32_t fa[2][4];
-                        const uint8_t * p = vst + b * block_bytes(VT);
-                        if (b & 1) v_frag<VT, true>(fa, p + 2 * t * G.vp, G.vp, v_ld + 64 * b, g);
-                        else v_frag<VT, false>(fa, p + 2 * t * G.vp, G.vp, v_ld + 64 * b, g);
-                        float d0 = 0.0f, d1 = 0.0f;
-                        if (VT != KV_TYPE_F16) {
-                            d0 = half_bits(lds16(p + g * G.vp)) * c13;
-                            d1 = half_bits(lds16(p + (g + 8) * G.vp)) * c13;
-                        }
+                        const uint8_t * p = vk + b * block_bytes(VT);
+                        if (b & 1) v_frag<VT, true, CENTRE>(fa, p, G.vp, v_ld + 64 * b, g);
+                        else v_frag<VT, false, CENTRE>(fa, p, G.vp, v_ld + 64 * b, g);
+                        const uint32_t fl = hmul2(dl[b], rs), fh = hmul2(dh[b], rs);
 #pragma unroll
                         for (int nb = 0; nb < NB; nb++) {
-                            if (VT != KV_TYPE_F16) probs(nb, d0, d1, bf[nb]);
-                            add(b, 0, nb, fa[0], bf[nb]);
-                            add(b, 1, nb, fa[1], bf[nb]);
-                        }
-                        if (VT == KV_TYPE_Q4_1) {
-                            const float e0 = half_bits(lds16(p + g * G.vp + 2)) * c13;
-                            const float e1 = half_bits(lds16(p + (g + 8) * G.vp + 2)) * c13;
-                            const uint32_t ones[4] = {0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
+                            uint32_t bf[NP][2];
+                            if (BLOCK) {
+                                times(nb, fl, fh, bf);
+                            } else {
 #pragma unroll
-                            for (int nb = 0; nb < NB; nb++) {
-                                probs(nb, e0, e1, bf[nb]);
-                                add(b, 0, nb, ones, bf[nb]);
-                                add(b, 1, nb, ones, bf[nb]);
+                                for (int pc = 0; pc < NP; pc++) {
+                                    bf[pc][0] = pf[nb][pc][0];
+                                    bf[pc][1] = pf[nb][pc][1];
+                                }
+                            }
+                            add(b, 0, nb, fa[0], bf);
+                            add(b, 1, nb, fa[1], bf);
+                            if (VT == KV_TYPE_Q4_1) {
+                                const uint32_t ones[4] = {0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
+                                uint32_t el = hmul2(pair16(lds16(p + 2), lds16(p + G.vp + 2)) & live_l, rs);
+                                uint32_t eh = hmul2(pair16(lds16(p + 8 * G.vp + 2), lds16(p + 9 * G.vp + 2)) & live_h, rs);
+                                if (CENTRE) {
+                                    el = hfma2(fl, 0x48004800u, el);
+                                    eh = hfma2(fh, 0x48004800u, eh);
+                                }
+                                times(nb, el, eh, bf);
+                                add(b, 0, nb, ones, bf);
+                                add(b, 1, nb, ones, bf);
                             }
                         }
                     }
                 }
             };
-            bool by_value = false;
-            if (own && vt == KV_TYPE_F16) {
-                // a row that the mask hides from some of the queries may hold infinities or NaN
+            if (vt == KV_TYPE_F16) {
                 bool bad = false;
-                for (int k = 0; k < KEYS; k++)
-                    for (int d = lane; d < 32 * G.nbv; d += 32) bad |= (lds16(vst + k * G.vp + 2 * d) & 0x7C00u) == 0x7C00u;
-                by_value = __any_sync(~0u, bad);
-            }
-            if (by_value) {                              // then this step's products are taken value by value
-                for (int k = 0; k < KEYS; k++) {
-#pragma unroll
-                    for (int nb = 0; nb < NB; nb++) {
-                        const int from = (k & 7) * 4 + t;
-                        const float x0 = __shfl_sync(~0u, S[nb][0], from), x1 = __shfl_sync(~0u, S[nb][1], from);
-                        const float x2 = __shfl_sync(~0u, S[nb][2], from), x3 = __shfl_sync(~0u, S[nb][3], from);
-                        const float p0 = (k < 8 ? x0 : x2) * 8192.0f, p1 = (k < 8 ? x1 : x3) * 8192.0f;
-#pragma unroll
-                        for (int b = 0; b < DB; b++)
-#pragma unroll
-                            for (int mt = 0; mt < 2; mt++)
-#pragma unroll
-                                for (int r8 = 0; r8 < 2; r8++) {
-                                    if (b < G.nbv) {
-                                        const float v = half_bits(
-                                            lds16(vst + k * G.vp + 2 * (32 * b + v_dim(KV_TYPE_F16, mt, g, r8))));
-                                        if (p0 != 0.0f) O[b][mt][nb][2 * r8] = fmaf(p0, v, O[b][mt][nb][2 * r8]);
-                                        if (p1 != 0.0f) O[b][mt][nb][2 * r8 + 1] = fmaf(p1, v, O[b][mt][nb][2 * r8 + 1]);
-                                    }
-                                }
-                    }
-                }
+                if (own || hidden)
+                    for (int k = 0; k < KEYS; k++)
+                        for (int d = lane; d < 32 * G.nbv; d += 32) bad |= (lds16(vs + k * G.vp + 2 * d) & 0x7C00u) == 0x7C00u;
+                if (__any_sync(~0u, bad)) by_value();
+                else product(kvc_int<KV_TYPE_F16>{});
+            } else if (vt == KV_TYPE_Q8_0) {
+                product(kvc_int<KV_TYPE_Q8_0>{});
+            } else if (vt == KV_TYPE_Q4_0) {
+                product(kvc_int<KV_TYPE_Q4_0>{});
             } else {
-                switch (vt) {
-                case KV_TYPE_F16: product(kvc_int<KV_TYPE_F16>{}); break;
-                case KV_TYPE_Q8_0: product(kvc_int<KV_TYPE_Q8_0>{}); break;
-                case KV_TYPE_Q4_0: product(kvc_int<KV_TYPE_Q4_0>{}); break;
-                default: product(kvc_int<KV_TYPE_Q4_1>{}); break;
-                }
+                product(kvc_int<KV_TYPE_Q4_1>{});
             }
-        }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        };
 
-        // ---- join the warps: every warp's sums go to shared memory (over the rings)
-        __syncthreads();
-        float * jo = reinterpret_cast<float *>(ring_all);                       // [WARPS][RB][dv]
-        const float back = R > -1000 ? scalbnf(1.0f, R - P_SHIFT) : 0.0f;
+        int turn = sub;                                  // groups until this warp's next one
+        for (int i = lo; i < hi; i++) {
+            await(full + c_stage, c_phase);
+            const uint8_t * st = ring + (size_t)c_stage * G.stage_bytes;
+            const uint8_t * sv = st + KT * G.kp;
+            const uint32_t missing = tma ? bad[c_stage] : 0;
+            const int keys = min(KT, q.ln - i * KT);
+            for (int k = 0; k < keys; k += KEYS) {
+                if (active && turn == 0)
+                    group(i * KT + k, k, st + k * G.kp + k_off + hc * (int)a.k_hb, sv + k * G.vp + v_off + hc * (int)a.v_hb,
+                          reinterpret_cast<const float *>(sv + KT * G.vp), missing);
+                turn = turn == 0 ? nsub - 1 : turn - 1;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty + c_stage);
+            step(c_stage, c_phase);
+            if (!tma || warp == 0) fill();
+        }
+
+        // ---- join the warps of a unit
 #pragma unroll
-        for (int nb = 0; nb < NB; nb++) {
+        for (int nb = 0; nb < NB; nb++)
 #pragma unroll
             for (int c = 0; c < 2; c++) {
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) l[nb][c] += __shfl_xor_sync(~0u, l[nb][c], o);
                 if (g == 0) {
-                    jm[warp * RB + 8 * nb + 2 * t + c] = m[nb][c];
-                    jl[warp * RB + 8 * nb + 2 * t + c] = l[nb][c];
+                    jm[warp * RW + 8 * nb + 2 * t + c] = m[nb][c];
+                    jl[warp * RW + 8 * nb + 2 * t + c] = l[nb][c];
                 }
             }
-#pragma unroll
-            for (int b = 0; b < DB; b++)
-                if (b < G.nbv) {
-#pragma unroll
-                    for (int mt = 0; mt < 2; mt++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            jo[((size_t)warp * RB + 8 * nb + 2 * t + (e & 1)) * a.dv + 32 * b + v_dim(vt, mt, g, e >> 1)] =
-                                O[b][mt][nb][e] * back;
-                }
-        }
         __syncthreads();
-        float * part = slot >= 0 ? attn_part<RB>(a, qb, h, w, slot) : nullptr;
-        for (int e = threadIdx.x; e < nr * a.dv; e += THREADS) {
-            const int r = e / a.dv, d = e - r * a.dv;
-            float M = -INFINITY;
+        const float back = R > -1000 ? scalbnf(1.0f, R - P_SHIFT) : 0.0f;
+        float f[NB][2];
 #pragma unroll
-            for (int u = 0; u < WARPS; u++) M = fmaxf(M, jm[u * RB + r]);
-            const float base = M == -INFINITY ? 0.0f : M;
-            float L = 0.0f, o = 0.0f;
+        for (int nb = 0; nb < NB; nb++)
 #pragma unroll
-            for (int u = 0; u < WARPS; u++) {
-                const float fu = expf(jm[u * RB + r] - base);
-                L = fmaf(fu, jl[u * RB + r], L);
-                o = fmaf(fu, jo[((size_t)u * RB + r) * a.dv + d], o);
+            for (int c = 0; c < 2; c++) {
+                float M = -INFINITY;
+                for (int u = unit; u < units * nsub; u += units) M = fmaxf(M, jm[u * RW + 8 * nb + 2 * t + c]);
+                f[nb][c] = expf(m[nb][c] - (M == -INFINITY ? 0.0f : M)) * back;
             }
-            if (part) {
-                part[r * a.dv + d] = o;
-                if (d == 0) {
-                    part[RB * a.dv + r] = M;
-                    part[RB * a.dv + RB + r] = L;
-                }
-            } else {
-                const int i = (int)a.by_group.div(r0 + r);
-                const size_t at = (size_t)(q.q0 + i) * a.Hq + h * a.g + (r0 + r - i * a.g);
-                const float v = L > 0.0f ? o / L : (L == 0.0f ? 0.0f : L);
-                if (a.q_type == KV_TYPE_F16) reinterpret_cast<__half *>(a.out)[at * a.dv + d] = __float2half_rn(v);
-                else reinterpret_cast<float *>(a.out)[at * a.dv + d] = v;
-                if (d == 0 && a.lse) a.lse[at] = L == 0.0f ? -INFINITY : M + logf(L);
-            }
+        for (int e = threadIdx.x; e < units * RW; e += 32 * NW) {
+            float M = -INFINITY, L = 0.0f;
+            for (int u = e; u < units * nsub * RW; u += units * RW) M = fmaxf(M, jm[u]);
+            for (int u = e; u < units * nsub * RW; u += units * RW)
+                L = fmaf(expf(jm[u] - (M == -INFINITY ? 0.0f : M)), jl[u], L);
+            uM[e] = M;
+            uL[e] = L;
         }
-    });
+#pragma unroll
+        for (int b0 = 0; b0 < DB; b0 += JD / 32) {
+            if (b0 >= G.nbv) break;
+            if (active) {
+#pragma unroll
+                for (int b = b0; b < b0 + JD / 32; b++)
+                    if (b < G.nbv) {
+#pragma unroll
+                        for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                            for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+                                for (int e = 0; e < 4; e++)
+                                    jo[(warp * RW + 8 * nb + 2 * t + (e & 1)) * JP + 32 * (b - b0) + v_dim(vt, mt, g, e >> 1)] =
+                                        O[b][mt][nb][e] * f[nb][e & 1];
+                    }
+            }
+            __syncthreads();
+            for (int ur = warp; ur < units * RW; ur += NW) {
+                const int u = ur / RW, r = ur - u * RW;
+                const int block = u / nh, rr = block * RW + r, hh = h0 + u - block * nh;   // row of the CTA's, KV head
+                if (rr >= rows_here) continue;
+                const float M = uM[ur], L = uL[ur];
+                const int row = qb * a.rb + rr, i = (int)a.by_group.div(row);
+                const size_t out = (size_t)(q.q0 + i) * a.Hq + hh * a.g + (row - i * a.g);
+                float * part = slot >= 0 ? attn_part(a, qb, hh, w, slot) : nullptr;
+#pragma unroll
+                for (int c = 0; c < JD; c += 32) {
+                    const int d = 32 * b0 + c + lane;
+                    if (d >= a.dv) continue;
+                    float o = 0.0f;
+                    for (int k = ur; k < units * nsub * RW; k += units * RW) o += jo[k * JP + c + lane];
+                    if (part) part[rr * a.dv + d] = o;
+                    else attn_store(a, out, d, o, M, L);
+                }
+                if (part && b0 == 0 && lane == 0) {
+                    part[a.rb * a.dv + rr] = M;
+                    part[a.rb * a.dv + a.rb + rr] = L;
+                }
+            }
+            __syncthreads();
+        }
+    }
+        if (n_segs[1] <= batch + MAX_SEGS) break;
+    }
+    if (dead && threadIdx.x < G.stages) {                // copies in flight land before the CTA ends
+        mbar_wait(full + threadIdx.x, 0, POLLS);
+        mbar_wait(full + threadIdx.x, 1, POLLS);
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// Ring geometry, or false where the rows are not ones that the kernel reads.
-bool geometry(const kvc_attn_args & a, int rb, mma_geom * G) {
+int round_pitch(int bytes) {
+    int p = (bytes + 15) & ~15;
+    return (p / 16) % 2 ? p : p + 16;
+}
+
+constexpr int SMEM_MOST = 227 * 1024;
+
+// Shared memory besides the ring, for that many (KV head, row block) units.
+template <int DB, int NB, int NP, int MAXW>
+int fixed_bytes(int nw, int units) {
+    return MAX_STAGES * (8 + 8 + 4) + 32 + MAX_SEGS * (int)sizeof(segment) + nw * 8 * NB * (DB + 4) * 4 +
+           shared_region<DB, NB, NP>(nw, units);
+}
+
+// Ring geometry and split, or false where the rows are not ones that the kernel reads.
+using fixed_fn = int (*)(int, int);
+bool geometry(const kvc_attn_args & a, int rw, int nw, fixed_fn fixed, mma_geom * G, int * tile) {
     if (a.k_type == KV_TYPE_F32 || a.v_type == KV_TYPE_F32 || a.dk % 32 || a.dv % 32) return false;
-    auto side = [](const void * base, long long rbytes, long long hb, int * g, int * p, int seg) {
-        const uintptr_t all = (uintptr_t)base | (uintptr_t)rbytes;
-        if ((hb & 3) || (all & 3)) return false;
-        int most = seg;
-        if ((all & 15) == 0) {                           // 16-byte pieces from the boundary below the head's part
-            *g = 16;
-            most = seg + (int)(((hb & 15) == 0) ? 0 : (hb & 7) == 0 ? 8 : 12);
-        } else {
-            *g = ((all | (uintptr_t)hb) & 7) == 0 ? 8 : 4;
-        }
-        *p = (most + 15) & ~15;
-        if ((*p / 16) % 2 == 0) *p += 16;
-        return true;
+    auto piece = [](const void * base, long long rb, long long hb) {
+        const uintptr_t all = (uintptr_t)base | (uintptr_t)rb;
+        if ((all | (uintptr_t)hb) & 3) return 0;
+        return (all & 15) == 0 ? 16 : ((all | (uintptr_t)hb) & 7) == 0 ? 8 : 4;
     };
-    G->kseg = (int)a.k_hb;
-    G->vseg = (int)a.v_hb;
-    if (!side(a.K, a.k_rb, a.k_hb, &G->kg, &G->kp, G->kseg) || !side(a.V, a.v_rb, a.v_hb, &G->vg, &G->vp, G->vseg))
-        return false;
+    G->nw = nw;
+    G->kg = piece(a.K, a.k_rb, a.k_hb);
+    G->vg = piece(a.V, a.v_rb, a.v_hb);
+    if (!G->kg || !G->vg) return false;
     G->nbk = a.dk / 32;
     G->nbv = a.dv / 32;
-    const int stage = KEYS * (G->kp + G->vp) + KEYS * 4;
-    // as many stages (2 to 4) as leave room for two CTAs and more per SM
-    G->stages = WARPS * 4 * stage <= 76 * 1024 ? 4 : WARPS * 3 * stage <= 108 * 1024 ? 3 : 2;
-    const int join = WARPS * rb * a.dv * 4;
-    G->ring = WARPS * G->stages * stage;
-    if (join > G->ring) G->ring = join;
-    return true;
+    G->qvec = ((uintptr_t)a.q % (a.q_type == KV_TYPE_F32 ? 8 : 4)) == 0 && a.q_stride % 2 == 0;
+    const long long rows = (long long)a.max_q * a.g, qb = (rows + rw - 1) / rw;
+    // all row blocks of a head in one CTA where they fit, so that its rows are read once
+    const long long ngr = (qb + nw - 1) / nw;
+    G->rc = (int)((qb + ngr - 1) / ngr);
+    auto pitch = [&](int hc, long long hb) { return round_pitch(hc * (int)hb + ((hb & 15) ? 15 : 0)); };
+    // as many heads per CTA as leave a stage of 16 keys under 40 KB and a row in a TMA box (256 x 8 bytes)
+    int hc = nw / G->rc < a.Hkv ? nw / G->rc : a.Hkv;
+    while (hc > 1 && (KEYS * (pitch(hc, a.k_hb) + pitch(hc, a.v_hb)) > 40 * 1024 || pitch(hc, a.k_hb) > 2048 ||
+                      pitch(hc, a.v_hb) > 2048))
+        hc--;
+    G->ngh = (a.Hkv + hc - 1) / hc;
+    G->hc = (a.Hkv + G->ngh - 1) / G->ngh;
+    G->kp = pitch(G->hc, a.k_hb);
+    G->vp = pitch(G->hc, a.v_hb);
+    // a stage of about 32 KB (16 to 256 keys), 2 to 8 of them
+    int kt = 32 * 1024 / (KEYS * (G->kp + G->vp)) * KEYS;
+    kt = kt < KEYS ? KEYS : kt > MAX_TILE ? MAX_TILE : kt;
+    // rows side by side in a page that divide the tile: TMA boxes, at most 32 per tile, from 128-byte boundaries
+    int run = 1;
+    while (run < kt && run < a.page && a.page % (2 * run) == 0 && kt % (2 * run) == 0) run *= 2;
+    const bool tma = G->kg == 16 && G->vg == 16 && run >= 8 && G->kp <= 2048 && G->vp <= 2048 &&
+                     (!a.beta || ((uintptr_t)a.beta & 15) == 0);
+    if (tma && kt > 32 * run) kt = 32 * run;
+    G->run = tma ? run : 0;
+    G->by_run = kvc_make_divisor((uint32_t)run);
+    G->bbox = (run * G->hc * 4 + 127) / 128 * 32;
+    if (!tma && kt > 32 * nw) kt = 32 * nw;              // a lane per row of a warp's share
+    *tile = kt;
+    const int bias = tma ? (a.beta ? kt / run * G->bbox * 4 : 0) : kt * G->hc * 4;
+    G->stage_bytes = (kt * (G->kp + G->vp) + bias + 127) & ~127;
+    G->stages = (SMEM_MOST - fixed(nw, G->hc * G->rc)) / G->stage_bytes;
+    if (G->stages > MAX_STAGES) G->stages = MAX_STAGES;
+    return G->stages >= 2;
 }
 
-template <int DB, int NB, int NP>
-size_t smem_bytes(const mma_geom & G) {
-    constexpr int RB = 8 * NB;
-    return (size_t)DB * 2 * NP * NB * 32 * 8 + (DB * RB + RB + 2 * WARPS * RB) * 4 + G.ring;
+using encode_fn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                               const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                               CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+encode_fn encoder() {
+    static const encode_fn fn = [] {
+        void * p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess) {
+            cudaGetLastError();
+            p = nullptr;
+        }
+        return (encode_fn)p;
+    }();
+    return fn;
 }
 
-// CTAs per SM, asked once per shared-memory size and device.
-template <int DB, int NB, int NP>
-int resident(int * ctas, const mma_geom & G) {
-    static std::atomic<uint64_t> known[64];
-    const size_t sm = smem_bytes<DB, NB, NP>(G);
+// Rows of `rb` bytes as 8-byte elements; a box is `pitch` bytes of `run` rows (bytes past the row read as 0).
+bool row_map(CUtensorMap * m, const void * base, long long rb, long long rows, int pitch, int run) {
+    const cuuint64_t dims[2] = {(cuuint64_t)rb / 8, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)rb};
+    const cuuint32_t box[2] = {(cuuint32_t)pitch / 8, (cuuint32_t)run}, one[2] = {1, 1};
+    return encoder()(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT64, 2, const_cast<void *>(base), dims, strides, box, one,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+bool beta_map(CUtensorMap * m, const kvc_attn_args & a, int hc, int run) {
+    const cuuint64_t dims[3] = {(cuuint64_t)a.page, (cuuint64_t)a.Hkv, (cuuint64_t)a.n_pages};
+    const cuuint64_t strides[2] = {(cuuint64_t)a.page * 4, (cuuint64_t)a.page * a.Hkv * 4};
+    const cuuint32_t box[3] = {(cuuint32_t)run, (cuuint32_t)hc, 1}, one[3] = {1, 1, 1};
+    return encoder()(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<float *>(a.beta), dims, strides, box, one,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int DB, int NB, int NP, int MAXW>
+int run(const kvc_attn_args & a, const mma_geom & G, int ngr, cudaStream_t st) {
+    static std::atomic<bool> set[64];
     int dev = 0;
     KVC_CUDA(cudaGetDevice(&dev));
-    const uint64_t v = known[dev & 63].load(std::memory_order_relaxed);
-    if ((v >> 8) == sm) {
-        *ctas = (int)(v & 255);
-        return KVC_OK;
+    auto * k = k_tree_mma<DB, NB, NP, MAXW>;
+    if (!set[dev & 63].load(std::memory_order_relaxed)) {
+        KVC_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MOST));
+        set[dev & 63].store(true, std::memory_order_relaxed);
     }
-    KVC_CUDA(cudaFuncSetAttribute(k_tree_mma<DB, NB, NP>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
-    KVC_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(ctas, k_tree_mma<DB, NB, NP>, THREADS, sm));
-    known[dev & 63].store((uint64_t)sm << 8 | (uint64_t)*ctas, std::memory_order_relaxed);
-    return KVC_OK;
-}
-
-template <int DB, int NB, int NP>
-int run(const kvc_attn_args & a, const mma_geom & G, dim3 grid, cudaStream_t st) {
-    k_tree_mma<DB, NB, NP><<<grid, THREADS, smem_bytes<DB, NB, NP>(G), st>>>(a, G);
+    CUtensorMap maps[3] = {};
+    if (G.run) {
+        const long long rows = (long long)a.n_pages * a.page;
+        if (!row_map(&maps[0], a.K, a.k_rb, rows, G.kp, G.run) || !row_map(&maps[1], a.V, a.v_rb, rows, G.vp, G.run) ||
+            (a.beta && !beta_map(&maps[2], a, G.hc, G.run))) {
+            fprintf(stderr, "[kvc] cuTensorMapEncodeTiled failed for a cache of %d pages\n", a.n_pages);
+            return KVC_ERR_CUDA;
+        }
+    }
+    const int sm = fixed_bytes<DB, NB, NP, MAXW>(G.nw, G.hc * G.rc) + G.stages * G.stage_bytes;
+    k<<<dim3((unsigned)a.W, (unsigned)(G.ngh * ngr)), 32 * G.nw, sm, st>>>(a, G, maps[0], maps[1], maps[2]);
     g_serve_launches++;
     KVC_CUDA(cudaGetLastError());
-    return kvc_launch_attn_join(a, 8 * NB, TILE, st);
+    return kvc_launch_attn_join(a, true, st);
 }
 
-#define TREE_CASE(DB, NB, CALL) \
-    return np == 2 ? CALL<DB, NB, 2> : CALL<DB, NB, 1>
-#define TREE_SELECT(CALL)                              \
-    if (db <= 2) {                                     \
-        if (nb == 1) TREE_CASE(2, 1, CALL);            \
-        if (nb == 2) TREE_CASE(2, 2, CALL);            \
-        TREE_CASE(2, 4, CALL);                         \
-    }                                                  \
-    if (db <= 4) {                                     \
-        if (nb == 1) TREE_CASE(4, 1, CALL);            \
-        if (nb == 2) TREE_CASE(4, 2, CALL);            \
-        TREE_CASE(4, 4, CALL);                         \
-    }                                                  \
-    if (nb == 1) TREE_CASE(8, 1, CALL);                \
-    TREE_CASE(8, 2, CALL)
+using run_fn = int (*)(const kvc_attn_args &, const mma_geom &, int, cudaStream_t);
+struct variant {
+    int db, nb, np, warps;
+    fixed_fn fixed;
+    run_fn run;
+};
+#define TREE_VARIANT(DB, NB, NP, W) {DB, NB, NP, W, fixed_bytes<DB, NB, NP, W>, run<DB, NB, NP, W>}
+// Up to 8 query rows per KV head (single tokens): 16 warps of 8 rows. More rows: 8 warps of 16 rows, whose
+// registers hold twice the output. d > 128: twice that again, 8 warps of 8 rows.
+const variant variants[] = {
+    TREE_VARIANT(2, 1, 1, 16), TREE_VARIANT(2, 1, 2, 16), TREE_VARIANT(4, 1, 1, 16), TREE_VARIANT(4, 1, 2, 16),
+    TREE_VARIANT(2, 2, 1, 8),  TREE_VARIANT(2, 2, 2, 8),  TREE_VARIANT(4, 2, 1, 8),  TREE_VARIANT(4, 2, 2, 8),
+    TREE_VARIANT(8, 1, 1, 8),  TREE_VARIANT(8, 1, 2, 8),
+};
 
-using resident_fn = int (*)(int *, const mma_geom &);
-using run_fn = int (*)(const kvc_attn_args &, const mma_geom &, dim3, cudaStream_t);
-resident_fn select_resident(int db, int nb, int np) { TREE_SELECT(resident); }
-run_fn select_run(int db, int nb, int np) { TREE_SELECT(run); }
+const variant & select(const kvc_attn_args & a) {
+    const int top = a.dk > a.dv ? a.dk : a.dv;
+    const int db = top <= 64 ? 2 : top <= 128 ? 4 : 8;
+    const int nb = db == 8 || (long long)a.max_q * a.g <= 8 ? 1 : 2;
+    const int np = a.q_type == KV_TYPE_F32 ? 2 : 1;
+    for (const variant & v : variants)
+        if (v.db == db && v.nb == nb && v.np == np) return v;
+    return variants[0];
+}
+
+bool plan(const kvc_attn_args & a, mma_geom * G, int * tile, int * ngr) {
+    const variant & v = select(a);
+    if (!geometry(a, 8 * v.nb, v.warps, v.fixed, G, tile)) return false;
+    const long long qb = ((long long)a.max_q * a.g + 8 * v.nb - 1) / (8 * v.nb);
+    const long long n = (qb + G->rc - 1) / G->rc;
+    if (n * G->ngh > 65535 || (G->run && !encoder())) return false;
+    *ngr = (int)n;
+    return true;
+}
 
 }  // namespace
 
-bool kvc_attn_tree_mma_plan(kvc_attn_args * a, int sms, kvc_tree_mma_plan * p) {
-    const int top = a->dk > a->dv ? a->dk : a->dv;
-    const long long rows = (long long)a->max_q * a->g;
-    p->db = top <= 64 ? 2 : top <= 128 ? 4 : 8;
-    p->nb = rows <= 8 ? 1 : rows <= 16 || p->db == 8 ? 2 : 4;
-    p->np = a->q_type == KV_TYPE_F32 ? 2 : 1;
-    p->rb = 8 * p->nb;
-    p->blocks = (rows + p->rb - 1) / p->rb;
+bool kvc_attn_tree_mma_plan(kvc_attn_args * a, int sms, long long * blocks) {
     mma_geom G;
-    if (p->blocks * a->Hkv > 65535 || !geometry(*a, p->rb, &G)) return false;
-    int ctas = 0;
-    if (select_resident(p->db, p->nb, p->np)(&ctas, G) != KVC_OK || ctas < 1) return false;
-    // one wave: every CTA gets an equal stretch of the keys
-    const long long w = (long long)sms * ctas / (p->blocks * a->Hkv);
-    a->W = (int)(w < 1 ? 1 : w);
+    int tile, ngr;
+    if (!plan(*a, &G, &tile, &ngr)) return false;
+    a->rb = 8 * select(*a).nb * G.rc;
+    a->tile = tile;
+    a->by_tile = kvc_make_divisor((uint32_t)tile);
+    const int w = sms / (G.ngh * ngr);                   // one CTA per SM, equal stretches
+    a->W = w < 1 ? 1 : w;
+    *blocks = ngr;
     return true;
 }
 
-int kvc_launch_attn_tree_mma(const kvc_attn_args & a, const kvc_tree_mma_plan & p, cudaStream_t st) {
+int kvc_launch_attn_tree_mma(const kvc_attn_args & a, cudaStream_t st) {
     mma_geom G;
-    if (!geometry(a, p.rb, &G)) return KVC_ERR_SHAPE;
-    return select_run(p.db, p.nb, p.np)(a, G, dim3((unsigned)a.W, (unsigned)(p.blocks * a.Hkv)), st);
+    int tile, ngr;
+    if (!plan(a, &G, &tile, &ngr)) return KVC_ERR_SHAPE;
+    return select(a).run(a, G, ngr, st);
 }
