@@ -44,6 +44,7 @@ struct kvc_attn_args {
     int rb, tile, W;
     kvc_divisor by_tile;
     float * part;           // partial results
+    int * meta;             // [row blocks][n_seqs][2]: first and last worker of a sequence (W > 1)
     int * status;           // set to KVC_ERR_CUDA by a device wait that ran out (or null)
 };
 
@@ -98,8 +99,8 @@ __device__ __forceinline__ bool attn_sees(const kvc_attn_args & a, const kvc_att
 // ---- the split of the keys ---------------------------------------------------
 //
 // For one (KV head, row block) the key tiles of all sequences that
-// have rows in the block are laid end to end, and worker w of W takes tiles
-// [w*T/W, (w+1)*T/W). Sequences of any lengths then load the workers evenly.
+// have rows in the block are laid end to end, and worker w of W (at most T)
+// takes tiles [w*T/W, (w+1)*T/W). Sequences of any lengths then load the workers evenly.
 // A worker's stretch meets at most two sequences that it does not cover whole:
 // the one it starts inside of (slot 0) and the one it ends inside of (slot 1);
 // their partial results go to those slots and are joined afterwards, in the
@@ -112,22 +113,39 @@ __device__ __forceinline__ int attn_tiles(const kvc_attn_args & a, int s, int qb
     return q.ln ? (int)a.by_tile.div((uint32_t)q.ln - 1u) + 1 : 0;
 }
 
-// fn(s, lo, hi, slot) for every piece of worker w's stretch: tiles lo..hi-1 of
-// sequence s; slot -1 where that is all of them. Every warp of a CTA takes the
-// same steps.
+// Worker that holds tile x of T.
+__device__ __forceinline__ int attn_worker(long long x, long long T, int W) {
+    return (int)(((x + 1) * W - 1) / T);
+}
+
+// fn(s, q, lo, hi, slot) for every piece of worker w's stretch: tiles lo..hi-1
+// of sequence s; slot -1 where that is all of them. Every warp of a CTA takes
+// the same steps. note: write which workers share a sequence, for the join.
 template <typename F>
-__device__ __forceinline__ void attn_walk(const kvc_attn_args & a, int qb, int w, F && fn) {
+__device__ __forceinline__ void attn_walk(const kvc_attn_args & a, int qb, int w, bool note, F && fn) {
     const int lane = threadIdx.x & 31;
-    const int mine0 = lane < a.n_seqs ? attn_tiles(a, lane, qb) : 0;
+    auto tiles = [&](const kvc_attn_seq & q) {
+        if ((long long)qb * a.rb >= (long long)q.nq * a.g || !q.ln) return 0;
+        return (int)a.by_tile.div((uint32_t)q.ln - 1u) + 1;
+    };
+    kvc_attn_seq mine{};
+    if (lane < a.n_seqs) mine = attn_seq(a, lane);
+    const int mine0 = tiles(mine);
     long long T = mine0;
     for (int s = lane + 32; s < a.n_seqs; s += 32) T += attn_tiles(a, s, qb);
 #pragma unroll
     for (int o = 16; o; o >>= 1) T += __shfl_xor_sync(~0u, T, o);
-    const long long from = w * T / a.W, to = (w + 1) * T / a.W;
+    const int W = (int)min((long long)a.W, T);           // every worker has a tile
+    if (w >= W) return;
+    const long long from = w * T / W, to = (w + 1) * T / W;
     long long at = 0;
     for (int s0 = 0; s0 < a.n_seqs && at < to; s0 += 32) {
-        const int s = s0 + lane;
-        const int t = s0 == 0 ? mine0 : (s < a.n_seqs ? attn_tiles(a, s, qb) : 0);
+        int t = mine0;
+        if (s0) {
+            mine = kvc_attn_seq{};
+            if (s0 + lane < a.n_seqs) mine = attn_seq(a, s0 + lane);
+            t = tiles(mine);
+        }
         long long p = t;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -136,30 +154,39 @@ __device__ __forceinline__ void attn_walk(const kvc_attn_args & a, int qb, int w
         }
         const long long end = __shfl_sync(~0u, p, 31);
         p += at - t;
-        unsigned hit = __ballot_sync(~0u, t > 0 && p < to && p + t > from);
+        const bool in = t > 0 && p < to && p + t > from;
+        unsigned hit = __ballot_sync(~0u, in);
+        if (note && in && p >= from && a.W > 1) {
+            int * m = a.meta + ((size_t)qb * a.n_seqs + s0 + lane) * 2;
+            m[0] = w;
+            m[1] = attn_worker(p + t - 1, T, W);
+        }
         while (hit) {
             const int l = __ffs(hit) - 1;
             hit &= hit - 1;
             const long long ps = __shfl_sync(~0u, p, l);
             const int ts = __shfl_sync(~0u, t, l);
             const int lo = (int)(max(from, ps) - ps), hi = (int)(min(to, ps + ts) - ps);
-            fn(s0 + l, lo, hi, lo == 0 && hi == ts ? -1 : (from > ps ? 0 : 1));
+            kvc_attn_seq q;
+            q.q0 = __shfl_sync(~0u, mine.q0, l);
+            q.nq = __shfl_sync(~0u, mine.nq, l);
+            q.ln = __shfl_sync(~0u, mine.ln, l);
+            q.k0 = __shfl_sync(~0u, mine.k0, l);
+            q.table = reinterpret_cast<const int *>(__shfl_sync(~0u, (unsigned long long)mine.table, l));
+            fn(s0 + l, q, lo, hi, lo == 0 && hi == ts ? -1 : (from > ps ? 0 : 1));
         }
         at += end;
     }
-}
-
-// Worker that holds tile x of T.
-__device__ __forceinline__ int attn_worker(long long x, long long T, int W) {
-    return (int)(((x + 1) * W - 1) / T);
 }
 
 // Partial results of worker w, slot s: rb sums of d_v, then rb maxima, rb sums.
 __device__ __forceinline__ float * attn_part(const kvc_attn_args & a, int qb, int h, int w, int slot) {
     return a.part + ((((size_t)qb * a.Hkv + h) * a.W + w) * 2 + slot) * ((size_t)a.rb * (a.dv + 2));
 }
-inline size_t kvc_attn_part_bytes(const kvc_attn_args & a, long long blocks) {
-    return a.W > 1 ? (size_t)blocks * a.Hkv * a.W * 2 * a.rb * (a.dv + 2) * sizeof(float) : 0;
+// Workspace bytes: the partial results, then meta.
+inline size_t kvc_attn_part_bytes(const kvc_attn_args & a, long long blocks, size_t * meta_at) {
+    *meta_at = (size_t)blocks * a.Hkv * a.W * 2 * a.rb * (a.dv + 2) * sizeof(float);
+    return a.W > 1 ? *meta_at + (size_t)blocks * a.n_seqs * 2 * sizeof(int) : 0;
 }
 
 // Output row (token, head) from its sum and statistics.

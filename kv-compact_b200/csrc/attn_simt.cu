@@ -36,8 +36,7 @@ __global__ void __launch_bounds__(THREADS) k_attn_simt(const __grid_constant__ k
     const int n_blocks = (int)(((long long)a.max_q * a.g + RB - 1) / RB);
 
     for (int qb = blockIdx.y / a.Hkv; qb < n_blocks; qb += gridDim.y / a.Hkv) {
-    attn_walk(a, qb, w, [&](int s, int lo, int hi, int slot) {
-        const kvc_attn_seq q = attn_seq(a, s);
+    attn_walk(a, qb, w, h == 0 && threadIdx.x < 32, [&](int, const kvc_attn_seq & q, int lo, int hi, int slot) {
         const int r0 = qb * RB;
         const int nr = (int)min((long long)RB, (long long)q.nq * a.g - r0);
         __syncthreads();
@@ -207,36 +206,20 @@ __global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ kvc_a
     const int h = hq / a.g;
     const int rho = i * a.g + (hq - h * a.g);
     const int qb = rho / a.rb, r = rho - qb * a.rb;
-    long long before = 0, T = 0;
-    for (int u = lane; u < a.n_seqs; u += 32) {
-        const int t = attn_tiles(a, u, qb);
-        T += t;
-        if (u < s) before += t;
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        T += __shfl_xor_sync(~0u, T, o);
-        before += __shfl_xor_sync(~0u, before, o);
-    }
-    const int tiles = attn_tiles(a, s, qb);
     const size_t row = (size_t)token * a.Hq + hq;
     cudaGridDependencySynchronize();
-    if (tiles == 0) {
+    if (q.ln == 0) {
         for (int d = threadIdx.x; d < a.dv; d += 128) attn_store(a, row, d, 0.0f, 0.0f, 0.0f);
         return;
     }
-    const int w0 = attn_worker(before, T, a.W), w1 = attn_worker(before + tiles - 1, T, a.W);
-    if (w0 == w1) return;
+    if (a.W == 1) return;
+    const int w0 = a.meta[((size_t)qb * a.n_seqs + s) * 2], w1 = a.meta[((size_t)qb * a.n_seqs + s) * 2 + 1];
+    if (w0 >= w1) return;
+    // the first worker's piece lies in its slot 1 (its stretch began before the sequence or with it), the others' in
+    // slot 0, but for a worker whose stretch begins with the sequence: that is the first one
     const size_t step = 2 * (size_t)a.rb * (a.dv + 2);
-    // slot 1 of the first worker where the sequence starts inside its stretch
-    const int slot0 = (long long)w0 * T / a.W > before ? 0 : 1;
-    const float * base_p = attn_part(a, qb, h, w0, 0);
-    const float * first_p = attn_part(a, qb, h, w0, slot0);
-    auto at = [&](int w) {
-        // a later worker's stretch starts inside the sequence, or with it (w*T/W == before)
-        const bool inside = (long long)w * T / a.W > before;
-        return w == w0 ? first_p : base_p + (size_t)(w - w0) * step + (inside ? 0 : step / 2);
-    };
+    const float * first_p = attn_part(a, qb, h, w0, 1);
+    auto at = [&](int w) { return w == w0 ? first_p : first_p + (size_t)(w - w0) * step - step / 2; };
     float M = -INFINITY;
     for (int w = w0 + lane; w <= w1; w += 32) M = fmaxf(M, at(w)[a.rb * a.dv + r]);
 #pragma unroll

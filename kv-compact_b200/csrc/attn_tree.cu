@@ -10,7 +10,7 @@ namespace {
 struct tree_plan {
     kvc_attn_args a;
     bool use_mma;
-    size_t bytes;
+    size_t bytes, meta_at;
 };
 
 int head_bytes(int type, int d) {
@@ -87,7 +87,7 @@ int make_plan(const kvc_page_cache * c, const kvc_tree_desc * t, int sms, tree_p
         kvc_attn_simt_split(&a, sms, false);
         blocks = ((long long)a.max_q * a.g + a.rb - 1) / a.rb;
     }
-    p->bytes = kvc_attn_part_bytes(a, blocks);
+    p->bytes = kvc_attn_part_bytes(a, blocks, &p->meta_at);
     return KVC_OK;
 }
 
@@ -112,6 +112,7 @@ KVC_EXPORT int kvc_attn_tree(const kvc_page_cache * cache, const kvc_tree_desc *
     if (p.bytes && !workspace) return KVC_ERR_NULL;
     if (p.bytes > workspace_bytes || ((uintptr_t)workspace & 15)) return KVC_ERR_SHAPE;
     p.a.part = static_cast<float *>(workspace);
+    p.a.meta = reinterpret_cast<int *>(static_cast<uint8_t *>(workspace) + p.meta_at);
     if (p.use_mma) return kvc_launch_attn_tree_mma(p.a, (cudaStream_t)stream);
     return kvc_launch_attn_simt(p.a, (cudaStream_t)stream);
 }

@@ -24,7 +24,7 @@
 // the CTA's heads, loaded by TMA in boxes of as many rows as lie side by side
 // in a page. The box is up to 31 bytes wider than that part, so that rows lie an
 // odd number of 16 bytes apart and fragment reads meet no bank conflict. Warp
-// 0 refills the ring between its own steps, two tiles behind the fastest reader.
+// 0 refills the ring between its own steps, a tile or two behind the readers.
 // A warp owns one KV head and one block of query rows for a sequence, takes
 // every nsub-th group of 16 keys, and keeps its own maximum, sum and output;
 // the warps of a head are joined at the end of the CTA's stretch of a
@@ -54,8 +54,10 @@ struct mma_geom {
     int run;                    // rows per TMA box; 0: cp.async
     int bbox;                   // floats between the beta of two boxes
     int stages, stage_bytes;
+    int lag;                    // tiles that a refill stays behind the reader
     int nbk, nbv;               // 32-value blocks per head
-    int qvec;                   // rows of q may be read four elements at a time
+    int qvec;                   // rows of q may be read two elements at a time
+    int ovec;                   // rows of out may be written four at a time
     kvc_divisor by_run;
 };
 
@@ -236,16 +238,9 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void * map, int 
                  :: "r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar)) : "memory");
 }
 
-// Bytes of the region that holds the query fragments (two pieces) in the loop and
-// the outputs that are joined after it.
-template <int DB, int NB, int NP>
-__host__ __device__ constexpr int join_dims() { return DB == 2 ? 64 : 64; }
-template <int DB, int NB, int NP>
-__host__ __device__ inline int shared_region(int nw, int units) {
-    const int frags = NP == 2 ? units * DB * 2 * NB * 32 * 16 : 0;
-    const int join = nw * 8 * NB * (join_dims<DB, NB, NP>() + 4) * 4;
-    return frags > join ? frags : join;
-}
+// One slot of the shared region: a unit's query fragments in two pieces (in the
+// loop), or a warp's output, maxima and sums (when the warps of a unit are joined).
+constexpr int slot_bytes(int db, int nb) { return db * nb * 1024 + nb * 512; }
 
 template <int DB, int NB, int NP, int MAXW>
 __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant__ kvc_attn_args a,
@@ -256,7 +251,7 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
     using namespace kvc_tc;
     constexpr int RW = 8 * NB;                           // query rows of a warp
     constexpr bool QS = NP == 2;                         // query fragments in shared memory
-    constexpr int JD = join_dims<DB, NB, NP>(), JP = JD + 4;
+    constexpr int SLOT = slot_bytes(DB, NB);
     extern __shared__ __align__(128) uint8_t sm[];
     const int NW = G.nw, KT = a.tile;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -269,12 +264,7 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
     int * n_segs = reinterpret_cast<int *>(bad + MAX_STAGES);                // [2]: of this batch, of all
     segment * segs = reinterpret_cast<segment *>(n_segs + 8);
     float * qsum_all = reinterpret_cast<float *>(segs + MAX_SEGS);           // [NW][DB][RW]
-    float * jm = qsum_all + NW * DB * RW;                                    // [NW][RW] maxima, sums; of the units
-    float * jl = jm + NW * RW;
-    float * uM = jl + NW * RW;
-    float * uL = uM + NW * RW;
-    uint4 * qs_all = reinterpret_cast<uint4 *>(uL + NW * RW);                // [units][DB][2][NB][32] (two pieces)
-    float * jo = reinterpret_cast<float *>(qs_all);                          // [NW][RW][JP], after the loop
+    uint8_t * region = reinterpret_cast<uint8_t *>(qsum_all + NW * DB * RW);
     if (threadIdx.x == 0) {
         for (int i = 0; i < G.stages; i++) {
             mbar_init(full + i, tma ? 1 : 64 * NW);
@@ -313,9 +303,8 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
         __syncthreads();
         if (warp == 0) {
             int n = 0;
-            attn_walk(a, qb, w, [&](int s, int lo, int hi, int slot) {
+            attn_walk(a, qb, w, hg == 0, [&](int, const kvc_attn_seq & q, int lo, int hi, int slot) {
                 if (n >= batch && n < batch + MAX_SEGS && lane == 0) {
-                    const kvc_attn_seq q = attn_seq(a, s);
                     segs[n - batch] = segment{lo, hi, slot, q.q0, q.nq, q.ln, (int)((q.table - a.table) / a.max_pages)};
                 }
                 n++;
@@ -404,9 +393,10 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
         };
         if (!tma || warp == 0) {
             if (tma) look();
-            for (int i = 0; i < G.stages - 1; i++) fill();
+            for (int i = 0; i < G.stages - G.lag; i++) fill();
         }
 
+    int units_before = 0;
     for (int seg = 0; seg < ns; seg++) {
         const int lo = segs[seg].lo, hi = segs[seg].hi, slot = segs[seg].slot;
         kvc_attn_seq q;
@@ -417,6 +407,8 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
         const int rows_here = (int)min((long long)a.rb, (long long)q.nq * a.g - (long long)qb * a.rb);
         const int units = nh * ((rows_here + RW - 1) / RW);
         const int nsub = NW / units;
+        if (units != units_before) __syncthreads();      // the units' barriers change hands
+        units_before = units;
         const int sub = warp / units, unit = warp - sub * units;
         const bool active = sub < nsub;
         const int hc = unit % nh, h = h0 + hc;
@@ -429,7 +421,11 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
         // shared memory (32 registers less in the loop), written by a unit's
         // first warp
         uint32_t qf[QS ? 1 : DB][2][NB][2];
-        uint4 * qs = qs_all + (size_t)(active ? unit : 0) * (DB * 2 * NB * 32) + lane;
+        uint4 * qs = reinterpret_cast<uint4 *>(region + (size_t)(active ? unit : 0) * SLOT) + lane;
+        auto unit_sync = [&]() {                         // the warps of a unit
+            if (nsub > 1) asm volatile("bar.sync %0, %1;" :: "r"(1 + unit), "r"(32 * nsub) : "memory");
+            else __syncwarp();
+        };
         float mul[NB][2];
 #pragma unroll
         for (int nb = 0; nb < NB; nb++) {
@@ -515,7 +511,7 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
                 }
             }
         }
-        if (QS) __syncthreads();
+        if (QS && active) unit_sync();
         else __syncwarp();
         float m[NB][2], l[NB][2], O[DB][2][NB][4];
 #pragma unroll
@@ -850,79 +846,121 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
             if (!tma || warp == 0) fill();
         }
 
-        // ---- join the warps of a unit
+        // ---- join the warps of a unit, half of them giving their results to the other half at a time
 #pragma unroll
         for (int nb = 0; nb < NB; nb++)
 #pragma unroll
-            for (int c = 0; c < 2; c++) {
+            for (int c = 0; c < 2; c++)
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) l[nb][c] += __shfl_xor_sync(~0u, l[nb][c], o);
-                if (g == 0) {
-                    jm[warp * RW + 8 * nb + 2 * t + c] = m[nb][c];
-                    jl[warp * RW + 8 * nb + 2 * t + c] = l[nb][c];
+        if (!active) continue;
+        float back = R > -1000 ? scalbnf(1.0f, R - P_SHIFT) : 0.0f;    // of this warp's O
+        if (nsub > 1) unit_sync();                       // the fragments have been read
+        for (int n = nsub; n > 1;) {
+            const int half = (n + 1) / 2;
+            if (sub >= half && sub < n) {
+                float4 * o = reinterpret_cast<float4 *>(region + (size_t)(unit + units * (sub - half)) * SLOT) + lane;
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++) {
+#pragma unroll
+                    for (int b = 0; b < DB; b++)
+#pragma unroll
+                        for (int mt = 0; mt < 2; mt++)
+                            o[((b * 2 + mt) * NB + nb) * 32] = make_float4(O[b][mt][nb][0] * back, O[b][mt][nb][1] * back,
+                                                                           O[b][mt][nb][2] * back, O[b][mt][nb][3] * back);
+                    o[(DB * 2 * NB + nb) * 32] = make_float4(m[nb][0], m[nb][1], l[nb][0], l[nb][1]);
                 }
             }
-        __syncthreads();
-        const float back = R > -1000 ? scalbnf(1.0f, R - P_SHIFT) : 0.0f;
-        float f[NB][2];
+            unit_sync();
+            if (sub < n - half) {
+                const float4 * o = reinterpret_cast<const float4 *>(region + (size_t)(unit + units * sub) * SLOT) + lane;
 #pragma unroll
-        for (int nb = 0; nb < NB; nb++)
+                for (int nb = 0; nb < NB; nb++) {
+                    const float4 ml = o[(DB * 2 * NB + nb) * 32];
+                    float f0[2], f1[2];
 #pragma unroll
-            for (int c = 0; c < 2; c++) {
-                float M = -INFINITY;
-                for (int u = unit; u < units * nsub; u += units) M = fmaxf(M, jm[u * RW + 8 * nb + 2 * t + c]);
-                f[nb][c] = expf(m[nb][c] - (M == -INFINITY ? 0.0f : M)) * back;
-            }
-        for (int e = threadIdx.x; e < units * RW; e += 32 * NW) {
-            float M = -INFINITY, L = 0.0f;
-            for (int u = e; u < units * nsub * RW; u += units * RW) M = fmaxf(M, jm[u]);
-            for (int u = e; u < units * nsub * RW; u += units * RW)
-                L = fmaf(expf(jm[u] - (M == -INFINITY ? 0.0f : M)), jl[u], L);
-            uM[e] = M;
-            uL[e] = L;
-        }
-#pragma unroll
-        for (int b0 = 0; b0 < DB; b0 += JD / 32) {
-            if (b0 >= G.nbv) break;
-            if (active) {
-#pragma unroll
-                for (int b = b0; b < b0 + JD / 32; b++)
-                    if (b < G.nbv) {
-#pragma unroll
-                        for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-                            for (int mt = 0; mt < 2; mt++)
-#pragma unroll
-                                for (int e = 0; e < 4; e++)
-                                    jo[(warp * RW + 8 * nb + 2 * t + (e & 1)) * JP + 32 * (b - b0) + v_dim(vt, mt, g, e >> 1)] =
-                                        O[b][mt][nb][e] * f[nb][e & 1];
+                    for (int c = 0; c < 2; c++) {
+                        const float om = c ? ml.y : ml.x, ol = c ? ml.w : ml.z;
+                        const float mn = fmaxf(m[nb][c], om), base = mn == -INFINITY ? 0.0f : mn;
+                        f0[c] = ex2((m[nb][c] - base) * LOG2E);
+                        f1[c] = ex2((om - base) * LOG2E);
+                        l[nb][c] = l[nb][c] * f0[c] + ol * f1[c];
+                        m[nb][c] = mn;
+                        f0[c] *= back;
                     }
-            }
-            __syncthreads();
-            for (int ur = warp; ur < units * RW; ur += NW) {
-                const int u = ur / RW, r = ur - u * RW;
-                const int block = u / nh, rr = block * RW + r, hh = h0 + u - block * nh;   // row of the CTA's, KV head
-                if (rr >= rows_here) continue;
-                const float M = uM[ur], L = uL[ur];
-                const int row = qb * a.rb + rr, i = (int)a.by_group.div(row);
-                const size_t out = (size_t)(q.q0 + i) * a.Hq + hh * a.g + (row - i * a.g);
-                float * part = slot >= 0 ? attn_part(a, qb, hh, w, slot) : nullptr;
 #pragma unroll
-                for (int c = 0; c < JD; c += 32) {
-                    const int d = 32 * b0 + c + lane;
-                    if (d >= a.dv) continue;
-                    float o = 0.0f;
-                    for (int k = ur; k < units * nsub * RW; k += units * RW) o += jo[k * JP + c + lane];
-                    if (part) part[rr * a.dv + d] = o;
-                    else attn_store(a, out, d, o, M, L);
+                    for (int b = 0; b < DB; b++)
+#pragma unroll
+                        for (int mt = 0; mt < 2; mt++) {
+                            const float4 v = o[((b * 2 + mt) * NB + nb) * 32];
+                            O[b][mt][nb][0] = O[b][mt][nb][0] * f0[0] + v.x * f1[0];
+                            O[b][mt][nb][1] = O[b][mt][nb][1] * f0[1] + v.y * f1[1];
+                            O[b][mt][nb][2] = O[b][mt][nb][2] * f0[0] + v.z * f1[0];
+                            O[b][mt][nb][3] = O[b][mt][nb][3] * f0[1] + v.w * f1[1];
+                        }
                 }
-                if (part && b0 == 0 && lane == 0) {
-                    part[a.rb * a.dv + rr] = M;
-                    part[a.rb * a.dv + a.rb + rr] = L;
-                }
+                back = 1.0f;
             }
-            __syncthreads();
+            n = half;
+            if (n > 1) unit_sync();
         }
+        if (sub == 0) {
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    const int r = 8 * nb + 2 * t + c;
+                    if (r >= nr) continue;
+                    const int rr = r0 - qb * a.rb + r, i = (int)a.by_group.div(r0 + r);
+                    const size_t out = (size_t)(q.q0 + i) * a.Hq + h * a.g + (r0 + r - i * a.g);
+                    float * part = slot >= 0 ? attn_part(a, qb, h, w, slot) : nullptr;
+                    const float M = m[nb][c], L = l[nb][c];
+                    const float mul_o = part ? back : L > 0.0f ? back / L : (L == 0.0f ? 0.0f : L);
+                    if (g == 0) {
+                        if (part) {
+                            part[a.rb * a.dv + rr] = M;
+                            part[a.rb * a.dv + a.rb + rr] = L;
+                        } else if (a.lse) {
+                            a.lse[out] = L == 0.0f ? -INFINITY : M + logf(L);
+                        }
+                    }
+#pragma unroll
+                    for (int b = 0; b < DB; b++) {
+                        if (b >= G.nbv) break;
+                        const float v[4] = {O[b][0][nb][c] * mul_o, O[b][0][nb][2 + c] * mul_o, O[b][1][nb][c] * mul_o,
+                                            O[b][1][nb][2 + c] * mul_o};
+                        if (vt == KV_TYPE_F16) {
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                const int d = 32 * b + v_dim(KV_TYPE_F16, e >> 1, g, e & 1);
+                                if (part) part[rr * a.dv + d] = v[e];
+                                else if (a.q_type == KV_TYPE_F16) reinterpret_cast<__half *>(a.out)[out * a.dv + d] = __float2half_rn(v[e]);
+                                else reinterpret_cast<float *>(a.out)[out * a.dv + d] = v[e];
+                            }
+                        } else {                         // four neighbouring dimensions
+                            const int d = 32 * b + 4 * g;
+                            float * f = part ? part + rr * a.dv + d : reinterpret_cast<float *>(a.out) + out * a.dv + d;
+                            if (part || (a.q_type == KV_TYPE_F32 && G.ovec)) {
+                                *reinterpret_cast<float4 *>(f) = make_float4(v[0], v[1], v[2], v[3]);
+                            } else if (a.q_type == KV_TYPE_F32) {
+#pragma unroll
+                                for (int e = 0; e < 4; e++) f[e] = v[e];
+                            } else {
+                                __half * o = reinterpret_cast<__half *>(a.out) + out * a.dv + d;
+                                if (G.ovec) {
+                                    *reinterpret_cast<uint2 *>(o) = make_uint2(pack(v[0], v[1]), pack(v[2], v[3]));
+                                } else {
+#pragma unroll
+                                    for (int e = 0; e < 4; e++) o[e] = __float2half_rn(v[e]);
+                                }
+                            }
+                        }
+                    }
+                }
+        }
+        // the region is free again (the next piece's fragments go there)
+        if (nsub > 1) unit_sync();
+        else __syncwarp();
     }
         if (n_segs[1] <= batch + MAX_SEGS) break;
     }
@@ -943,8 +981,8 @@ constexpr int SMEM_MOST = 227 * 1024;
 // Shared memory besides the ring, for that many (KV head, row block) units.
 template <int DB, int NB, int NP, int MAXW>
 int fixed_bytes(int nw, int units) {
-    return MAX_STAGES * (8 + 8 + 4) + 32 + MAX_SEGS * (int)sizeof(segment) + nw * 8 * NB * (DB + 4) * 4 +
-           shared_region<DB, NB, NP>(nw, units);
+    const int slots = NP == 2 && units > nw / 2 ? units : nw / 2;
+    return MAX_STAGES * (8 + 8 + 4) + 32 + MAX_SEGS * (int)sizeof(segment) + nw * 8 * NB * DB * 4 + slots * slot_bytes(DB, NB);
 }
 
 // Ring geometry and split, or false where the rows are not ones that the kernel reads.
@@ -962,6 +1000,7 @@ bool geometry(const kvc_attn_args & a, int rw, int nw, fixed_fn fixed, mma_geom 
     if (!G->kg || !G->vg) return false;
     G->nbk = a.dk / 32;
     G->nbv = a.dv / 32;
+    G->ovec = (uintptr_t)a.out % (a.q_type == KV_TYPE_F32 ? 16 : 8) == 0;
     G->qvec = ((uintptr_t)a.q % (a.q_type == KV_TYPE_F32 ? 8 : 4)) == 0 && a.q_stride % 2 == 0;
     const long long rows = (long long)a.max_q * a.g, qb = (rows + rw - 1) / rw;
     // all row blocks of a head in one CTA where they fit, so that its rows are read once
@@ -995,6 +1034,7 @@ bool geometry(const kvc_attn_args & a, int rw, int nw, fixed_fn fixed, mma_geom 
     G->stage_bytes = (kt * (G->kp + G->vp) + bias + 127) & ~127;
     G->stages = (SMEM_MOST - fixed(nw, G->hc * G->rc)) / G->stage_bytes;
     if (G->stages > MAX_STAGES) G->stages = MAX_STAGES;
+    G->lag = G->stages >= 4 ? 2 : 1;
     return G->stages >= 2;
 }
 
