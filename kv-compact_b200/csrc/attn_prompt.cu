@@ -1,5 +1,6 @@
 // attn_prompt.cu — attention over whole prompts (include/kvc-attn.h).
 #include "attn.h"
+#include "attn_prompt.h"
 
 #include <limits.h>
 
@@ -54,6 +55,7 @@ KVC_EXPORT int kvc_attn_prompt(const kvc_prompt_desc * t, void * stream) {
     a.page = 1;
     a.by_page = kvc_make_divisor(1);
     a.by_group = kvc_make_divisor((uint32_t)a.g);
+    if (kvc_attn_prompt_tc_ok(a)) return kvc_launch_attn_prompt_tc(a, (cudaStream_t)stream);
     kvc_attn_simt_split(&a, sms, true);
     return kvc_launch_attn_simt(a, (cudaStream_t)stream);
 }
