@@ -717,6 +717,28 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
                         return;
                     }
                     const int e = top ? max((int)(top >> 10), 1) - 15 : -14;    // |scale| < 2^(e+1)
+                    if (own) {
+                        // a node's row with scales far above the others' is not to cost the queries that do not see it
+                        // their precision
+                        int least = e;
+                        if (R == -1000) {
+#pragma unroll
+                            for (int b = 0; b < DB; b++)
+                                if (b < G.nbv) {
+                                    const uint32_t x[4] = {dl[b] & 0x7FFFu, dl[b] >> 16 & 0x7FFFu, dh[b] & 0x7FFFu, dh[b] >> 16 & 0x7FFFu};
+#pragma unroll
+                                    for (int u = 0; u < 4; u++)
+                                        if (x[u]) least = min(least, max((int)(x[u] >> 10), 1) - 15);
+                                }
+                            least = __reduce_min_sync(~0u, least);
+                        } else {
+                            least = R;
+                        }
+                        if (e > least + 8) {
+                            by_value();
+                            return;
+                        }
+                    }
                     if (e > R) {
                         if (R > -1000) {
                             const float fr = scalbnf(1.0f, R - e);
@@ -812,8 +834,16 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
                 }
             };
             if (vt == KV_TYPE_F16) {
+                if (hidden) {                            // rows that no query of the head sees: zeros, whatever they hold
+                    for (int k = 0; k < KEYS; k++)
+                        if (key_bias(k) == -INFINITY)
+                            for (int o = lane; o < 4 * G.nbv; o += 32)
+                                *reinterpret_cast<int4 *>(const_cast<uint8_t *>(vs) + k * G.vp + 16 * o) = make_int4(0, 0, 0, 0);
+                    fence_smem_to_async();               // the next box goes over them
+                    __syncwarp();
+                }
                 bool bad = false;
-                if (own || hidden)
+                if (own)
                     for (int k = 0; k < KEYS; k++)
                         for (int d = lane; d < 32 * G.nbv; d += 32) bad |= (lds16(vs + k * G.vp + 2 * d) & 0x7C00u) == 0x7C00u;
                 if (__any_sync(~0u, bad)) by_value();

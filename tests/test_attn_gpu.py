@@ -1,0 +1,490 @@
+"""Attention over prompts and paged caches against the definition in 64 bits.
+
+Tolerances: a score is the sum of products exact to 22 bits (fp16 pieces) added in fp32, so it is off by at most
+A 2^-21 with A = max sum |q||k| scale, and x = score + beta and its scaling to base 2 add 2^-22 |x|; the exponential adds
+2^-22. A probability's relative error is that sum e, the output's is 2 e max|V| (numerator and denominator). With F16
+queries P times the row scale is rounded to fp16 once, 2^-11 (half an eps), the output once more; Q4_1 rounds two such
+products and the sum of minimum and centre.
+"""
+import math
+
+import pytest
+import torch
+
+import servref as R
+from kvc_b200 import attn
+
+pytestmark = pytest.mark.gpu
+
+
+def bounds(q, K, V, x_max, kind_v, f16, scale):
+    A = float((q.double().abs().flatten(0, 1) @ K.abs().flatten(0, -2).t()).max()) * scale if K.numel() else 0.0
+    e = A * 2.0 ** -21 + (A + x_max) * 2.0 ** -22 + 2.0 ** -21
+    v = float(V.abs().max()) if V.numel() else 0.0
+    out = 2 * e * v + 2.0 ** -21 * v
+    if f16:
+        out += (4 if kind_v == R.Q4_1 else 2) * 2.0 ** -11 * v
+    return out, 2 * e + 2.0 ** -21
+
+
+def check(got, want, tol, what):
+    got = got.double()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), what
+    inf = torch.isinf(want)
+    assert torch.equal(got[inf], want[inf]), what
+    d = (got - want)[~inf & ~torch.isnan(want)].abs()
+    assert d.numel() == 0 or float(d.max()) <= tol, f"{what}: {float(d.max()):.3e} > {tol:.3e}"
+
+
+def tree_case(kvc, lens, nodes, hkv=2, g=4, dk=64, dv=64, kt=R.Q8_0, vt=R.Q8_0, page=16, beta=False, qt=torch.float16, seed=0,
+              mask="tree", edit=None, layers=1, layer=0, seqs=None):
+    total = [n + m for n, m in zip(lens, nodes)]
+    c = R.Cache(total, hkv, dk, dv, kt, vt, page, layers=layers, beta=beta, seed=seed)
+    gen = torch.Generator().manual_seed(seed + 1)
+    q = torch.randn(sum(nodes), hkv * g, dk, generator=gen).to("cuda", qt)
+    cu = [0]
+    for m in nodes:
+        cu.append(cu[-1] + m)
+    words = max(1, -(-max(nodes + [1]) // 32))
+    parents = [[int(torch.randint(-1, i, (1,), generator=gen)) if i else -1 for i in range(m)] for m in nodes]
+    bits = attn.tree_mask(parents, words) if mask == "tree" else torch.zeros(sum(nodes), words, dtype=torch.int32)
+    seqs = list(range(len(lens))) if seqs is None else seqs
+    if edit:
+        edit(c, q)
+    h = c.handle(kvc)
+    dev = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    t = attn.Tree(kvc, h, q, dev(cu), dev(seqs), mask=None if mask is None else bits.cuda(), max_nodes=max(nodes + [1]),
+                  scale=dk ** -0.5, layer=layer)
+
+    def see(i, m, n):
+        s = torch.ones(m, n, dtype=torch.bool)
+        if mask is None:
+            return s
+        for a in range(m):
+            for b in range(m):
+                if n - m + b >= 0:
+                    s[a, n - m + b] = bool((int(bits[cu[i] + a, b // 32]) >> (b % 32)) & 1)
+        return s
+
+    want = c.attend(q, cu, seqs, see, dk ** -0.5, layer)
+    return c, q, t, want
+
+
+def tree_check(kvc, **kw):
+    c, q, t, (out, lse) = tree_case(kvc, **kw)
+    layer = kw.get("layer", 0)
+    K, V = R.decode(c.K[layer], c.kt), R.decode(c.V[layer], c.vt)
+    used = torch.cat([c.rows(s) for s in range(len(kw["lens"]))] + [torch.zeros(0, dtype=torch.long, device="cuda")])
+    K, V = K[used].view(-1, c.hkv, c.dk), V[used]
+    fin = torch.isfinite(K).all() and torch.isfinite(V).all()
+    xb = 0.0 if c.beta is None else float(torch.nan_to_num(c.beta, 0.0, 0.0, 0.0).abs().clamp(max=1e4).max())
+    K = torch.nan_to_num(K, 0.0, 0.0, 0.0) if not fin else K
+    V = torch.nan_to_num(V, 0.0, 0.0, 0.0) if not fin else V
+    o_tol, l_tol = bounds(q, K, V, xb, c.vt, q.dtype == torch.float16, c.dk ** -0.5)
+    t.out.fill_(7.0)
+    t.lse.fill_(7.0)
+    t.run()
+    torch.cuda.synchronize()
+    check(t.out, out, o_tol, "out")
+    check(t.lse, lse, l_tol, "lse")
+    first = t.out.clone(), t.lse.clone()
+    t.run()
+    torch.cuda.synchronize()
+    assert torch.equal(first[0], t.out) and torch.equal(first[1], t.lse)       # the same bits every time
+    assert int(c.status) == 0
+    return t
+
+
+KINDS = [R.F32, R.F16, R.Q8_0, R.Q4_0, R.Q4_1]
+
+
+@pytest.mark.parametrize("qt", [torch.float16, torch.float32])
+@pytest.mark.parametrize("vt", KINDS)
+@pytest.mark.parametrize("kt", KINDS)
+def test_tree_types(kvc, kt, vt, qt):
+    tree_check(kvc, lens=[130, 0, 7], nodes=[3, 1, 5], kt=kt, vt=vt, qt=qt, beta=kt != vt, seed=kt * 10 + vt)
+
+
+@pytest.mark.parametrize("dk,dv", [(32, 32), (64, 128), (128, 64), (96, 96), (128, 128), (256, 256), (192, 160), (256, 64)])
+@pytest.mark.parametrize("kind", [R.F16, R.Q8_0, R.Q4_1])
+@pytest.mark.parametrize("qt", [torch.float16, torch.float32])
+def test_tree_head_sizes(kvc, dk, dv, kind, qt):
+    tree_check(kvc, lens=[77, 300], nodes=[1, 9], hkv=2, g=2, dk=dk, dv=dv, kt=kind, vt=kind, qt=qt, beta=True, seed=dk + dv)
+
+
+@pytest.mark.parametrize("dk,dv", [(8, 8), (40, 24), (1, 3), (250, 33)])
+@pytest.mark.parametrize("kind", [R.F16, R.F32])
+def test_tree_odd_head_sizes(kvc, dk, dv, kind):
+    tree_check(kvc, lens=[50, 3], nodes=[2, 1], hkv=3, g=1, dk=dk, dv=dv, kt=kind, vt=kind, qt=torch.float32, seed=dk)
+
+
+@pytest.mark.parametrize("hkv", [1, 2, 3, 5, 8, 17])
+@pytest.mark.parametrize("g", [1, 3, 8])
+def test_tree_heads(kvc, hkv, g):
+    tree_check(kvc, lens=[200, 31], nodes=[1, 1], hkv=hkv, g=g, dk=64, dv=64, kt=R.Q8_0, vt=R.Q4_0, beta=True, seed=hkv)
+    tree_check(kvc, lens=[40], nodes=[6], hkv=hkv, g=g, dk=64, dv=64, kt=R.F16, vt=R.Q8_0, seed=g)
+
+
+@pytest.mark.parametrize("page", [1, 3, 8, 12, 16, 24, 40, 64, 100, 256])
+@pytest.mark.parametrize("kind", [R.F16, R.Q8_0])
+def test_tree_pages(kvc, page, kind):
+    for hkv in (4, 3):
+        tree_check(kvc, lens=[333, 15, 64], nodes=[2, 1, 17], hkv=hkv, g=2, kt=kind, vt=kind, page=page, beta=True, seed=page)
+
+
+@pytest.mark.parametrize("n", [0, 1, 15, 16, 17, 63, 64, 65, 1000, 5001])
+@pytest.mark.parametrize("qt", [torch.float16, torch.float32])
+def test_tree_lengths(kvc, n, qt):
+    tree_check(kvc, lens=[n], nodes=[1], hkv=8, g=4, dk=128, dv=128, page=16, qt=qt, beta=True, seed=n)
+
+
+@pytest.mark.parametrize("nodes", [[2], [33], [64, 1, 30], [100], [0, 5, 0]])
+@pytest.mark.parametrize("g", [1, 4])
+def test_tree_nodes(kvc, nodes, g):
+    tree_check(kvc, lens=[100] * len(nodes), nodes=nodes, g=g, dk=128, dv=128, kt=R.F16, vt=R.F16, seed=sum(nodes))
+    tree_check(kvc, lens=[20] * len(nodes), nodes=nodes, g=g, kt=R.Q4_0, vt=R.Q8_0, qt=torch.float32, seed=sum(nodes))
+
+
+def test_tree_many_sequences(kvc):
+    lens = [(i * 37) % 90 for i in range(150)]
+    tree_check(kvc, lens=lens, nodes=[1 + i % 3 for i in range(150)], hkv=1, g=2, kt=R.Q8_0, vt=R.F16, page=8, beta=True)
+    tree_check(kvc, lens=lens, nodes=[1] * 150, hkv=4, g=2, kt=R.Q8_0, vt=R.Q8_0, page=32)
+
+
+def test_tree_without_mask_sees_all(kvc):
+    tree_check(kvc, lens=[40, 3], nodes=[4, 2], mask=None)
+    tree_check(kvc, lens=[40, 3], nodes=[4, 2], mask=None, kt=R.F32, vt=R.F32)
+
+
+@pytest.mark.parametrize("kind", [R.F32, R.F16, R.Q8_0])
+def test_tree_rows_that_see_nothing(kvc, kind):
+    """No cached rows and an empty mask, or beta of -inf on every row: output 0, log-sum-exp -inf."""
+    t = tree_check(kvc, lens=[0, 20], nodes=[3, 2], kt=kind, vt=kind, mask="none")
+    assert float(t.out[:3].abs().max()) == 0.0 and bool((t.lse[:3] == -math.inf).all())
+    t = tree_check(kvc, lens=[33, 5], nodes=[1, 1], kt=kind, vt=kind, beta=True,
+                   edit=lambda c, q: c.beta.fill_(-math.inf))
+    assert float(t.out.abs().max()) == 0.0 and bool((t.lse == -math.inf).all())
+
+
+@pytest.mark.parametrize("kind", [R.F32, R.F16, R.Q8_0, R.Q4_1])
+@pytest.mark.parametrize("qt", [torch.float16, torch.float32])
+def test_tree_lowest_beta(kvc, kind, qt):
+    """beta of the type's lowest value is a finite bias: alone it leaves a plain average, next to others nothing."""
+    low = torch.finfo(torch.float32).min
+    tree_check(kvc, lens=[40], nodes=[1], kt=kind, vt=kind, qt=qt, beta=True, edit=lambda c, q: c.beta.fill_(low))
+
+    def some(c, q):
+        c.beta[..., ::3] = low
+    tree_check(kvc, lens=[40], nodes=[1], kt=kind, vt=kind, qt=qt, beta=True, edit=some)
+
+
+@pytest.mark.parametrize("kind", [R.F32, R.F16, R.Q8_0, R.Q4_0, R.Q4_1])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, 60000.0])
+def test_tree_hidden_rows_may_hold_anything(kvc, kind, bad):
+    """Rows hidden by beta, by the mask, behind a sequence's end, or in free pages."""
+    def edit(c, q):
+        rows = c.rows(0)
+        hidden = [int(rows[5]), int(rows[16]), int(rows[40])]
+        for r in hidden:
+            c.beta[0, r // c.page, :, r % c.page] = -math.inf
+        own = c.rows(1)[-1:].tolist()                  # the last node's own row: the others do not see it
+        free = [r for r in range(c.n_pages * c.page) if r not in set(torch.cat([c.rows(0), c.rows(1)]).tolist())]
+        for store, t in ((c.K, c.kt), (c.V, c.vt)):
+            for r in hidden + own + free:
+                if t == R.F32:
+                    store[0, r].view(torch.float32).fill_(bad)
+                elif t == R.F16:
+                    store[0, r].view(torch.float16).fill_(bad)
+                else:
+                    b = store[0, r].view(-1, R.BLOCK[t])
+                    b[:, :2] = torch.tensor([bad], dtype=torch.float16).view(torch.uint8).to(b.device)
+    for qt in (torch.float16, torch.float32):
+        c, q, t, (out, lse) = tree_case(kvc, lens=[50, 20], nodes=[1, 4], kt=kind, vt=kind, beta=True, page=16, qt=qt,
+                                        edit=edit, seed=3)
+        t.run()
+        torch.cuda.synchronize()
+        # the last node sees its own row and gets what that gives; everybody else is as if it were not there
+        ok = torch.ones(5, dtype=torch.bool, device="cuda")
+        ok[4] = False
+        assert bool(torch.isfinite(t.out[ok]).all()) and bool(torch.isfinite(t.lse[ok]).all())
+        assert float((t.out[ok].double() - out[ok]).abs().max()) <= 4 * 2.0 ** -11 * 5
+        if not math.isfinite(bad):
+            assert not bool(torch.isfinite(t.out[4]).all())
+
+
+def test_tree_large_and_small_scales(kvc):
+    """Block scales from fp16's largest to its subnormals, queries far from 1."""
+    for size in (1e-6, 1e-2, 3e3):
+        def edit(c, q):
+            for store, t in ((c.K, c.kt), (c.V, c.vt)):
+                b = store[0].view(-1, R.BLOCK[t])
+                d = b[:, :2].contiguous().view(torch.float16).float() * size
+                b[:, :2] = d.half().view(torch.uint8)
+            q.mul_(1.0 / size)
+        for kind in (R.Q8_0, R.Q4_1):
+            tree_check(kvc, lens=[100], nodes=[1], kt=kind, vt=kind, qt=torch.float32, edit=edit, seed=11)
+
+
+def test_tree_bad_pages_and_slots(kvc):
+    """Entries outside the pool count as no rows; an id outside the cache as an empty sequence."""
+    for hkv, page, kt in ((2, 16, R.Q8_0), (3, 16, R.Q8_0), (2, 16, R.F32), (2, 5, R.F16)):
+        c, q, t, _ = tree_case(kvc, lens=[60], nodes=[1], hkv=hkv, page=page, kt=kt, vt=kt, qt=torch.float32, beta=True)
+        c.table[0, 1], c.table[0, 2] = -1, c.n_pages
+        t.run()
+        torch.cuda.synchronize()
+        n = int(c.seq_len[0])
+        keep = [r for r in range(n) if r // page not in (1, 2)]
+        table = c.table[0].tolist()
+        rows = torch.tensor([table[r // page] * page + r % page for r in keep], device="cuda")
+        K, V = R.decode(c.K[0][rows], kt).view(-1, hkv, 64), R.decode(c.V[0][rows], kt).view(-1, hkv, 64)
+        for h in range(q.shape[1]):
+            bias = c.beta[0, rows // page, h // 4, rows % page]
+            o, w = R.attend(q[:, h], K[:, h // 4], V[:, h // 4], bias, torch.ones(1, len(keep), dtype=torch.bool, device="cuda"),
+                            64 ** -0.5)
+            assert float((t.out[:, h].double() - o).abs().max()) < 1e-4 and float((t.lse[:, h].double() - w).abs().max()) < 1e-4
+    c, q, t, _ = tree_case(kvc, lens=[60, 5], nodes=[1, 1], seqs=[0, 1])
+    dev = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    for ids in ([0, 99], [0, -1]):
+        u = attn.Tree(kvc, c.handle(kvc), q, dev([0, 1, 2]), dev(ids), max_nodes=1)
+        u.out.fill_(3.0)
+        u.run()
+        torch.cuda.synchronize()
+        assert float(u.out[1].abs().max()) == 0.0 and bool((u.lse[1] == -math.inf).all())
+
+
+def test_tree_layers_strides_and_rows_behind(kvc):
+    """Another layer of the cache, queries in a wider tensor, output rows that belong to no entry."""
+    tree_check(kvc, lens=[90, 20], nodes=[1, 3], layers=3, layer=2, beta=True)
+    c, q, t, (out, lse) = tree_case(kvc, lens=[90, 20], nodes=[1, 3], qt=torch.float32)
+    wide = torch.randn(6, 3 * 8, 64, device="cuda")
+    wide[:4, 8:16] = q
+    dev = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    mask = torch.zeros(6, 1, dtype=torch.int32, device="cuda")
+    mask[:4] = t._keep[3]
+    for view in (wide[:, 8:16], wide.flatten(1)[:, 8 * 64 + 0:16 * 64].view(6, 8, 64)):
+        u = attn.Tree(kvc, c.handle(kvc), view, dev([0, 1, 4]), dev([0, 1]), mask=mask, max_nodes=3, scale=64 ** -0.5)
+        u.out.fill_(5.0)
+        u.lse.fill_(5.0)
+        u.run()
+        torch.cuda.synchronize()
+        assert bool((u.out[4:] == 5.0).all()) and bool((u.lse[4:] == 5.0).all())
+        assert float((u.out[:4].double() - out).abs().max()) < 1e-4
+    # entries with more nodes than max_nodes are cut to it
+    u = attn.Tree(kvc, c.handle(kvc), view, dev([0, 1, 4]), dev([0, 1]), mask=mask, max_nodes=1, scale=64 ** -0.5)
+    u.out.fill_(5.0)
+    u.run()
+    torch.cuda.synchronize()
+    assert bool((u.out[2:] == 5.0).all()) and float((u.out[0].double() - out[0]).abs().max()) < 1e-4
+
+
+def test_tree_on_a_stream_and_in_a_graph(kvc):
+    c, q, t, (out, _) = tree_case(kvc, lens=[3000, 100], nodes=[1, 2], qt=torch.float32, hkv=4, dk=128, dv=128)
+    t.run()
+    torch.cuda.synchronize()
+    want = t.out.clone()
+    side = torch.cuda.Stream()
+    t.out.zero_()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        t.run()
+    side.synchronize()
+    assert torch.equal(t.out, want)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        t.run()
+        t.run()
+    t.out.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(t.out, want)
+    # a longer sequence and other queries, the same graph
+    c.seq_len[0] = 1500
+    q.copy_(torch.randn_like(q))
+    g.replay()
+    torch.cuda.synchronize()
+    bits = t._keep[3].cpu()
+    cu = [0, 1, 3]
+
+    def see(i, m, n):
+        s = torch.ones(m, n, dtype=torch.bool)
+        for a in range(m):
+            for b in range(m):
+                s[a, n - m + b] = bool((int(bits[cu[i] + a, 0]) >> b) & 1)
+        return s
+    out, _ = c.attend(q, cu, [0, 1], see, 128 ** -0.5)
+    assert float((t.out.double() - out).abs().max()) < 2e-4
+
+
+def test_tree_refuses_a_small_workspace(kvc):
+    c, q, t, _ = tree_case(kvc, lens=[3000], nodes=[1])
+    cache, desc, ws, size = t._args
+    assert size > 0
+    assert t.fn(cache, desc, ws, size - 1, None) == -13
+    assert t.fn(cache, desc, None, size, None) == -1
+    assert t.fn(cache, desc, ws + 4, size, None) == -13
+
+
+# ---- prompts ------------------------------------------------------------------------------
+
+def prompt_case(new, past, hkv=2, g=4, dk=64, dv=64, dtype=torch.float16, causal=True, seed=0, wide=False, scale=None, edit=None):
+    gen = torch.Generator().manual_seed(seed)
+    nk = [a + b for a, b in zip(new, past)]
+    rnd = lambda *s: torch.randn(*s, generator=gen).to("cuda", dtype)  # noqa: E731
+    q, k, v = rnd(sum(new), hkv * g, dk), rnd(sum(nk), hkv, dk), rnd(sum(nk), hkv, dv)
+    if wide:                                           # slices of one fused projection
+        fused = rnd(sum(new), hkv * (g * dk + dk + dv))
+        fused[:, :hkv * g * dk] = q.flatten(1)
+        fused[:, hkv * g * dk:hkv * (g + 1) * dk] = k.flatten(1)
+        fused[:, hkv * (g + 1) * dk:] = v.flatten(1)
+        q = fused[:, :hkv * g * dk].unflatten(1, (hkv * g, dk))
+        k = fused[:, hkv * g * dk:hkv * (g + 1) * dk].unflatten(1, (hkv, dk))
+        v = fused[:, hkv * (g + 1) * dk:].unflatten(1, (hkv, dv))
+    if edit:
+        edit(q, k, v)
+    cum = lambda x: torch.tensor([sum(x[:i]) for i in range(len(x) + 1)], dtype=torch.int32, device="cuda")  # noqa: E731
+    scale = dk ** -0.5 if scale is None else scale
+    out = torch.zeros(sum(new), hkv * g, dv, dtype=torch.float64, device="cuda")
+    lse = torch.zeros(sum(new), hkv * g, dtype=torch.float64, device="cuda")
+    a0 = b0 = 0
+    for a, b in zip(new, nk):
+        i, j = torch.arange(a, device="cuda")[:, None], torch.arange(b, device="cuda")[None]
+        see = (j <= i + b - a) if causal else (j >= 0) & (i >= 0)
+        for h in range(hkv * g):
+            out[a0:a0 + a, h], lse[a0:a0 + a, h] = R.attend(q[a0:a0 + a, h], k[b0:b0 + b, h // g].double(),
+                                                            v[b0:b0 + b, h // g].double(), None, see, scale)
+        a0, b0 = a0 + a, b0 + b
+    return q, k, v, cum(new), cum(nk), scale, out, lse
+
+
+def prompt_check(kvc, *args, **kw):
+    q, k, v, cu_q, cu_k, scale, out, lse = prompt_case(*args, **kw)
+    p = attn.Prompt(kvc, q, k, v, cu_q, cu_k, scale=scale, causal=kw.get("causal", True))
+    o_tol, l_tol = bounds(q, k.double(), v.double(), 0.0, R.F16, q.dtype == torch.float16, abs(scale))
+    p.out.fill_(7.0)
+    p.run()
+    torch.cuda.synchronize()
+    check(p.out, out, o_tol, "out")
+    check(p.lse, lse, l_tol, "lse")
+    first = p.out.clone()
+    p.run()
+    torch.cuda.synchronize()
+    assert torch.equal(first, p.out)
+    return p
+
+
+@pytest.mark.parametrize("d", [8, 40, 64, 72, 96, 128])
+@pytest.mark.parametrize("g", [1, 3, 4])
+def test_prompt_head_sizes(kvc, d, g):
+    prompt_check(kvc, [130, 1, 70], [0, 0, 0], g=g, dk=d, dv=d, seed=d)
+
+
+@pytest.mark.parametrize("dk,dv", [(64, 128), (128, 64), (32, 96), (136, 64), (256, 256), (20, 20), (7, 5)])
+def test_prompt_other_head_sizes(kvc, dk, dv):
+    prompt_check(kvc, [50, 20], [10, 0], dk=dk, dv=dv, seed=dk)
+
+
+@pytest.mark.parametrize("n", [1, 2, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 257, 600])
+def test_prompt_lengths(kvc, n):
+    prompt_check(kvc, [n], [0], dk=128, dv=128, seed=n)
+    prompt_check(kvc, [n], [0], g=1, seed=n, causal=False)
+
+
+@pytest.mark.parametrize("past", [1, 100, 128, 511])
+def test_prompt_on_past_rows(kvc, past):
+    prompt_check(kvc, [65, 3, 1], [past, 0, past + 1], dk=128, dv=128, seed=past)
+
+
+@pytest.mark.parametrize("g", [1, 2, 5, 7, 16, 128, 130])
+def test_prompt_groups(kvc, g):
+    prompt_check(kvc, [40, 9], [5, 0], hkv=1, g=g, seed=g)
+
+
+def test_prompt_many_sequences(kvc):
+    new = [(i * 29) % 50 for i in range(90)]
+    prompt_check(kvc, new, [(i * 7) % 13 for i in range(90)], hkv=2, g=2)
+
+
+def test_prompt_fewer_keys_than_queries(kvc):
+    """Queries that lie before the first key see nothing; a sequence without keys as well."""
+    p = prompt_check(kvc, [100, 5], [-60, -5], dk=128, dv=128)
+    assert float(p.out[:60].abs().max()) == 0.0 and bool((p.lse[:60] == -math.inf).all())
+    assert float(p.out[100:].abs().max()) == 0.0
+    prompt_check(kvc, [7], [-7])
+    prompt_check(kvc, [100, 5], [-60, -5], dtype=torch.float32)
+
+
+def test_prompt_strides(kvc):
+    prompt_check(kvc, [70, 20], [0, 0], dk=64, dv=64, wide=True)
+    prompt_check(kvc, [70, 20], [0, 0], hkv=1, g=2, dk=24, dv=8, wide=True)
+    prompt_check(kvc, [70, 20], [0, 0], hkv=3, g=1, dk=12, dv=4, wide=True)       # strides that are no multiple of 16 bytes
+
+
+def test_prompt_f32_and_scales(kvc):
+    prompt_check(kvc, [70, 20], [3, 0], dtype=torch.float32, dk=96, dv=128)
+    for scale in (0.0, -0.3, 1.0):
+        prompt_check(kvc, [70, 20], [3, 0], scale=scale)
+
+
+def test_prompt_growing_maximum(kvc):
+    """Scores that rise along the keys move the reference maximum at every step."""
+    def edit(q, k, v):
+        q.abs_()
+        k.abs_()
+        k.mul_(torch.linspace(0, 6, k.shape[0], device="cuda")[:, None, None].half())
+    prompt_check(kvc, [700], [0], dk=64, dv=64, scale=0.5, edit=edit)
+
+
+def test_prompt_neighbours_never_matter(kvc):
+    """A sequence between others full of NaN and infinities, and rows behind the last one."""
+    q, k, v, cu_q, cu_k, scale, out, lse = prompt_case([40, 70, 33], [0, 20, 0], dk=128, dv=128)
+    for bad in (math.nan, math.inf):
+        for t in (q, k, v):
+            t[:40] = bad
+            t[-33:] = bad
+        p = attn.Prompt(kvc, q, k, v, cu_q, cu_k, scale=scale)
+        p.run()
+        torch.cuda.synchronize()
+        assert float((p.out[40:110].double() - out[40:110]).abs().max()) < 2 * 2.0 ** -11 * 5
+        assert bool(torch.isfinite(p.lse[40:110]).all())
+    cu_q[3], cu_k[3] = cu_q[2], cu_k[2]                # the last sequence is empty: its rows are nobody's
+    p.out.fill_(9.0)
+    p.run()
+    torch.cuda.synchronize()
+    assert bool((p.out[110:] == 9.0).all())
+
+
+def test_prompt_on_a_stream_and_in_a_graph(kvc):
+    q, k, v, cu_q, cu_k, scale, out, lse = prompt_case([300, 20], [0, 0], dk=128, dv=128)
+    p = attn.Prompt(kvc, q, k, v, cu_q, cu_k, scale=scale)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        p.run()
+    side.synchronize()
+    want = p.out.clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        p.run()
+    p.out.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(p.out, want) and float((want.double() - out).abs().max()) < 2 * 2.0 ** -11 * 5
+
+
+def test_wrappers_check_their_tensors(kvc):
+    q, k = torch.randn(4, 4, 64, device="cuda").half(), torch.randn(4, 2, 64, device="cuda").half()
+    cu = torch.tensor([0, 4], dtype=torch.int32, device="cuda")
+    for args in ((q.bfloat16(), k.bfloat16(), k.bfloat16(), cu), (q, k.float(), k, cu), (q, k, k, cu.long()),
+                 (q, k[:3], k, cu), (q[:, :3], k, k, cu), (q.cpu(), k, k, cu), (q, k, k, cu, cu[:1]),
+                 (q.transpose(1, 2), k, k, cu)):
+        with pytest.raises(ValueError):
+            attn.Prompt(kvc, *args)
+    c = R.Cache([10], 2, 64, 64, R.Q8_0, R.Q8_0, 16)
+    h, s = c.handle(kvc), torch.zeros(1, dtype=torch.int32, device="cuda")
+    for args, kw in (((q[..., :32], cu, s), {}), ((q, cu[:1], s), {}), ((q, cu, s.long()), {}), ((q.bfloat16(), cu, s), {}),
+                     ((q, cu, s), dict(mask=torch.zeros(3, 1, dtype=torch.int32, device="cuda"))),
+                     ((q, cu, s), dict(out=torch.empty(4, 4, 64, device="cuda")))):
+        with pytest.raises(ValueError):
+            attn.Tree(kvc, h, *args, max_nodes=4, **kw)
+    with pytest.raises(RuntimeError):
+        attn.Tree(kvc, h, q, cu, s, max_nodes=4, layer=1)
