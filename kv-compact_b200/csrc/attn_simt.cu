@@ -178,12 +178,14 @@ __global__ void __launch_bounds__(THREADS) k_attn_simt(const __grid_constant__ k
 
 // One CTA per (token, query head): the rows whose keys were split over several
 // workers, joined in the workers' order, and rows of sequences without keys.
-// Sequences that one worker covered are written already. The four warps take
-// every fourth partial result each, several in flight; bound by the latency of
-// those reads. What does not depend on the kernel before is done first, while
-// that one still runs.
+// Sequences that one worker covered are written already. Bound by the latency of
+// its reads, so they are few and side by side: which workers share the sequence
+// (meta), then all maxima and sums, then the outputs, four values a lane and
+// eight partial results in flight per warp. What does not depend on the kernel
+// before is done first, while that one still runs.
+constexpr int JOIN_MOST = 512;                           // partial results whose factors fit shared memory at a time
 __global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ kvc_attn_args a) {
-    __shared__ float s_l[4], s_o[4][KVC_MAX_D];
+    __shared__ float s_f[JOIN_MOST], s_o[4][KVC_MAX_D], s_red[8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int token = (int)(blockIdx.x / (unsigned)a.Hq), hq = (int)(blockIdx.x - (unsigned)token * (unsigned)a.Hq);
     // the sequence of the token
@@ -215,34 +217,83 @@ __global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ kvc_a
     if (a.W == 1) return;
     const int w0 = a.meta[((size_t)qb * a.n_seqs + s) * 2], w1 = a.meta[((size_t)qb * a.n_seqs + s) * 2 + 1];
     if (w0 >= w1) return;
-    // the first worker's piece lies in its slot 1 (its stretch began before the sequence or with it), the others' in
-    // slot 0, but for a worker whose stretch begins with the sequence: that is the first one
+    // the first worker's piece lies in its slot 1 (its stretch began before the sequence or with it), the others' in slot 0
     const size_t step = 2 * (size_t)a.rb * (a.dv + 2);
     const float * first_p = attn_part(a, qb, h, w0, 1);
     auto at = [&](int w) { return w == w0 ? first_p : first_p + (size_t)(w - w0) * step - step / 2; };
+    auto over = [&](float v, bool largest) {             // of all threads
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            const float u = __shfl_xor_sync(~0u, v, o);
+            v = largest ? fmaxf(v, u) : v + u;
+        }
+        float * red = s_red + (largest ? 0 : 4);
+        if (lane == 0) red[warp] = v;
+        __syncthreads();
+        return largest ? fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])) : (red[0] + red[1]) + (red[2] + red[3]);
+    };
+    const int n = w1 - w0 + 1;
     float M = -INFINITY;
-    for (int w = w0 + lane; w <= w1; w += 32) M = fmaxf(M, at(w)[a.rb * a.dv + r]);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, o));
+    for (int k = threadIdx.x; k < n; k += 128) M = fmaxf(M, at(w0 + k)[a.rb * a.dv + r]);
+    M = over(M, true);
     const float base = M == -INFINITY ? 0.0f : M;
-    float L = 0.0f, O[KVC_MAX_D / 32];
+    const bool wide = (a.dv & 3) == 0;                   // the partial results' rows lie on 16-byte boundaries
+    float L = 0.0f;
+    float4 O[2] = {make_float4(0, 0, 0, 0), make_float4(0, 0, 0, 0)};
+    float O1[KVC_MAX_D / 32];
 #pragma unroll
-    for (int c = 0; c < KVC_MAX_D / 32; c++) O[c] = 0.0f;
-#pragma unroll 4
-    for (int w = w0 + warp; w <= w1; w += 4) {
-        const float * p = at(w);
-        const float f = expf(p[a.rb * a.dv + r] - base);
-        L = fmaf(f, p[a.rb * a.dv + a.rb + r], L);
+    for (int c = 0; c < KVC_MAX_D / 32; c++) O1[c] = 0.0f;
+    for (int k0 = 0; k0 < n; k0 += JOIN_MOST) {
+        const int m = min(n - k0, JOIN_MOST);
+        __syncthreads();
+        for (int k = threadIdx.x; k < m; k += 128) {
+            const float * p = at(w0 + k0 + k) + a.rb * a.dv + r;
+            const float f = expf(p[0] - base);
+            s_f[k] = f;
+            L = fmaf(f, p[a.rb], L);
+        }
+        __syncthreads();
+        if (wide) {
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                const int d = 4 * lane + 128 * c;
+                if (d >= a.dv) break;
+                for (int k = warp; k < m; k += 32) {
+                    float4 v[8];
+#pragma unroll
+                    for (int u = 0; u < 8; u++)
+                        if (k + 4 * u < m) v[u] = *reinterpret_cast<const float4 *>(at(w0 + k0 + k + 4 * u) + r * a.dv + d);
+#pragma unroll
+                    for (int u = 0; u < 8; u++)
+                        if (k + 4 * u < m) {
+                            const float f = s_f[k + 4 * u];
+                            O[c].x = fmaf(f, v[u].x, O[c].x);
+                            O[c].y = fmaf(f, v[u].y, O[c].y);
+                            O[c].z = fmaf(f, v[u].z, O[c].z);
+                            O[c].w = fmaf(f, v[u].w, O[c].w);
+                        }
+                }
+            }
+        } else {
+            for (int k = warp; k < m; k += 4) {
+                const float * p = at(w0 + k0 + k) + r * a.dv;
+                const float f = s_f[k];
+#pragma unroll
+                for (int c = 0; c < KVC_MAX_D / 32; c++)
+                    if (lane + 32 * c < a.dv) O1[c] = fmaf(f, p[lane + 32 * c], O1[c]);
+            }
+        }
+    }
+    if (wide) {
+#pragma unroll
+        for (int c = 0; c < 2; c++)
+            if (4 * lane + 128 * c < a.dv) *reinterpret_cast<float4 *>(&s_o[warp][4 * lane + 128 * c]) = O[c];
+    } else {
 #pragma unroll
         for (int c = 0; c < KVC_MAX_D / 32; c++)
-            if (lane + 32 * c < a.dv) O[c] = fmaf(f, p[r * a.dv + lane + 32 * c], O[c]);
+            if (lane + 32 * c < a.dv) s_o[warp][lane + 32 * c] = O1[c];
     }
-    if (lane == 0) s_l[warp] = L;
-#pragma unroll
-    for (int c = 0; c < KVC_MAX_D / 32; c++)
-        if (lane + 32 * c < a.dv) s_o[warp][lane + 32 * c] = O[c];
-    __syncthreads();
-    L = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
+    L = over(L, false);
     for (int d = threadIdx.x; d < a.dv; d += 128)
         attn_store(a, row, d, (s_o[0][d] + s_o[1][d]) + (s_o[2][d] + s_o[3][d]), M, L);
 }

@@ -262,7 +262,8 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
     uint64_t * empty = full + MAX_STAGES;
     uint32_t * bad = reinterpret_cast<uint32_t *>(empty + MAX_STAGES);       // [stages] boxes without a page
     int * n_segs = reinterpret_cast<int *>(bad + MAX_STAGES);                // [2]: of this batch, of all
-    segment * segs = reinterpret_cast<segment *>(n_segs + 8);
+    int * pages = n_segs + 8;                                                // [32]
+    segment * segs = reinterpret_cast<segment *>(pages + 32);
     float * qsum_all = reinterpret_cast<float *>(segs + MAX_SEGS);           // [NW][DB][RW]
     uint8_t * region = reinterpret_cast<uint8_t *>(qsum_all + NW * DB * RW);
     if (threadIdx.x == 0) {
@@ -319,13 +320,16 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
 
         // ---- filling: the next tile of the batch, in order
         int p_seg = 0, p_tile = ns > 0 ? segs[0].lo : 0;
-        int p_page = -1;                                 // TMA: page of box `lane` of that tile, read ahead
+        // TMA: the page of box `lane` of that tile, read ahead by an asynchronous copy (a load into a register would be
+        // waited for at the end of the refill)
+        int * p_page = pages + lane;
         auto look = [&]() {
-            p_page = -1;
             if (p_seg < ns) {
                 const segment & S = segs[p_seg];
                 const long long j = (long long)p_tile * KT + lane * G.run;
-                if (lane * G.run < KT && j < S.ln) p_page = a.table[(size_t)S.table * a.max_pages + a.by_page.div((uint32_t)j)];
+                if (lane * G.run < KT && j < S.ln)
+                    copy_async<4>(smem_u32(p_page), reinterpret_cast<const uint8_t *>(
+                                                       a.table + (size_t)S.table * a.max_pages + a.by_page.div((uint32_t)j)));
             }
         };
         auto fill = [&]() {
@@ -340,7 +344,9 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
                 const int k = lane * G.run;
                 const long long j = (long long)p_tile * KT + k;
                 const bool want = k < KT && j < S.ln;
-                const bool have = want && p_page >= 0 && p_page < a.n_pages && !dead;
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                const int page = want ? *p_page : -1;
+                const bool have = page >= 0 && page < a.n_pages && !dead;
                 const uint32_t boxes = __ballot_sync(~0u, have), missing = __ballot_sync(~0u, want && !have);
                 if (lane == 0) {
                     bad[p_stage] = missing;
@@ -350,10 +356,10 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
                 __syncwarp();
                 if (have) {
                     const int off = (int)(j - (long long)a.by_page.div((uint32_t)j) * a.page);
-                    const int row = p_page * a.page + off;
+                    const int row = page * a.page + off;
                     tma_load_2d(st + k * G.kp, &k_map, (k_at - k_off) >> 3, row, bar);
                     tma_load_2d(sv + k * G.vp, &v_map, (v_at - v_off) >> 3, row, bar);
-                    if (a.beta) tma_load_3d(smem_addr(sb + lane * G.bbox), &b_map, off, h0, p_page, bar);
+                    if (a.beta) tma_load_3d(smem_addr(sb + lane * G.bbox), &b_map, off, h0, page, bar);
                 }
             } else {
                 // rows warp, warp + NW, ...; lane r knows the place of the r-th of them
@@ -414,7 +420,9 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
         const int hc = unit % nh, h = h0 + hc;
         const int r0 = qb * a.rb + unit / nh * RW;
         const int nr = min(RW, rows_here - unit / nh * RW);
-        const int first_own = q.ln - q.nq;               // rows from here on are the nodes' own
+        // rows from here on are the nodes' own, and the mask decides on them (one node that sees itself needs none)
+        const bool masked = a.mask && a.mask_words > 0 && !(q.nq == 1 && (a.mask[(size_t)q.q0 * a.mask_words] & 1u));
+        const int first_own = masked || (a.mask && !a.mask_words) ? q.ln - q.nq : INT_MAX;
 
         // query fragments: lane (g, t) holds, of row g of each block of 8, the
         // elements that the k-steps of its K type ask of it; two pieces lie in
@@ -605,7 +613,7 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
             }
 
             // ---- softmax: running maximum per row (the 8 lane groups hold the keys), probabilities
-            const bool own = a.mask && j0 + KEYS > first_own;          // the group holds rows that the mask decides on
+            const bool own = j0 + KEYS > first_own;          // the group holds rows that the mask decides on
             const bool hidden = __any_sync(~0u, b0 == -INFINITY || b1 == -INFINITY);
             bool moved = false;
             float f[NB][2];
@@ -835,17 +843,24 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
             };
             if (vt == KV_TYPE_F16) {
                 if (hidden) {                            // rows that no query of the head sees: zeros, whatever they hold
-                    for (int k = 0; k < KEYS; k++)
-                        if (key_bias(k) == -INFINITY)
-                            for (int o = lane; o < 4 * G.nbv; o += 32)
-                                *reinterpret_cast<int4 *>(const_cast<uint8_t *>(vs) + k * G.vp + 16 * o) = make_int4(0, 0, 0, 0);
+                    unsigned rows = __ballot_sync(~0u, lane < KEYS && key_bias(lane & (KEYS - 1)) == -INFINITY);
+                    while (rows) {
+                        const int k = __ffs(rows) - 1;
+                        rows &= rows - 1;
+                        for (int o = lane; o < 4 * G.nbv; o += 32)
+                            *reinterpret_cast<int4 *>(const_cast<uint8_t *>(vs) + k * G.vp + 16 * o) = make_int4(0, 0, 0, 0);
+                    }
                     fence_smem_to_async();               // the next box goes over them
                     __syncwarp();
                 }
                 bool bad = false;
                 if (own)
                     for (int k = 0; k < KEYS; k++)
-                        for (int d = lane; d < 32 * G.nbv; d += 32) bad |= (lds16(vs + k * G.vp + 2 * d) & 0x7C00u) == 0x7C00u;
+                        for (int o = lane; o < 4 * G.nbv; o += 32) {
+                            const uint4 v = *reinterpret_cast<const uint4 *>(vs + k * G.vp + 16 * o);
+                            for (uint32_t x : {v.x, v.y, v.z, v.w})
+                                bad |= (x & 0x7C00u) == 0x7C00u || (x & 0x7C000000u) == 0x7C000000u;
+                        }
                 if (__any_sync(~0u, bad)) by_value();
                 else product(kvc_int<KV_TYPE_F16>{});
             } else if (vt == KV_TYPE_Q8_0) {
@@ -1012,7 +1027,7 @@ constexpr int SMEM_MOST = 227 * 1024;
 template <int DB, int NB, int NP, int MAXW>
 int fixed_bytes(int nw, int units) {
     const int slots = NP == 2 && units > nw / 2 ? units : nw / 2;
-    return MAX_STAGES * (8 + 8 + 4) + 32 + MAX_SEGS * (int)sizeof(segment) + nw * 8 * NB * DB * 4 + slots * slot_bytes(DB, NB);
+    return MAX_STAGES * (8 + 8 + 4) + 32 + 128 + MAX_SEGS * (int)sizeof(segment) + nw * 8 * NB * DB * 4 + slots * slot_bytes(DB, NB);
 }
 
 // Ring geometry and split, or false where the rows are not ones that the kernel reads.
