@@ -23,8 +23,8 @@
 // ring of stages, each `tile` whole rows: the part of every row that belongs to
 // the CTA's heads, loaded by TMA in boxes of as many rows as lie side by side
 // in a page. The box is up to 31 bytes wider than that part, so that rows lie an
-// odd number of 16 bytes apart and fragment reads meet no bank conflict. Warp
-// 0 refills the ring between its own steps, a tile or two behind the readers.
+// odd number of 16 bytes apart and fragment reads meet no bank conflict. The
+// warps take turns at refilling the ring, a tile or two behind the readers.
 // A warp owns one KV head and one block of query rows for a sequence, takes
 // every nsub-th group of 16 keys, and keeps its own maximum, sum and output;
 // the warps of a head are joined at the end of the CTA's stretch of a
@@ -262,8 +262,8 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
     uint64_t * empty = full + MAX_STAGES;
     uint32_t * bad = reinterpret_cast<uint32_t *>(empty + MAX_STAGES);       // [stages] boxes without a page
     int * n_segs = reinterpret_cast<int *>(bad + MAX_STAGES);                // [2]: of this batch, of all
-    int * pages = n_segs + 8;                                                // [32]
-    segment * segs = reinterpret_cast<segment *>(pages + 32);
+    int * pages = n_segs + 8;                                                // [NW][32]
+    segment * segs = reinterpret_cast<segment *>(pages + 32 * NW);
     float * qsum_all = reinterpret_cast<float *>(segs + MAX_SEGS);           // [NW][DB][RW]
     uint8_t * region = reinterpret_cast<uint8_t *>(qsum_all + NW * DB * RW);
     if (threadIdx.x == 0) {
@@ -290,8 +290,9 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
             if (a.status) *a.status = KVC_ERR_CUDA;
         }
     };
-    int p_stage = 0, c_stage = 0;                        // next stage to fill / to read
-    uint32_t p_phase = 1, c_phase = 0;
+    int c_stage = 0;                                     // next stage to read
+    uint32_t c_phase = 0;
+    int filled = 0;                                      // tiles of the batches before
     auto step = [&](int & st, uint32_t & ph) {
         if (++st == G.stages) {
             st = 0;
@@ -318,38 +319,49 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
         __syncthreads();
         const int ns = n_segs[0];
 
-        // ---- filling: the next tile of the batch, in order
-        int p_seg = 0, p_tile = ns > 0 ? segs[0].lo : 0;
-        // TMA: the page of box `lane` of that tile, read ahead by an asynchronous copy (a load into a register would be
-        // waited for at the end of the refill)
-        int * p_page = pages + lane;
+        // ---- filling: with TMA tile f of the batch is the business of warp f % NW alone (so that no warp has more to
+        // do than another), with cp.async every warp's
+        const int stride = tma ? NW : 1;
+        int f_tile = tma ? warp : 0;                     // this warp's next tile to fill: its number in the batch,
+        int f_seg = 0, f_at = ns > 0 ? segs[0].lo : 0;   // its piece and its tile there
+        auto ahead = [&](int n) {
+            f_at += n;
+            while (f_seg < ns && f_at >= segs[f_seg].hi) {
+                f_at -= segs[f_seg].hi;
+                if (++f_seg < ns) f_at += segs[f_seg].lo;
+            }
+        };
+        if (tma) ahead(warp);
+        // TMA: the page of box `lane` of that tile, read ahead by an asynchronous copy
+        int * p_page = pages + 32 * warp + lane;
         auto look = [&]() {
-            if (p_seg < ns) {
-                const segment & S = segs[p_seg];
-                const long long j = (long long)p_tile * KT + lane * G.run;
+            if (f_seg < ns) {
+                const segment & S = segs[f_seg];
+                const long long j = (long long)f_at * KT + lane * G.run;
                 if (lane * G.run < KT && j < S.ln)
                     copy_async<4>(smem_u32(p_page), reinterpret_cast<const uint8_t *>(
                                                        a.table + (size_t)S.table * a.max_pages + a.by_page.div((uint32_t)j)));
             }
         };
         auto fill = [&]() {
-            if (p_seg >= ns) return;
-            const segment & S = segs[p_seg];
-            await(empty + p_stage, p_phase);
-            uint8_t * st = ring + (size_t)p_stage * G.stage_bytes;
+            if (f_seg >= ns) return;
+            const segment & S = segs[f_seg];
+            const int num = filled + f_tile, stage = num % G.stages;
+            await(empty + stage, (num / G.stages & 1) ^ 1);
+            uint8_t * st = ring + (size_t)stage * G.stage_bytes;
             uint8_t * sv = st + KT * G.kp;
             float * sb = reinterpret_cast<float *>(sv + KT * G.vp);
-            uint64_t * bar = full + p_stage;
+            uint64_t * bar = full + stage;
             if (tma) {
                 const int k = lane * G.run;
-                const long long j = (long long)p_tile * KT + k;
+                const long long j = (long long)f_at * KT + k;
                 const bool want = k < KT && j < S.ln;
                 asm volatile("cp.async.wait_all;" ::: "memory");
                 const int page = want ? *p_page : -1;
                 const bool have = page >= 0 && page < a.n_pages && !dead;
                 const uint32_t boxes = __ballot_sync(~0u, have), missing = __ballot_sync(~0u, want && !have);
                 if (lane == 0) {
-                    bad[p_stage] = missing;
+                    bad[stage] = missing;
                     const uint32_t bytes = (uint32_t)G.run * (uint32_t)(G.kp + G.vp + (a.beta ? 4 * G.hc : 0));
                     mbar_arrive_expect_tx(bar, bytes * (uint32_t)__popc(boxes));
                 }
@@ -364,7 +376,7 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
             } else {
                 // rows warp, warp + NW, ...; lane r knows the place of the r-th of them
                 const int k0 = warp + NW * lane;
-                const long long j = (long long)p_tile * KT + k0;
+                const long long j = (long long)f_at * KT + k0;
                 int row = -1;
                 if (k0 < KT && j < S.ln) {
                     const int b = (int)a.by_page.div((uint32_t)j);
@@ -391,16 +403,13 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
                 asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(smem_addr(bar)) : "memory");
                 mbar_arrive(bar);
             }
-            step(p_stage, p_phase);
-            if (++p_tile == S.hi) {
-                if (++p_seg < ns) p_tile = segs[p_seg].lo;
-            }
+            f_tile += stride;
+            ahead(stride);
             if (tma) look();
         };
-        if (!tma || warp == 0) {
-            if (tma) look();
-            for (int i = 0; i < G.stages - G.lag; i++) fill();
-        }
+        if (tma) look();
+        while (f_seg < ns && f_tile < G.stages - G.lag) fill();
+        int tile = 0;                                    // of the batch, being read
 
     int units_before = 0;
     for (int seg = 0; seg < ns; seg++) {
@@ -888,7 +897,8 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
             __syncwarp();
             if (lane == 0) mbar_arrive(empty + c_stage);
             step(c_stage, c_phase);
-            if (!tma || warp == 0) fill();
+            if (f_tile == tile + G.stages - G.lag) fill();
+            tile++;
         }
 
         // ---- join the warps of a unit, half of them giving their results to the other half at a time
@@ -1007,6 +1017,7 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
         if (nsub > 1) unit_sync();
         else __syncwarp();
     }
+        filled += tile;
         if (n_segs[1] <= batch + MAX_SEGS) break;
     }
     if (dead && threadIdx.x < G.stages) {                // copies in flight land before the CTA ends
@@ -1027,7 +1038,7 @@ constexpr int SMEM_MOST = 227 * 1024;
 template <int DB, int NB, int NP, int MAXW>
 int fixed_bytes(int nw, int units) {
     const int slots = NP == 2 && units > nw / 2 ? units : nw / 2;
-    return MAX_STAGES * (8 + 8 + 4) + 32 + 128 + MAX_SEGS * (int)sizeof(segment) + nw * 8 * NB * DB * 4 + slots * slot_bytes(DB, NB);
+    return MAX_STAGES * (8 + 8 + 4) + 32 + nw * 128 + MAX_SEGS * (int)sizeof(segment) + nw * 8 * NB * DB * 4 + slots * slot_bytes(DB, NB);
 }
 
 // Ring geometry and split, or false where the rows are not ones that the kernel reads.
