@@ -205,6 +205,11 @@ int kvc_launch_attn_join(const kvc_attn_args & a, bool overlap, cudaStream_t st)
 void kvc_attn_simt_split(kvc_attn_args * a, int sms, bool whole);
 int kvc_launch_attn_simt(const kvc_attn_args & a, cudaStream_t st);
 
+// Bytes of a 32-value block.
+__host__ __device__ __forceinline__ constexpr int kvc_block_size(int type) {
+    return type == KV_TYPE_Q8_0 ? 34 : type == KV_TYPE_Q4_0 ? 18 : type == KV_TYPE_Q4_1 ? 20 : type == KV_TYPE_F16 ? 64 : 128;
+}
+
 // ---- stored elements -----------------------------------------------------------
 // Element e of a row's head segment at p (block types: segments start on a block).
 __device__ __forceinline__ float attn_half(const uint8_t * p) {        // 2-byte aligned

@@ -22,14 +22,13 @@
 // multiply-adds) and the tensor cores about equally at d = 128.
 #include "attn.h"
 #include "attn_prompt.h"
-#include "tc_sm100.h"
-
-#include <cuda.h>
+#include "attn_tc.h"
 #include <math.h>
 
 namespace {
 
 using namespace kvc_tc;
+using namespace kvc_attn_tc;
 
 constexpr int TM = 128, TN = 128;               // rows and keys of a tile
 constexpr int THREADS = 320;
@@ -47,70 +46,6 @@ struct cfg {
     static constexpr uint32_t COLS = 512;
 };
 
-// Shared-memory descriptors of tiles whose rows are 128 bytes, 128-byte swizzled
-// as TMA writes them (start addresses below are multiples of 16 bytes).
-// K-major operand (rows = M or N, 64 values of K a row): groups of 8 rows 1,024 bytes apart.
-__device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
-    return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
-           (uint64_t)2 << 61;
-}
-// N-major operand (rows = K, 64 values of N a row): blocks of 64 N `next` bytes apart, groups of 8 K 1,024 bytes.
-__device__ __forceinline__ uint64_t desc_n(uint32_t addr, uint32_t next) {
-    return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)(next >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
-           (uint64_t)2 << 61;
-}
-
-// D[tmem] (+)= A[tmem] B[smem], fp16 operands.
-__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n"
-        :: "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc));
-}
-
-#define KVC_R8(r, o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7])
-#define KVC_I8(r, o) "r"(r[o]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]), "r"(r[o + 7])
-// 32 consecutive columns of this thread's lane, without waiting.
-__device__ __forceinline__ void ld32(uint32_t addr, uint32_t * r) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : KVC_R8(r, 0), KVC_R8(r, 8), KVC_R8(r, 16), KVC_R8(r, 24) : "r"(addr));
-}
-__device__ __forceinline__ void st32(uint32_t addr, const uint32_t * r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
-        :: "r"(addr), KVC_I8(r, 0), KVC_I8(r, 8), KVC_I8(r, 16), KVC_I8(r, 24) : "memory");
-}
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ uint32_t pack(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-// Two fp32 operations in one instruction.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    unsigned long long x, y, z, d;
-    memcpy(&x, &a, 8), memcpy(&y, &b, 8), memcpy(&z, &c, 8);
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(x), "l"(y), "l"(z));
-    float2 r;
-    memcpy(&r, &d, 8);
-    return r;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    unsigned long long x, y, d;
-    memcpy(&x, &a, 8), memcpy(&y, &b, 8);
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(x), "l"(y));
-    float2 r;
-    memcpy(&r, &d, 8);
-    return r;
-}
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void * map, int x, int y, int z, uint64_t * bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
                  :: "r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar)) : "memory");
@@ -410,30 +345,13 @@ __global__ void __launch_bounds__(THREADS, 1) k_prompt_tc(const __grid_constant_
     }
 }
 
-using encode_fn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                               const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                               CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-encode_fn encoder() {
-    static const encode_fn fn = [] {
-        void * p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
-            q != cudaDriverEntryPointSuccess) {
-            cudaGetLastError();
-            p = nullptr;
-        }
-        return (encode_fn)p;
-    }();
-    return fn;
-}
-
 // [tokens][heads][d] F16 with the given byte strides; boxes of 64 values x `heads` x `rows` (values past d read as 0).
 bool rows_map(CUtensorMap * m, const void * base, int d, int heads, int tokens, long long head_bytes, long long token_bytes,
               int box_heads, int box_rows) {
     const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)(tokens > 0 ? tokens : 1)};
     const cuuint64_t strides[2] = {(cuuint64_t)head_bytes, (cuuint64_t)token_bytes};
     const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_rows}, one[3] = {1, 1, 1};
-    return encoder()(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(base), dims, strides, box, one,
+    return kvc_tensor_map_encoder()(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(base), dims, strides, box, one,
                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -467,7 +385,7 @@ bool kvc_attn_prompt_tc_ok(const kvc_attn_args & a) {
     for (long long x : {a.q_stride * 2, a.q_head * 2, a.k_rb, a.k_hb, a.v_rb, a.v_hb})
         if (x <= 0 || x >= 1LL << 40) return false;
     const long long tiles = a.n_total / (2 * (TM / a.g)) + a.n_seqs;
-    return a.n_keys > 0 && tiles * a.Hkv <= INT32_MAX && encoder() != nullptr;
+    return a.n_keys > 0 && tiles * a.Hkv <= INT32_MAX && kvc_tensor_map_encoder() != nullptr;
 }
 
 int kvc_launch_attn_prompt_tc(const kvc_attn_args & a, cudaStream_t st) {

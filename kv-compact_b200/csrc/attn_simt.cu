@@ -8,6 +8,7 @@
 //
 // in one pass over the keys with a running m, l and sum (flash decoding).
 #include "attn.h"
+#include "attn_tc.h"
 
 #include <math.h>
 
@@ -352,4 +353,18 @@ int kvc_launch_attn_join(const kvc_attn_args & a, bool overlap, cudaStream_t st)
     KVC_CUDA(cudaLaunchKernelEx(&cfg, k_attn_join, a));
     g_serve_launches++;
     return KVC_OK;
+}
+
+kvc_encode_fn kvc_tensor_map_encoder() {
+    static const kvc_encode_fn fn = [] {
+        void * p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess) {
+            cudaGetLastError();
+            p = nullptr;
+        }
+        return (kvc_encode_fn)p;
+    }();
+    return fn;
 }

@@ -9,7 +9,7 @@ namespace {
 
 struct tree_plan {
     kvc_attn_args a;
-    bool use_mma;
+    enum { SIMT, MMA, TC } kernel;
     size_t bytes, meta_at;
 };
 
@@ -82,8 +82,12 @@ int make_plan(const kvc_page_cache * c, const kvc_tree_desc * t, int sms, tree_p
         return KVC_OK;
     }
     long long blocks = 0;
-    p->use_mma = kvc_attn_tree_mma_plan(&a, sms, &blocks);
-    if (!p->use_mma) {
+    if (kvc_attn_tree_tc_plan(&a, sms, &blocks)) {
+        p->kernel = tree_plan::TC;
+    } else if (kvc_attn_tree_mma_plan(&a, sms, &blocks)) {
+        p->kernel = tree_plan::MMA;
+    } else {
+        p->kernel = tree_plan::SIMT;
         kvc_attn_simt_split(&a, sms, false);
         blocks = ((long long)a.max_q * a.g + a.rb - 1) / a.rb;
     }
@@ -113,7 +117,8 @@ KVC_EXPORT int kvc_attn_tree(const kvc_page_cache * cache, const kvc_tree_desc *
     if (p.bytes > workspace_bytes || ((uintptr_t)workspace & 15)) return KVC_ERR_SHAPE;
     p.a.part = static_cast<float *>(workspace);
     p.a.meta = reinterpret_cast<int *>(static_cast<uint8_t *>(workspace) + p.meta_at);
-    if (p.use_mma) return kvc_launch_attn_tree_mma(p.a, (cudaStream_t)stream);
+    if (p.kernel == tree_plan::TC) return kvc_launch_attn_tree_tc(p.a, (cudaStream_t)stream);
+    if (p.kernel == tree_plan::MMA) return kvc_launch_attn_tree_mma(p.a, (cudaStream_t)stream);
     return kvc_launch_attn_simt(p.a, (cudaStream_t)stream);
 }
 

@@ -33,9 +33,7 @@
 // by side) are copied by all warps with cp.async instead.
 #include "attn.h"
 #include "attn_tree.h"
-#include "tc_sm100.h"
-
-#include <cuda.h>
+#include "attn_tc.h"
 
 namespace {
 
@@ -1094,28 +1092,11 @@ bool geometry(const kvc_attn_args & a, int rw, int nw, fixed_fn fixed, mma_geom 
     return G->stages >= 2;
 }
 
-using encode_fn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                               const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                               CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-encode_fn encoder() {
-    static const encode_fn fn = [] {
-        void * p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
-            q != cudaDriverEntryPointSuccess) {
-            cudaGetLastError();
-            p = nullptr;
-        }
-        return (encode_fn)p;
-    }();
-    return fn;
-}
-
 // Rows of `rb` bytes as 8-byte elements; a box is `pitch` bytes of `run` rows (bytes past the row read as 0).
 bool row_map(CUtensorMap * m, const void * base, long long rb, long long rows, int pitch, int run) {
     const cuuint64_t dims[2] = {(cuuint64_t)rb / 8, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)rb};
     const cuuint32_t box[2] = {(cuuint32_t)pitch / 8, (cuuint32_t)run}, one[2] = {1, 1};
-    return encoder()(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT64, 2, const_cast<void *>(base), dims, strides, box, one,
+    return kvc_tensor_map_encoder()(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT64, 2, const_cast<void *>(base), dims, strides, box, one,
                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -1123,7 +1104,7 @@ bool beta_map(CUtensorMap * m, const kvc_attn_args & a, int hc, int run) {
     const cuuint64_t dims[3] = {(cuuint64_t)a.page, (cuuint64_t)a.Hkv, (cuuint64_t)a.n_pages};
     const cuuint64_t strides[2] = {(cuuint64_t)a.page * 4, (cuuint64_t)a.page * a.Hkv * 4};
     const cuuint32_t box[3] = {(cuuint32_t)run, (cuuint32_t)hc, 1}, one[3] = {1, 1, 1};
-    return encoder()(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<float *>(a.beta), dims, strides, box, one,
+    return kvc_tensor_map_encoder()(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<float *>(a.beta), dims, strides, box, one,
                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -1184,7 +1165,7 @@ bool plan(const kvc_attn_args & a, mma_geom * G, int * tile, int * ngr) {
     if (!geometry(a, 8 * v.nb, v.warps, v.fixed, G, tile)) return false;
     const long long qb = ((long long)a.max_q * a.g + 8 * v.nb - 1) / (8 * v.nb);
     const long long n = (qb + G->rc - 1) / G->rc;
-    if (n * G->ngh > 65535 || (G->run && !encoder())) return false;
+    if (n * G->ngh > 65535 || (G->run && !kvc_tensor_map_encoder())) return false;
     *ngr = (int)n;
     return true;
 }
