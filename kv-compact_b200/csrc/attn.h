@@ -106,77 +106,81 @@ __device__ __forceinline__ bool attn_sees(const kvc_attn_args & a, const kvc_att
 // their partial results go to those slots and are joined afterwards, in the
 // workers' order.
 
-// Key tiles of sequence s in row block qb (blocks of a.rb rows, tiles of a.tile keys).
-__device__ __forceinline__ int attn_tiles(const kvc_attn_args & a, int s, int qb) {
-    const kvc_attn_seq q = attn_seq(a, s);
-    if ((long long)qb * a.rb >= (long long)q.nq * a.g) return 0;
-    return q.ln ? (int)a.by_tile.div((uint32_t)q.ln - 1u) + 1 : 0;
-}
-
 // Worker that holds tile x of T.
 __device__ __forceinline__ int attn_worker(long long x, long long T, int W) {
     return (int)(((x + 1) * W - 1) / T);
 }
 
-// fn(s, q, lo, hi, slot) for every piece of worker w's stretch: tiles lo..hi-1
-// of sequence s; slot -1 where that is all of them. Every warp of a CTA takes
-// the same steps. note: write which workers share a sequence, for the join.
+// fn(qb, q, lo, hi, slot) for every piece of worker w's stretch: tiles lo..hi-1
+// of a sequence in row block qb; slot -1 where that is all of them. Row blocks
+// qb0 .. qb1-1 are laid end to end, each with its sequences. Every warp of a
+// CTA takes the same steps. note: write which workers share a sequence, for the
+// join.
 template <typename F>
-__device__ __forceinline__ void attn_walk(const kvc_attn_args & a, int qb, int w, bool note, F && fn) {
+__device__ __forceinline__ void attn_walk(const kvc_attn_args & a, int qb0, int qb1, int w, bool note, F && fn) {
     const int lane = threadIdx.x & 31;
-    auto tiles = [&](const kvc_attn_seq & q) {
+    auto tiles = [&](const kvc_attn_seq & q, int qb) {
         if ((long long)qb * a.rb >= (long long)q.nq * a.g || !q.ln) return 0;
         return (int)a.by_tile.div((uint32_t)q.ln - 1u) + 1;
     };
-    kvc_attn_seq mine{};
-    if (lane < a.n_seqs) mine = attn_seq(a, lane);
-    const int mine0 = tiles(mine);
-    long long T = mine0;
-    for (int s = lane + 32; s < a.n_seqs; s += 32) T += attn_tiles(a, s, qb);
+    kvc_attn_seq first{};                                // the first 32 sequences stay in registers
+    if (lane < a.n_seqs) first = attn_seq(a, lane);
+    long long T = 0;
+    for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
+        kvc_attn_seq q = first;
+        if (s0) {
+            q = kvc_attn_seq{};
+            if (s0 + lane < a.n_seqs) q = attn_seq(a, s0 + lane);
+        }
+        const long long rows = (long long)q.nq * a.g;
+        const long long blocks = rows <= 0 || !q.ln ? 0 : min((rows - 1) / a.rb + 1, (long long)qb1) - qb0;
+        if (blocks > 0) T += blocks * ((int)a.by_tile.div((uint32_t)q.ln - 1u) + 1);
+    }
 #pragma unroll
     for (int o = 16; o; o >>= 1) T += __shfl_xor_sync(~0u, T, o);
     const int W = (int)min((long long)a.W, T);           // every worker has a tile
     if (w >= W) return;
     const long long from = w * T / W, to = (w + 1) * T / W;
     long long at = 0;
-    for (int s0 = 0; s0 < a.n_seqs && at < to; s0 += 32) {
-        int t = mine0;
-        if (s0) {
-            mine = kvc_attn_seq{};
-            if (s0 + lane < a.n_seqs) mine = attn_seq(a, s0 + lane);
-            t = tiles(mine);
-        }
-        long long p = t;
+    for (int qb = qb0; qb < qb1 && at < to; qb++)
+        for (int s0 = 0; s0 < a.n_seqs && at < to; s0 += 32) {
+            kvc_attn_seq mine = first;
+            if (s0) {
+                mine = kvc_attn_seq{};
+                if (s0 + lane < a.n_seqs) mine = attn_seq(a, s0 + lane);
+            }
+            const int t = tiles(mine, qb);
+            long long p = t;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long u = __shfl_up_sync(~0u, p, o);
-            if (lane >= o) p += u;
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long u = __shfl_up_sync(~0u, p, o);
+                if (lane >= o) p += u;
+            }
+            const long long end = __shfl_sync(~0u, p, 31);
+            p += at - t;
+            const bool in = t > 0 && p < to && p + t > from;
+            unsigned hit = __ballot_sync(~0u, in);
+            if (note && in && p >= from && a.W > 1) {
+                int * m = a.meta + ((size_t)qb * a.n_seqs + s0 + lane) * 2;
+                m[0] = w;
+                m[1] = attn_worker(p + t - 1, T, W);
+            }
+            while (hit) {
+                const int l = __ffs(hit) - 1;
+                hit &= hit - 1;
+                const long long ps = __shfl_sync(~0u, p, l);
+                const int ts = __shfl_sync(~0u, t, l);
+                const int lo = (int)(max(from, ps) - ps), hi = (int)(min(to, ps + ts) - ps);
+                kvc_attn_seq q;
+                q.q0 = __shfl_sync(~0u, mine.q0, l);
+                q.nq = __shfl_sync(~0u, mine.nq, l);
+                q.ln = __shfl_sync(~0u, mine.ln, l);
+                q.k0 = __shfl_sync(~0u, mine.k0, l);
+                q.table = reinterpret_cast<const int *>(__shfl_sync(~0u, (unsigned long long)mine.table, l));
+                fn(qb, q, lo, hi, lo == 0 && hi == ts ? -1 : (from > ps ? 0 : 1));
+            }
+            at += end;
         }
-        const long long end = __shfl_sync(~0u, p, 31);
-        p += at - t;
-        const bool in = t > 0 && p < to && p + t > from;
-        unsigned hit = __ballot_sync(~0u, in);
-        if (note && in && p >= from && a.W > 1) {
-            int * m = a.meta + ((size_t)qb * a.n_seqs + s0 + lane) * 2;
-            m[0] = w;
-            m[1] = attn_worker(p + t - 1, T, W);
-        }
-        while (hit) {
-            const int l = __ffs(hit) - 1;
-            hit &= hit - 1;
-            const long long ps = __shfl_sync(~0u, p, l);
-            const int ts = __shfl_sync(~0u, t, l);
-            const int lo = (int)(max(from, ps) - ps), hi = (int)(min(to, ps + ts) - ps);
-            kvc_attn_seq q;
-            q.q0 = __shfl_sync(~0u, mine.q0, l);
-            q.nq = __shfl_sync(~0u, mine.nq, l);
-            q.ln = __shfl_sync(~0u, mine.ln, l);
-            q.k0 = __shfl_sync(~0u, mine.k0, l);
-            q.table = reinterpret_cast<const int *>(__shfl_sync(~0u, (unsigned long long)mine.table, l));
-            fn(s0 + l, q, lo, hi, lo == 0 && hi == ts ? -1 : (from > ps ? 0 : 1));
-        }
-        at += end;
-    }
 }
 
 // Partial results of worker w, slot s: rb sums of d_v, then rb maxima, rb sums.

@@ -37,7 +37,7 @@ __global__ void __launch_bounds__(THREADS) k_attn_simt(const __grid_constant__ k
     const int n_blocks = (int)(((long long)a.max_q * a.g + RB - 1) / RB);
 
     for (int qb = blockIdx.y / a.Hkv; qb < n_blocks; qb += gridDim.y / a.Hkv) {
-    attn_walk(a, qb, w, h == 0 && threadIdx.x < 32, [&](int, const kvc_attn_seq & q, int lo, int hi, int slot) {
+    attn_walk(a, qb, qb + 1, w, h == 0 && threadIdx.x < 32, [&](int, const kvc_attn_seq & q, int lo, int hi, int slot) {
         const int r0 = qb * RB;
         const int nr = (int)min((long long)RB, (long long)q.nq * a.g - r0);
         __syncthreads();

@@ -41,7 +41,7 @@ constexpr int MAX_SEGS = 64;
 constexpr uint32_t POLLS = 1u << 22;            // bound of every wait
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int P_SHIFT = 10;
-constexpr int HIDDEN = -1000;                   // exponent of a row that counts for nothing
+constexpr int HIDDEN = -200 * (1 << 23);        // exponent bits of a row that counts for nothing
 // registers per thread of the warp groups; their sum x 128 is what the block is launched with
 constexpr int REG_SOFTMAX = 192, REG_PRODUCE = 88, REG_MMA = 40, REG_LAUNCH = 128;
 static_assert(2 * REG_SOFTMAX + REG_PRODUCE + REG_MMA <= 4 * REG_LAUNCH, "more registers than the block has");
@@ -63,14 +63,14 @@ struct cfg {
 };
 
 struct segment {
-    int lo, hi, slot, q0, nq, ln, table;
+    int lo, hi, slot, qb, q0, nq, ln, table;
 };
 
 // Per key of a tile. Eight tiles deep: when tile i is filled, tile i - 5 and those before it have been read.
 struct tile_info {
     float f[TN];                // factor of S: scale 2^e
     float b[TN];                // beta, or -inf
-    int e[TN];                  // exponent of the V row, or HIDDEN
+    int e[TN];                  // exponent of the V row << 23, or HIDDEN
 };
 
 struct shared {
@@ -186,7 +186,7 @@ __device__ __forceinline__ void block_values(const raw_block & r, bool odd, int 
 }
 
 template <int D, int QP, int KP>
-__global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ kvc_attn_args a) {
+__global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ kvc_attn_args a, int n_blocks) {
     using C = cfg<D, QP, KP>;
     extern __shared__ uint8_t sm_raw[];
     uint8_t * sm = reinterpret_cast<uint8_t *>(((uintptr_t)sm_raw + 1023) & ~(uintptr_t)1023);
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
     uint8_t * ring = sq + C::Q;                          // slots: [piece][half][64 rows][128 bytes]
     shared & X = *reinterpret_cast<shared *>(ring + C::REGION);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int h = blockIdx.y % a.Hkv, qb = blockIdx.y / a.Hkv, w = blockIdx.x;
+    const int h = blockIdx.y, w = blockIdx.x;
     if (warp == 12) tmem_alloc(&X.tmem, C::COLS);
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::SLOTS; i++) {
@@ -228,9 +228,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
             __syncthreads();
             if (decltype(walks)::value && warp == 0) {
                 int n = 0;
-                attn_walk(a, qb, w, h == 0, [&](int, const kvc_attn_seq & q, int lo, int hi, int slot) {
+                attn_walk(a, 0, n_blocks, w, h == 0, [&](int qb, const kvc_attn_seq & q, int lo, int hi, int slot) {
                     if (n >= batch && n < batch + MAX_SEGS && lane == 0)
-                        X.segs[n - batch] = segment{lo, hi, slot, q.q0, q.nq, q.ln, (int)((q.table - a.table) / a.max_pages)};
+                        X.segs[n - batch] = segment{lo, hi, slot, qb, q.q0, q.nq, q.ln, (int)((q.table - a.table) / a.max_pages)};
                     n++;
                 });
                 if (lane == 0) {
@@ -261,8 +261,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
         const uint32_t s_addr = tmem + lanes + C::S_COL + t * TN, o_addr = tmem + lanes + C::O_COL + t * D;
         const uint32_t p_addr = tmem + lanes + C::P_COL + t * 64;
         each(kvc_int<1>{}, [&](const segment & S, int n) {
-            const int rows_here = (int)min((long long)TM, (long long)S.nq * a.g - (long long)qb * TM);
-            const int r0 = qb * TM;
+            const int qb = S.qb, r0 = qb * TM;
+            const int rows_here = (int)min((long long)TM, (long long)S.nq * a.g - r0);
             {
                 // Q: two threads per row
                 const int row = threadIdx.x >> 1, part = threadIdx.x & 1;
@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
             };
             for (int j = 0; j < steps; j++) {
                 const int i = 2 * j + t;                 // tile of the segment
-                await(X.s_full + t, (turns[t] + j) & 1); // S of this tile, and the product before it, are complete
+                await(X.s_full + t, (turns[t] + j) & 1);
                 if (!__all_sync(~0u, ok)) break;
                 fence_after_sync();
                 const tile_info & I = X.info[i & 7];
@@ -354,117 +354,150 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                         if (!sees) vis &= ~(1ull << k);
                     }
                 }
-                auto score = [&](float s, int k) {
-                    const float x = fmaf(QP == 2 ? s * mul : s, I.f[k], I.b[k]);
-                    return I.b[k] == -INFINITY || (own && !((vis >> k) & 1)) ? -INFINITY : x;
-                };
-                float top = -INFINITY;
+                // x of columns c .. c+15; `show`: the keys that count
+                auto scores = [&](auto masked, int c, unsigned long long show, float x[16]) {
+                    uint32_t v[16];
+                    tmem_ld16_nowait(s_addr + c, v);
+                    float4 f[4], b[4];
 #pragma unroll
-                for (int c = 0; c < TN; c += 16) {
-                    uint32_t x[16];
-                    tmem_ld16_nowait(s_addr + c, x);
+                    for (int k = 0; k < 4; k++) {
+                        f[k] = *reinterpret_cast<const float4 *>(&I.f[c + 4 * k]);
+                        b[k] = *reinterpret_cast<const float4 *>(&I.b[c + 4 * k]);
+                    }
                     tmem_wait_ld();
 #pragma unroll
-                    for (int k = 0; k < 16; k++) top = fmaxf(top, score(__uint_as_float(x[k]), c + k));
-                }
+                    for (int k = 0; k < 16; k++) {
+                        const float s = __uint_as_float(v[k]);
+                        const float fk = k % 4 == 0 ? f[k / 4].x : k % 4 == 1 ? f[k / 4].y : k % 4 == 2 ? f[k / 4].z : f[k / 4].w;
+                        const float bk = k % 4 == 0 ? b[k / 4].x : k % 4 == 1 ? b[k / 4].y : k % 4 == 2 ? b[k / 4].z : b[k / 4].w;
+                        x[k] = fmaf(QP == 2 ? s * mul : s, fk, bk);        // hidden rows: S = 0 and beta = -inf
+                        if (decltype(masked)::value && !((show >> (c + k)) & 1)) x[k] = -INFINITY;
+                    }
+                };
+                float top = -INFINITY;
+                auto maximum = [&](auto masked) {
+#pragma unroll
+                    for (int c = 0; c < TN; c += 16) {
+                        float x[16];
+                        scores(masked, c, vis, x);
+#pragma unroll
+                        for (int k = 0; k < 16; k += 4)
+                            top = fmaxf(fmaxf(top, fmaxf(x[k], x[k + 1])), fmaxf(x[k + 2], x[k + 3]));
+                    }
+                };
+                if (own) maximum(kvc_int<1>{});
+                else maximum(kvc_int<0>{});
                 const float mn = fmaxf(m, top), base = mn == -INFINITY ? 0.0f : mn;
                 const float f = ex2((m - base) * LOG2E);
                 m = mn;
                 l *= f;
-                if (j > 0) collect(f);
+                if (j > 0) {
+                    await(X.o_full + t, (turns[t] + j - 1) & 1);       // the product of the tile before
+                    if (!__all_sync(~0u, ok)) break;
+                    fence_after_sync();
+                    collect(f);
+                }
                 // the tile's largest V exponent; rows that the mask hides from some of the queries and whose values are
                 // no finite numbers, or far above the others', are added value by value
                 int R = HIDDEN;
-                if (!own) {
-#pragma unroll
-                    for (int k = 0; k < 2; k++) R = max(R, I.e[2 * lane + k]);
-                    R = __reduce_max_sync(~0u, R);
-                } else {
-                    const int it = items + 2 * i + 1;
-                    await(X.full + it % C::SLOTS, (it / C::SLOTS) & 1);
-                    uint8_t * vt = ring + (it % C::SLOTS) * C::SLOT;
-                    if (r == 0) X.bad[t] = 0;
-                    int least = INT_MAX;
-#pragma unroll
-                    for (int k = 0; k < 2; k++)
-                        if (I.e[2 * lane + k] > HIDDEN) least = min(least, I.e[2 * lane + k]);
-                    least = __reduce_min_sync(~0u, least);
-                    group_sync(1 + t, 128);
-                    if (r < TN && I.e[r] > HIDDEN) {
-                        bool bad = I.e[r] - least > 8;
-                        for (int c = 0; c < D / 8; c++) {
-                            const uint4 v = *reinterpret_cast<const uint4 *>(vt + (c >> 3) * C::KBLOCK + swizzled(r, c & 7));
-                            for (uint32_t y : {v.x, v.y, v.z, v.w})
-                                bad |= (y & 0x7C00u) == 0x7C00u || (y & 0x7C000000u) == 0x7C000000u;
+                float sum = 0.0f;
+                if (KP == 2 || own) {
+                    const int2 e2 = *reinterpret_cast<const int2 *>(&I.e[2 * lane]);
+                    R = __reduce_max_sync(~0u, max(e2.x, e2.y));
+                    if (own) {
+                        const int it = items + 2 * i + 1;
+                        await(X.full + it % C::SLOTS, (it / C::SLOTS) & 1);
+                        uint8_t * vt = ring + (it % C::SLOTS) * C::SLOT;
+                        if (r == 0) X.bad[t] = 0;
+                        const int least = __reduce_min_sync(~0u, min(e2.x > HIDDEN ? e2.x : INT_MAX, e2.y > HIDDEN ? e2.y : INT_MAX));
+                        group_sync(1 + t, 128);
+                        if (r < TN && I.e[r] > HIDDEN) {
+                            bool bad = (I.e[r] >> 23) - (least >> 23) > 8;
+                            for (int c = 0; c < D / 8; c++) {
+                                const uint4 v = *reinterpret_cast<const uint4 *>(vt + (c >> 3) * C::KBLOCK + swizzled(r, c & 7));
+                                for (uint32_t y : {v.x, v.y, v.z, v.w})
+                                    bad |= (y & 0x7C00u) == 0x7C00u || (y & 0x7C000000u) == 0x7C000000u;
+                            }
+                            if (bad) atomicOr(&X.bad[t], 1ull << r);
                         }
-                        if (bad) atomicOr(&X.bad[t], 1ull << r);
+                        group_sync(1 + t, 128);
+                        const unsigned long long bad = X.bad[t];
+                        if (bad) {
+                            R = max((bad >> (2 * lane)) & 1 ? HIDDEN : e2.x, (bad >> (2 * lane + 1)) & 1 ? HIDDEN : e2.y);
+                            R = __reduce_max_sync(~0u, R);
+                            for (unsigned long long left = bad; left;) {
+                                const int k = __ffsll((long long)left) - 1;
+                                left &= left - 1;
+                                const float s = ld1(s_addr + k);
+                                const float x = (vis >> k) & 1 ? fmaf(QP == 2 ? s * mul : s, I.f[k], I.b[k]) : -INFINITY;
+                                const float p = ex2((x - base) * LOG2E), g = scalbnf(1.0f, I.e[k] >> 23);
+                                sum += p;
+#pragma unroll
+                                for (int d = 0; d < D / 2; d++) {
+                                    const uint32_t o = (d >> 5) * C::KBLOCK + swizzled(k, (d >> 2) & 7) + (d & 3) * 4;
+                                    uint32_t hv = *reinterpret_cast<const uint32_t *>(vt + o), lv = 0;
+                                    if (KP == 2) lv = *reinterpret_cast<const uint32_t *>(vt + C::PIECE + o);
+                                    const bool fin0 = (hv & 0x7C00u) != 0x7C00u, fin1 = (hv & 0x7C000000u) != 0x7C000000u;
+                                    const float v0 = half_of(hv) + (fin0 ? half_of(lv) : 0.0f);
+                                    const float v1 = half_of(hv >> 16) + (fin1 ? half_of(lv >> 16) : 0.0f);
+                                    if (p != 0.0f) {
+                                        O[d].x = fmaf(p, v0 * g, O[d].x);
+                                        O[d].y = fmaf(p, v1 * g, O[d].y);
+                                    }
+                                }
+                            }
+                            group_sync(1 + t, 128);
+                            if (r < TN && ((bad >> r) & 1))      // 0 * V is to be 0
+                                for (int pc = 0; pc < KP; pc++)
+                                    for (int c = 0; c < D / 8; c++)
+                                        *reinterpret_cast<uint4 *>(vt + pc * C::PIECE + (c >> 3) * C::KBLOCK + swizzled(r, c & 7)) =
+                                            make_uint4(0, 0, 0, 0);
+                            fence_smem_to_async();
+                            vis &= ~bad;
+                        }
                     }
-                    group_sync(1 + t, 128);
-                    const unsigned long long bad = X.bad[t];
+                    if (R == HIDDEN) R = 0;
+                } else {
+                    R = 0;
+                }
+                back = scalbnf(1.0f, (R >> 23) - P_SHIFT);
+                const int up_bits = (127 + P_SHIFT) * (1 << 23) - R;     // + exponent bits: 2^(10 + e - R)
+                auto probabilities = [&](auto masked) {
 #pragma unroll
-                    for (int k = 0; k < 2; k++)
-                        if (!((bad >> (2 * lane + k)) & 1)) R = max(R, I.e[2 * lane + k]);
-                    R = __reduce_max_sync(~0u, R);
-                    for (unsigned long long left = bad; left;) {
-                        const int k = __ffsll((long long)left) - 1;
-                        left &= left - 1;
-                        const float x = score(ld1(s_addr + k), k);
-                        const float p = ex2((x - base) * LOG2E), g = scalbnf(1.0f, I.e[k]);
+                    for (int c = 0; c < TN; c += 16) {
+                        float x[16];
+                        scores(masked, c, vis, x);
+                        int4 e[4];
+                        if (KP == 2) {
 #pragma unroll
-                        for (int d = 0; d < D / 2; d++) {
-                            const uint32_t o = (d >> 5) * C::KBLOCK + swizzled(k, (d >> 2) & 7) + (d & 3) * 4;
-                            uint32_t hv = *reinterpret_cast<const uint32_t *>(vt + o), lv = 0;
-                            if (KP == 2) lv = *reinterpret_cast<const uint32_t *>(vt + C::PIECE + o);
-                            const bool fin0 = (hv & 0x7C00u) != 0x7C00u, fin1 = (hv & 0x7C000000u) != 0x7C000000u;
-                            const float v0 = half_of(hv) + (fin0 ? half_of(lv) : 0.0f);
-                            const float v1 = half_of(hv >> 16) + (fin1 ? half_of(lv >> 16) : 0.0f);
-                            if (p != 0.0f) {
-                                O[d].x = fmaf(p, v0 * g, O[d].x);
-                                O[d].y = fmaf(p, v1 * g, O[d].y);
+                            for (int k = 0; k < 4; k++) e[k] = *reinterpret_cast<const int4 *>(&I.e[c + 4 * k]);
+                        }
+                        uint32_t p0[8], p1[8];
+#pragma unroll
+                        for (int k = 0; k < 8; k++) {
+                            float p[2];
+#pragma unroll
+                            for (int u = 0; u < 2; u++) {
+                                const int q = 2 * k + u;
+                                p[u] = ex2((x[q] - base) * LOG2E);
+                                sum += p[u];
+                                const int ek = q % 4 == 0 ? e[q / 4].x : q % 4 == 1 ? e[q / 4].y : q % 4 == 2 ? e[q / 4].z : e[q / 4].w;
+                                p[u] *= KP == 2 ? __int_as_float(max(ek + up_bits, 0)) : (float)(1 << P_SHIFT);
+                            }
+                            p0[k] = pack(p[0], p[1]);
+                            if (QP == 2) {
+                                __half2 hh;
+                                memcpy(&hh, &p0[k], 4);
+                                const float2 y = __half22float2(hh);
+                                p1[k] = pack(p[0] - y.x, p[1] - y.y);
                             }
                         }
+                        st8(p_addr + c / 2, p0);
+                        if (QP == 2) st8(p_addr + 32 + c / 2, p1);
                     }
-                    group_sync(1 + t, 128);
-                    if (r < TN && ((bad >> r) & 1))      // 0 * V is to be 0
-                        for (int pc = 0; pc < KP; pc++)
-                            for (int c = 0; c < D / 8; c++)
-                                *reinterpret_cast<uint4 *>(vt + pc * C::PIECE + (c >> 3) * C::KBLOCK + swizzled(r, c & 7)) =
-                                    make_uint4(0, 0, 0, 0);
-                    fence_smem_to_async();
-                }
-                if (R == HIDDEN) R = 0;
-                back = scalbnf(1.0f, R - P_SHIFT);
-                float sum = 0.0f;
-#pragma unroll
-                for (int c = 0; c < TN; c += 16) {
-                    uint32_t x[16];
-                    tmem_ld16_nowait(s_addr + c, x);
-                    tmem_wait_ld();
-                    uint32_t p0[8], p1[8];
-#pragma unroll
-                    for (int k = 0; k < 8; k++) {
-                        float p[2];
-#pragma unroll
-                        for (int u = 0; u < 2; u++) {
-                            const int col = c + 2 * k + u;
-                            p[u] = ex2((score(__uint_as_float(x[2 * k + u]), col) - base) * LOG2E);
-                            sum += p[u];
-                            // 2^(10 + e - R), 0 for rows that count for nothing or were taken by value
-                            const int e = KP == 2 ? I.e[col] - R : 0;
-                            p[u] *= KP == 2 ? (e < -100 || e > 0 ? 0.0f : __int_as_float((127 + P_SHIFT + e) << 23))
-                                            : (float)(1 << P_SHIFT);
-                        }
-                        p0[k] = pack(p[0], p[1]);
-                        if (QP == 2) {
-                            __half2 hh;
-                            memcpy(&hh, &p0[k], 4);
-                            const float2 y = __half22float2(hh);
-                            p1[k] = pack(p[0] - y.x, p[1] - y.y);
-                        }
-                    }
-                    st8(p_addr + c / 2, p0);
-                    if (QP == 2) st8(p_addr + 32 + c / 2, p1);
-                }
+                };
+                if (own) probabilities(kvc_int<1>{});
+                else probabilities(kvc_int<0>{});
                 l += sum;
                 tmem_wait_st();
                 fence_before_sync();
@@ -489,34 +522,43 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                 X.jl[r] = l;
             }
             group_sync(3, 256);
-            if (t == 0 && real) {
+            if (t == 0) {
                 const float om = X.jm[r], mn = fmaxf(m, om), base = mn == -INFINITY ? 0.0f : mn;
                 const float f0 = ex2((m - base) * LOG2E), f1 = ex2((om - base) * LOG2E);
                 l = l * f0 + X.jl[r] * f1;
-                const int head = h * a.g + (r0 + r - node * a.g);
-                const size_t out = (size_t)(S.q0 + node) * a.Hq + head;
-                float * part = S.slot >= 0 ? attn_part(a, qb, h, w, S.slot) : nullptr;
-                const float inv = part ? 1.0f : l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-                if (part) {
-                    part[a.rb * a.dv + r] = mn;
-                    part[a.rb * a.dv + a.rb + r] = l;
-                } else if (a.lse) {
-                    a.lse[out] = l == 0.0f ? -INFINITY : mn + logf(l);
-                }
+                const float inv = S.slot >= 0 ? 1.0f : l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+                X.jm[r] = mn;
+                X.jl[r] = l;
 #pragma unroll
                 for (int k = 0; k < D / 4; k++) {
-                    if (4 * k < a.dv) {
-                        const float4 o = *reinterpret_cast<const float4 *>(jo + 4 * k);
-                        const float v[4] = {(O[2 * k].x * f0 + o.x * f1) * inv, (O[2 * k].y * f0 + o.y * f1) * inv,
-                                            (O[2 * k + 1].x * f0 + o.z * f1) * inv, (O[2 * k + 1].y * f0 + o.w * f1) * inv};
-                        if (part)
-                            *reinterpret_cast<float4 *>(part + r * a.dv + 4 * k) = make_float4(v[0], v[1], v[2], v[3]);
-                        else if (QP == 2)
-                            for (int u = 0; u < 4; u++) reinterpret_cast<float *>(a.out)[out * a.dv + 4 * k + u] = v[u];
-                        else
-                            for (int u = 0; u < 4; u++)
-                                reinterpret_cast<__half *>(a.out)[out * a.dv + 4 * k + u] = __float2half_rn(v[u]);
+                    float4 o = *reinterpret_cast<const float4 *>(jo + 4 * k);
+                    o.x = (O[2 * k].x * f0 + o.x * f1) * inv;
+                    o.y = (O[2 * k].y * f0 + o.y * f1) * inv;
+                    o.z = (O[2 * k + 1].x * f0 + o.z * f1) * inv;
+                    o.w = (O[2 * k + 1].y * f0 + o.w * f1) * inv;
+                    *reinterpret_cast<float4 *>(jo + 4 * k) = o;
+                }
+            }
+            group_sync(3, 256);
+            // rows by warp, so that they are written side by side
+            for (int rr = warp; rr < rows_here; rr += 8) {
+                const int nd = (int)a.by_group.div(r0 + rr);
+                const size_t out = (size_t)(S.q0 + nd) * a.Hq + h * a.g + (r0 + rr - nd * a.g);
+                const float * from = reinterpret_cast<const float *>(ring) + rr * (D + 4);
+                float * part = S.slot >= 0 ? attn_part(a, qb, h, w, S.slot) : nullptr;
+                if (lane == 0) {
+                    const float mm = X.jm[rr], ll = X.jl[rr];
+                    if (part) {
+                        part[a.rb * a.dv + rr] = mm;
+                        part[a.rb * a.dv + a.rb + rr] = ll;
+                    } else if (a.lse) {
+                        a.lse[out] = ll == 0.0f ? -INFINITY : mm + logf(ll);
                     }
+                }
+                for (int d = lane; d < a.dv; d += 32) {
+                    if (part) part[rr * a.dv + d] = from[d];
+                    else if (QP == 2) reinterpret_cast<float *>(a.out)[out * a.dv + d] = from[d];
+                    else reinterpret_cast<__half *>(a.out)[out * a.dv + d] = __float2half_rn(from[d]);
                 }
             }
         });
@@ -683,7 +725,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                                     tv = max(tv, max(d < 0x7C00u ? d : 0u, m < 0x7C00u ? m : 0u));
                                 }
                             tv = max(tv, __shfl_xor_sync(~0u, tv, 1));
-                            if (part == 0) X.info[i & 7].e[key] = live ? max((int)(tv >> 10), 1) - 15 : HIDDEN;
+                            if (part == 0) X.info[i & 7].e[key] = live ? (max((int)(tv >> 10), 1) - 15) * (1 << 23) : HIDDEN;
                         }
                         fence_smem_to_async();
                         mbar_arrive(X.full + it % C::SLOTS);
@@ -751,8 +793,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                     await(X.p_full + (i & 1), (turns[i & 1] + (i >> 1)) & 1);
                     if (!ok) break;
                     fence_after_sync();
+                    if (i + 2 < n) qk(i + 2);            // first: the stream's next softmax can begin
                     pv(i);
-                    if (i + 2 < n) qk(i + 2);
                 }
             }
             __syncwarp();
@@ -788,7 +830,7 @@ int run(const kvc_attn_args & a, int ngr, cudaStream_t st) {
         fprintf(stderr, "[kvc] k_tree_tc was built with too few registers per thread\n");
         return KVC_ERR_CUDA;
     }
-    k<<<dim3((unsigned)a.W, (unsigned)(a.Hkv * ngr)), THREADS, smem_bytes<D, QP, KP>(), st>>>(a);
+    k<<<dim3((unsigned)a.W, (unsigned)a.Hkv), THREADS, smem_bytes<D, QP, KP>(), st>>>(a, ngr);
     g_serve_launches++;
     KVC_CUDA(cudaGetLastError());
     return kvc_launch_attn_join(a, true, st);
@@ -812,11 +854,11 @@ bool kvc_attn_tree_tc_plan(kvc_attn_args * a, int sms, long long * blocks) {
         return false;
     }
     const long long n = (rows + TM - 1) / TM;
-    if (n * a->Hkv > 65535) return false;
+    if (n > 65535 || a->Hkv > 65535) return false;
     a->rb = TM;
     a->tile = TN;
     a->by_tile = kvc_make_divisor(TN);
-    const long long w = sms / (n * a->Hkv);
+    const long long w = sms / a->Hkv;                    // one CTA per SM; the row blocks are laid end to end
     a->W = (int)(w < 1 ? 1 : w);
     *blocks = n;
     return true;
