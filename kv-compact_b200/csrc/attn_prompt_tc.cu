@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_prompt_tc(const __grid_constant_
                                                           const __grid_constant__ CUtensorMap v_map) {
     using C = cfg<D>;
     extern __shared__ uint8_t sm_raw[];
-    uint8_t * sm = reinterpret_cast<uint8_t *>(((uintptr_t)sm_raw + 1023) & ~(uintptr_t)1023);
+    uint8_t * sm = aligned_1024(sm_raw);
     uint8_t * sq = sm;                                   // two Q tiles
     uint8_t * ring = sq + 2 * C::TILE;
     uint64_t * bars = reinterpret_cast<uint64_t *>(ring + C::SLOTS * C::TILE);

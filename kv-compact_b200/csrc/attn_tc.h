@@ -8,6 +8,8 @@
 
 namespace kvc_attn_tc {
 
+using kvc_tc::smem_u32;
+
 // Shared-memory descriptors of tiles whose rows are 128 bytes, 128-byte swizzled
 // as TMA writes them (start addresses below are multiples of 16 bytes).
 // K-major operand (rows = M or N, 64 values of K a row): groups of 8 rows 1,024 bytes apart.
@@ -64,6 +66,14 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     memcpy(&r, &d, 8);
     return r;
 }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    unsigned long long x, y, d;
+    memcpy(&x, &a, 8), memcpy(&y, &b, 8);
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(x), "l"(y));
+    float2 r;
+    memcpy(&r, &d, 8);
+    return r;
+}
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     unsigned long long x, y, d;
     memcpy(&x, &a, 8), memcpy(&y, &b, 8);
@@ -72,6 +82,9 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     memcpy(&r, &d, 8);
     return r;
 }
+
+// Dynamic shared memory from its next 1,024-byte boundary (the swizzle's period); stays a shared-memory pointer.
+__device__ __forceinline__ uint8_t * aligned_1024(uint8_t * p) { return p + ((1024u - (smem_u32(p) & 1023u)) & 1023u); }
 
 #undef KVC_R8
 #undef KVC_I8

@@ -189,7 +189,7 @@ template <int D, int QP, int KP>
 __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ kvc_attn_args a, int n_blocks) {
     using C = cfg<D, QP, KP>;
     extern __shared__ uint8_t sm_raw[];
-    uint8_t * sm = reinterpret_cast<uint8_t *>(((uintptr_t)sm_raw + 1023) & ~(uintptr_t)1023);
+    uint8_t * sm = aligned_1024(sm_raw);
     uint8_t * sq = sm;                                   // [piece][half][128 rows][128 bytes]
     uint8_t * ring = sq + C::Q;                          // slots: [piece][half][64 rows][128 bytes]
     shared & X = *reinterpret_cast<shared *>(ring + C::REGION);
@@ -322,6 +322,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
             for (int k = 0; k < D / 2; k++) O[k] = make_float2(0.0f, 0.0f);
             // O = (O + product of the tile before) * f
             auto collect = [&](float f) {
+                const float2 b2 = make_float2(back, back), f2 = make_float2(f, f);
+                const bool moved = __any_sync(~0u, f != 1.0f);
 #pragma unroll
                 for (int c = 0; c < D; c += 16) {
                     uint32_t o[16];
@@ -330,10 +332,12 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
 #pragma unroll
                     for (int k = 0; k < 8; k++) {
                         float2 & x = O[c / 2 + k];
-                        x = fma2(make_float2(__uint_as_float(o[2 * k]), __uint_as_float(o[2 * k + 1])), make_float2(back, back), x);
-                        x.x *= f;
-                        x.y *= f;
+                        x = fma2(make_float2(__uint_as_float(o[2 * k]), __uint_as_float(o[2 * k + 1])), b2, x);
                     }
+                }
+                if (moved) {
+#pragma unroll
+                    for (int k = 0; k < D / 2; k++) O[k] = mul2(O[k], f2);
                 }
             };
             for (int j = 0; j < steps; j++) {
@@ -376,7 +380,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                 };
                 float top = -INFINITY;
                 auto maximum = [&](auto masked) {
-#pragma unroll
+#pragma unroll 1
                     for (int c = 0; c < TN; c += 16) {
                         float x[16];
                         scores(masked, c, vis, x);
@@ -463,7 +467,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                 back = scalbnf(1.0f, (R >> 23) - P_SHIFT);
                 const int up_bits = (127 + P_SHIFT) * (1 << 23) - R;     // + exponent bits: 2^(10 + e - R)
                 auto probabilities = [&](auto masked) {
-#pragma unroll
+#pragma unroll 1
                     for (int c = 0; c < TN; c += 16) {
                         float x[16];
                         scores(masked, c, vis, x);
