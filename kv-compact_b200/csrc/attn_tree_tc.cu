@@ -165,21 +165,30 @@ __device__ __forceinline__ void block_values(const raw_block & r, bool odd, int 
             lo[2 * i + 1] = h2fma(c1, d2, hi[2 * i + 1] ^ 0x80008000u);
         }
     } else {
+        // a byte holds values 2i (low) and 2i + 1 (high): 0x6400 | n is 1024 + n, 0x6400 | 16 n is 1024 + 16 n
+        const uint32_t d2 = pack(fd, fd);
         const float fm = half_of(m) * up;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const uint32_t w = code_word(r, odd, type, i);
 #pragma unroll
-            for (int b = 0; b < 4; b++) {                // a byte holds values 2i (low) and 2i + 1 (high)
-                const float n0 = (float)((w >> (8 * b)) & 15u), n1 = (float)((w >> (8 * b + 4)) & 15u);
-                const float v0 = type == KV_TYPE_Q4_0 ? (n0 - 8.0f) * fd : fmaf(n0, fd, fm);
-                const float v1 = type == KV_TYPE_Q4_0 ? (n1 - 8.0f) * fd : fmaf(n1, fd, fm);
-                const uint32_t h = pack(v0, v1);
-                __half2 hh;
-                memcpy(&hh, &h, 4);
-                const float2 f = __half22float2(hh);
-                hi[4 * i + b] = h;
-                lo[4 * i + b] = pack(v0 - f.x, v1 - f.y);
+            for (int b = 0; b < 4; b++) {
+                const uint32_t n = __byte_perm(w, 0x64646464u, 0x4040 | b << 8 | b) & 0x64F0640Fu;
+                if (type == KV_TYPE_Q4_0) {              // (1024 + n0) - 1032, (1024 + 16 n1) / 16 - 72
+                    const uint32_t c = h2fma(n, 0x2C003C00u, 0xD480E408u);
+                    hi[4 * i + b] = h2mul(c, d2);
+                    lo[4 * i + b] = h2fma(c, d2, hi[4 * i + b] ^ 0x80008000u);               // exact
+                } else {
+                    const uint32_t c = h2fma(n, 0x2C003C00u, 0xD400E400u);
+                    __half2 hc, hh;
+                    memcpy(&hc, &c, 4);
+                    const float2 x = __half22float2(hc);
+                    const float v0 = fmaf(x.x, fd, fm), v1 = fmaf(x.y, fd, fm);
+                    hi[4 * i + b] = pack(v0, v1);
+                    memcpy(&hh, &hi[4 * i + b], 4);
+                    const float2 f = __half22float2(hh);
+                    lo[4 * i + b] = pack(v0 - f.x, v1 - f.y);
+                }
             }
         }
     }
@@ -358,35 +367,37 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                         if (!sees) vis &= ~(1ull << k);
                     }
                 }
-                // x of columns c .. c+15; `show`: the keys that count
-                auto scores = [&](auto masked, int c, unsigned long long show, float x[16]) {
-                    uint32_t v[16];
-                    tmem_ld16_nowait(s_addr + c, v);
-                    float4 f[4], b[4];
+                // x of columns c .. c+15 from v; `show`: the keys that count
+                auto scores = [&](auto masked, int c, unsigned long long show, const uint32_t v[16], float x[16]) {
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        f[k] = *reinterpret_cast<const float4 *>(&I.f[c + 4 * k]);
-                        b[k] = *reinterpret_cast<const float4 *>(&I.b[c + 4 * k]);
-                    }
-                    tmem_wait_ld();
+                    for (int k = 0; k < 16; k += 4) {
+                        const float4 f = *reinterpret_cast<const float4 *>(&I.f[c + k]);
+                        const float4 b = *reinterpret_cast<const float4 *>(&I.b[c + k]);
+                        const float fk[4] = {f.x, f.y, f.z, f.w}, bk[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-                    for (int k = 0; k < 16; k++) {
-                        const float s = __uint_as_float(v[k]);
-                        const float fk = k % 4 == 0 ? f[k / 4].x : k % 4 == 1 ? f[k / 4].y : k % 4 == 2 ? f[k / 4].z : f[k / 4].w;
-                        const float bk = k % 4 == 0 ? b[k / 4].x : k % 4 == 1 ? b[k / 4].y : k % 4 == 2 ? b[k / 4].z : b[k / 4].w;
-                        x[k] = fmaf(QP == 2 ? s * mul : s, fk, bk);        // hidden rows: S = 0 and beta = -inf
-                        if (decltype(masked)::value && !((show >> (c + k)) & 1)) x[k] = -INFINITY;
+                        for (int u = 0; u < 4; u++) {
+                            const float s = __uint_as_float(v[k + u]);
+                            x[k + u] = fmaf(QP == 2 ? s * mul : s, fk[u], bk[u]);      // hidden rows: S = 0 and beta = -inf
+                            if (decltype(masked)::value && !((show >> (c + k + u)) & 1)) x[k + u] = -INFINITY;
+                        }
                     }
                 };
                 float top = -INFINITY;
                 auto maximum = [&](auto masked) {
 #pragma unroll 1
-                    for (int c = 0; c < TN; c += 16) {
-                        float x[16];
-                        scores(masked, c, vis, x);
+                    for (int c = 0; c < TN; c += 32) {
+                        uint32_t v[2][16];
+                        tmem_ld16_nowait(s_addr + c, v[0]);
+                        tmem_ld16_nowait(s_addr + c + 16, v[1]);
+                        tmem_wait_ld();
 #pragma unroll
-                        for (int k = 0; k < 16; k += 4)
-                            top = fmaxf(fmaxf(top, fmaxf(x[k], x[k + 1])), fmaxf(x[k + 2], x[k + 3]));
+                        for (int u = 0; u < 2; u++) {
+                            float x[16];
+                            scores(masked, c + 16 * u, vis, v[u], x);
+#pragma unroll
+                            for (int k = 0; k < 16; k += 4)
+                                top = fmaxf(fmaxf(top, fmaxf(x[k], x[k + 1])), fmaxf(x[k + 2], x[k + 3]));
+                        }
                     }
                 };
                 if (own) maximum(kvc_int<1>{});
@@ -467,10 +478,14 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                 back = scalbnf(1.0f, (R >> 23) - P_SHIFT);
                 const int up_bits = (127 + P_SHIFT) * (1 << 23) - R;     // + exponent bits: 2^(10 + e - R)
                 auto probabilities = [&](auto masked) {
+                    uint32_t v[16];
+                    tmem_ld16_nowait(s_addr, v);
 #pragma unroll 1
                     for (int c = 0; c < TN; c += 16) {
                         float x[16];
-                        scores(masked, c, vis, x);
+                        tmem_wait_ld();
+                        scores(masked, c, vis, v, x);
+                        if (c + 16 < TN) tmem_ld16_nowait(s_addr + c + 16, v);     // under the exponentials
                         int4 e[4];
                         if (KP == 2) {
 #pragma unroll
@@ -544,27 +559,37 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                 }
             }
             group_sync(3, 256);
-            // rows by warp, so that they are written side by side
-            for (int rr = warp; rr < rows_here; rr += 8) {
-                const int nd = (int)a.by_group.div(r0 + rr);
-                const size_t out = (size_t)(S.q0 + nd) * a.Hq + h * a.g + (r0 + rr - nd * a.g);
-                const float * from = reinterpret_cast<const float *>(ring) + rr * (D + 4);
-                float * part = S.slot >= 0 ? attn_part(a, qb, h, w, S.slot) : nullptr;
-                if (lane == 0) {
-                    const float mm = X.jm[rr], ll = X.jl[rr];
-                    if (part) {
-                        part[a.rb * a.dv + rr] = mm;
-                        part[a.rb * a.dv + a.rb + rr] = ll;
-                    } else if (a.lse) {
-                        a.lse[out] = ll == 0.0f ? -INFINITY : mm + logf(ll);
-                    }
-                }
-                for (int d = lane; d < a.dv; d += 32) {
-                    if (part) part[rr * a.dv + d] = from[d];
-                    else if (QP == 2) reinterpret_cast<float *>(a.out)[out * a.dv + d] = from[d];
-                    else reinterpret_cast<__half *>(a.out)[out * a.dv + d] = __float2half_rn(from[d]);
+            // written side by side: a partial result is one stretch of rows
+            float * part = S.slot >= 0 ? attn_part(a, qb, h, w, S.slot) : nullptr;
+            if (t == 0 && real) {
+                const size_t out = (size_t)(S.q0 + node) * a.Hq + h * a.g + (r0 + r - node * a.g);
+                if (part) {
+                    part[a.rb * a.dv + r] = X.jm[r];
+                    part[a.rb * a.dv + a.rb + r] = X.jl[r];
+                } else if (a.lse) {
+                    a.lse[out] = X.jl[r] == 0.0f ? -INFINITY : X.jm[r] + logf(X.jl[r]);
                 }
             }
+            // 32 lanes = one row's D / 4 pieces of 16 bytes, twice for D = 64
+            constexpr int PIECES = D / 4;
+            const int piece = threadIdx.x % PIECES;
+            if (4 * piece < a.dv)
+#pragma unroll 4
+                for (int rr = threadIdx.x / PIECES; rr < rows_here; rr += 256 / PIECES) {
+                    const float4 o = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(ring) + rr * (D + 4) + 4 * piece);
+                    if (part) {
+                        *reinterpret_cast<float4 *>(part + rr * a.dv + 4 * piece) = o;
+                    } else {
+                        const int nd = (int)a.by_group.div(r0 + rr);
+                        const size_t at = ((size_t)(S.q0 + nd) * a.Hq + h * a.g + (r0 + rr - nd * a.g)) * a.dv + 4 * piece;
+                        const float v[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+                        for (int u = 0; u < 4; u++) {
+                            if (QP == 2) reinterpret_cast<float *>(a.out)[at + u] = v[u];
+                            else reinterpret_cast<__half *>(a.out)[at + u] = __float2half_rn(v[u]);
+                        }
+                    }
+                }
         });
     } else if (warp < 12) {
         // ---- producers
