@@ -240,7 +240,7 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void * map, int 
 // loop), or a warp's output, maxima and sums (when the warps of a unit are joined).
 constexpr int slot_bytes(int db, int nb) { return db * nb * 1024 + nb * 512; }
 
-template <int DB, int NB, int NP, int MAXW>
+template <int DB, int NB, int NP, int MAXW, bool FULL>
 __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant__ kvc_attn_args a,
                                                            const __grid_constant__ mma_geom G,
                                                            const __grid_constant__ CUtensorMap k_map,
@@ -248,6 +248,7 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
                                                            const __grid_constant__ CUtensorMap b_map) {
     using namespace kvc_tc;
     constexpr int RW = 8 * NB;                           // query rows of a warp
+    const int NBK = FULL ? DB : G.nbk, NBV = FULL ? DB : G.nbv;      // FULL: all blocks are there, no checks in the loops
     constexpr bool QS = NP == 2;                         // query fragments in shared memory
     constexpr int SLOT = slot_bytes(DB, NB);
     extern __shared__ __align__(128) uint8_t sm[];
@@ -283,7 +284,7 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
     float * qsum = qsum_all + warp * DB * RW;
     bool dead = false;                                   // a wait ran out: no more waits, the status says so
     auto await = [&](uint64_t * bar, uint32_t parity) {
-        if (!dead && !mbar_wait(bar, parity, POLLS)) {
+        if (!dead && !mbar_wait_suspend(bar, parity, POLLS, 2000)) {
             dead = true;
             if (a.status) *a.status = KVC_ERR_CUDA;
         }
@@ -456,7 +457,7 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
                     const int d = 32 * b + (kt == KV_TYPE_F16 ? 2 * t + 8 * u
                                             : kt == KV_TYPE_Q8_0 ? 4 * t + 2 * (u & 1) + 16 * (u >> 1) : 8 * t + 2 * u);
                     float2 v = make_float2(0.0f, 0.0f);
-                    if (there && b < G.nbk) {
+                    if (there && b < NBK) {
                         if (a.q_type == KV_TYPE_F16) {
                             const __half * p = reinterpret_cast<const __half *>(a.q) + at + d;
                             v = G.qvec ? __half22float2(*reinterpret_cast<const __half2 *>(p))
@@ -569,7 +570,7 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
                 constexpr int KT_ = decltype(type)::value;
 #pragma unroll
                 for (int b = 0; b < DB; b++) {
-                    if (b < G.nbk) {
+                    if (b < NBK) {
                         uint32_t fa[2][4];
                         const uint8_t * p0 = kr0 + b * block_bytes(KT_);
                         const uint8_t * p1 = kr1 + b * block_bytes(KT_);
@@ -683,7 +684,7 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
                             for (int mt = 0; mt < 2; mt++)
 #pragma unroll
                                 for (int r8 = 0; r8 < 2; r8++) {
-                                    if (b < G.nbv) {
+                                    if (b < NBV) {
                                         const float v = attn_elem(vs + k * G.vp, vt, 32 * b + v_dim(vt, mt, g, r8));
                                         if (p0 != 0.0f) O[b][mt][nb][2 * r8] = fmaf(p0, v, O[b][mt][nb][2 * r8]);
                                         if (p1 != 0.0f) O[b][mt][nb][2 * r8 + 1] = fmaf(p1, v, O[b][mt][nb][2 * r8 + 1]);
@@ -714,7 +715,7 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
 #pragma unroll
                     for (int b = 0; b < DB; b++) {
                         dl[b] = dh[b] = 0;
-                        if (b < G.nbv) {
+                        if (b < NBV) {
                             const uint8_t * p = vk + b * block_bytes(VT);
                             dl[b] = pair16(lds16(p), lds16(p + G.vp)) & live_l;
                             dh[b] = pair16(lds16(p + 8 * G.vp), lds16(p + 9 * G.vp)) & live_h;
@@ -739,7 +740,7 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
                         if (R == -1000) {
 #pragma unroll
                             for (int b = 0; b < DB; b++)
-                                if (b < G.nbv) {
+                                if (b < NBV) {
                                     const uint32_t x[4] = {dl[b] & 0x7FFFu, dl[b] >> 16 & 0x7FFFu, dh[b] & 0x7FFFu, dh[b] >> 16 & 0x7FFFu};
 #pragma unroll
                                     for (int u = 0; u < 4; u++)
@@ -812,7 +813,7 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
                 };
 #pragma unroll
                 for (int b = 0; b < DB; b++) {
-                    if (b < G.nbv) {
+                    if (b < NBV) {
                         uint32_t fa[2][4];
                         const uint8_t * p = vk + b * block_bytes(VT);
                         if (b & 1) v_frag<VT, true, CENTRE>(fa, p, G.vp, v_ld + 64 * b, g);
@@ -854,7 +855,7 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
                     while (rows) {
                         const int k = __ffs(rows) - 1;
                         rows &= rows - 1;
-                        for (int o = lane; o < 4 * G.nbv; o += 32)
+                        for (int o = lane; o < 4 * NBV; o += 32)
                             *reinterpret_cast<int4 *>(const_cast<uint8_t *>(vs) + k * G.vp + 16 * o) = make_int4(0, 0, 0, 0);
                     }
                     fence_smem_to_async();               // the next box goes over them
@@ -863,7 +864,7 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
                 bool bad = false;
                 if (own)
                     for (int k = 0; k < KEYS; k++)
-                        for (int o = lane; o < 4 * G.nbv; o += 32) {
+                        for (int o = lane; o < 4 * NBV; o += 32) {
                             const uint4 v = *reinterpret_cast<const uint4 *>(vs + k * G.vp + 16 * o);
                             for (uint32_t x : {v.x, v.y, v.z, v.w})
                                 bad |= (x & 0x7C00u) == 0x7C00u || (x & 0x7C000000u) == 0x7C000000u;
@@ -979,7 +980,7 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
                     }
 #pragma unroll
                     for (int b = 0; b < DB; b++) {
-                        if (b >= G.nbv) break;
+                        if (b >= NBV) break;
                         const float v[4] = {O[b][0][nb][c] * mul_o, O[b][0][nb][2 + c] * mul_o, O[b][1][nb][c] * mul_o,
                                             O[b][1][nb][2 + c] * mul_o};
                         if (vt == KV_TYPE_F16) {
@@ -1109,12 +1110,12 @@ bool beta_map(CUtensorMap * m, const kvc_attn_args & a, int hc, int run) {
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int DB, int NB, int NP, int MAXW>
+template <int DB, int NB, int NP, int MAXW, bool FULL>
 int run(const kvc_attn_args & a, const mma_geom & G, int ngr, cudaStream_t st) {
     static std::atomic<bool> set[64];
     int dev = 0;
     KVC_CUDA(cudaGetDevice(&dev));
-    auto * k = k_tree_mma<DB, NB, NP, MAXW>;
+    auto * k = k_tree_mma<DB, NB, NP, MAXW, FULL>;
     if (!set[dev & 63].load(std::memory_order_relaxed)) {
         KVC_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MOST));
         set[dev & 63].store(true, std::memory_order_relaxed);
@@ -1137,13 +1138,15 @@ int run(const kvc_attn_args & a, const mma_geom & G, int ngr, cudaStream_t st) {
 
 using run_fn = int (*)(const kvc_attn_args &, const mma_geom &, int, cudaStream_t);
 struct variant {
-    int db, nb, np, warps;
+    int db, nb, np, full, warps;
     fixed_fn fixed;
     run_fn run;
 };
-#define TREE_VARIANT(DB, NB, NP, W) {DB, NB, NP, W, fixed_bytes<DB, NB, NP, W>, run<DB, NB, NP, W>}
+#define TREE_VARIANT(DB, NB, NP, W) \
+    {DB, NB, NP, 0, W, fixed_bytes<DB, NB, NP, W>, run<DB, NB, NP, W, false>}, {DB, NB, NP, 1, W, fixed_bytes<DB, NB, NP, W>, run<DB, NB, NP, W, true>}
 // Up to 8 query rows per KV head (single tokens): 16 warps of 8 rows. More rows: 8 warps of 16 rows, whose
-// registers hold twice the output. d > 128: twice that again, 8 warps of 8 rows.
+// registers hold twice the output. d > 128: twice that again, 8 warps of 8 rows. Each with and without checks of
+// the head's blocks (d_k = d_v = 32 DB: without; the checks cost decode_compacted 15 %).
 const variant variants[] = {
     TREE_VARIANT(2, 1, 1, 16), TREE_VARIANT(2, 1, 2, 16), TREE_VARIANT(4, 1, 1, 16), TREE_VARIANT(4, 1, 2, 16),
     TREE_VARIANT(2, 2, 1, 8),  TREE_VARIANT(2, 2, 2, 8),  TREE_VARIANT(4, 2, 1, 8),  TREE_VARIANT(4, 2, 2, 8),
@@ -1155,8 +1158,9 @@ const variant & select(const kvc_attn_args & a) {
     const int db = top <= 64 ? 2 : top <= 128 ? 4 : 8;
     const int nb = db == 8 || (long long)a.max_q * a.g <= 8 ? 1 : 2;
     const int np = a.q_type == KV_TYPE_F32 ? 2 : 1;
+    const int full = a.dk == 32 * db && a.dv == 32 * db;
     for (const variant & v : variants)
-        if (v.db == db && v.nb == nb && v.np == np) return v;
+        if (v.db == db && v.nb == nb && v.np == np && v.full == full) return v;
     return variants[0];
 }
 

@@ -111,6 +111,22 @@ __device__ __forceinline__ bool mbar_wait(uint64_t * mbar, uint32_t parity, uint
     return false;
 }
 
+// The same, each poll suspended by the hardware for up to `ns` nanoseconds (a
+// hint): a waiting warp leaves the issue slots to those that work.
+__device__ __forceinline__ bool mbar_wait_suspend(uint64_t * mbar, uint32_t parity, uint32_t limit, uint32_t ns) {
+    const uint32_t a = smem_u32(mbar);
+    for (uint32_t i = 0; i < limit; i++) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}\n"
+            : "=r"(done) : "r"(a), "r"(parity), "r"(ns) : "memory");
+        if (done) return true;
+    }
+    return false;
+}
+
 // Instruction descriptor of kind::f16 with f16 operands: fp32 accumulate,
 // A and B both F16 and K-major, M x N tile (A/B format 0 = F16).
 __host__ __device__ constexpr uint32_t idesc_f16(int M, int N) {
