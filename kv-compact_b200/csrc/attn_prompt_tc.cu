@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_prompt_tc(const __grid_constant_
         }
     } else if (warp == 9) {
         // ---- products
-        if (lane == 0 && n > 0) {
+        if (n > 0) {
             const uint32_t id_s = idesc_f16(TM, TN), id_o = idesc_f16(TM, D) | 1u << 16;      // V is N-major
             const bool fixed = nk - (n - 1) * TN < TN;
             auto qk = [&](int t, int j) {
@@ -183,9 +183,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_prompt_tc(const __grid_constant_
 #pragma unroll
                 for (int k = 0; k < D / 16; k++) {
                     const uint32_t o = (k >> 2) * C::BLOCK + (k & 3) * 32;
-                    mma_f16(tmem + C::S_COL + t * TN, desc_k(qa + o), desc_k(ka + o), id_s, k > 0);
+                    mma_f16_ss(tmem + C::S_COL + t * TN, desc_k(qa + o), desc_k(ka + o), id_s, k > 0);
                 }
-                commit(s_full + t);
+                commit_mma(s_full + t);
             };
             auto pv = [&](int t, int j) {
                 const uint32_t va = smem_u32(ring + (2 * j + 1) % C::SLOTS * C::TILE);
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_prompt_tc(const __grid_constant_
                 for (int k = 0; k < TN / 16; k++)
                     mma_f16_ts(tmem + C::O_COL + t * D, tmem + C::S_COL + t * TN + 8 * k, desc_n(va + k * 2048, C::BLOCK),
                                id_o, j > 0 || k > 0);
-                commit(o_full + t);
+                commit_mma(o_full + t);
             };
             auto wait_full = [&](int i) { ok = ok && mbar_wait(full + i % C::SLOTS, (i / C::SLOTS) & 1, POLLS); };
             ok = mbar_wait(q_full, 0, POLLS);
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_prompt_tc(const __grid_constant_
             if (ok) {
                 for (int t = 0; t < 2; t++)
                     if (steps[t] > 0) qk(t, 0);
-                commit(empty + 0);
+                commit_mma(empty + 0);
             }
             for (int j = 0; j < n && ok; j++) {
                 wait_full(2 * j + 1);
@@ -215,9 +215,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_prompt_tc(const __grid_constant_
                         fence_after_sync();
                         pv(t, j);
                     }
-                    if (t == 1) commit(empty + (2 * j + 1) % C::SLOTS);
+                    if (t == 1) commit_mma(empty + (2 * j + 1) % C::SLOTS);
                     if (j + 1 < steps[t]) qk(t, j + 1);
-                    if (t == 1 && j + 1 < n) commit(empty + (2 * j + 2) % C::SLOTS);
+                    if (t == 1 && j + 1 < n) commit_mma(empty + (2 * j + 2) % C::SLOTS);
                 }
             }
         }

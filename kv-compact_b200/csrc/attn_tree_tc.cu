@@ -770,7 +770,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
         // ---- products
         each(kvc_int<0>{}, [&](const segment & S, int n) {
             __syncthreads();                             // Q is there
-            if (warp == 12 && lane == 0) {
+            if (warp == 12) {
                 fence_after_sync();
                 constexpr uint32_t ID_S = (1u << 4) | ((uint32_t)(TN >> 3) << 17) | ((uint32_t)(TM >> 4) << 24);
                 constexpr uint32_t ID_O = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(TM >> 4) << 24);
@@ -788,13 +788,13 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                         const uint32_t q = qa + (pr == 2 ? C::HALVES * C::QBLOCK : 0), k = ka + (pr == 1 ? C::PIECE : 0);
 #pragma unroll
                         for (int s = 0; s < D / 16; s++) {
-                            mma_f16(tmem + C::S_COL + (i & 1) * TN, desc_k(q + (s >> 2) * C::QBLOCK + (s & 3) * 32),
+                            mma_f16_ss(tmem + C::S_COL + (i & 1) * TN, desc_k(q + (s >> 2) * C::QBLOCK + (s & 3) * 32),
                                     desc_k(k + (s >> 2) * C::KBLOCK + (s & 3) * 32), ID_S, acc);
                             acc = 1;
                         }
                     }
-                    commit(X.s_full + (i & 1));
-                    commit(X.empty + it % C::SLOTS);
+                    commit_mma(X.s_full + (i & 1));
+                    commit_mma(X.empty + it % C::SLOTS);
                 };
                 auto pv = [&](int i) {
                     const int it = items + 2 * i + 1;
@@ -813,8 +813,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                             acc = 1;
                         }
                     }
-                    commit(X.o_full + (i & 1));
-                    commit(X.empty + it % C::SLOTS);
+                    commit_mma(X.o_full + (i & 1));
+                    commit_mma(X.empty + it % C::SLOTS);
                 };
                 if (n > 0) qk(0);
                 if (n > 1) qk(1);
