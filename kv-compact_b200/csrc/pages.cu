@@ -240,10 +240,11 @@ __global__ void __launch_bounds__(256) k_commit(cache_dev c, const __grid_consta
 
 // ---- row movement -----------------------------------------------------------
 //
-// A CTA moves MOVE_ROWS rows of one layer: their places are looked up once
-// into shared memory, then all threads copy the K bytes and the V bytes in
-// the widest pieces that the row sizes and base addresses allow (16 bytes for
-// the common shapes), MOVE_DEPTH loads in flight per thread. Bound by HBM.
+// A CTA moves up to MOVE_ROWS rows of one layer (fewer where there are not
+// enough to fill the machine): their places are looked up once into shared
+// memory, then all threads copy the K bytes and the V bytes in the widest
+// pieces that the row sizes and base addresses allow (16 bytes for the common
+// shapes), MOVE_DEPTH loads in flight per thread. Bound by HBM.
 constexpr int MOVE_ROWS = 32;
 constexpr int MOVE_THREADS = 256;
 constexpr int MOVE_DEPTH = 4;
@@ -254,6 +255,7 @@ struct move_args {
     cache_dev c;
     int mode;
     long long krb, vrb;             // bytes per row
+    int per;                        // rows of a CTA and step, <= MOVE_ROWS
     int rows;                       // rows per entry (MV_PAGES, MV_FORK, MV_COMPACT) or in all (MV_WRITE / MV_READ)
     kvc_divisor kdiv, vdiv;         // pieces per row
     const int * ws;
@@ -324,8 +326,8 @@ __global__ void __launch_bounds__(MOVE_THREADS) k_move_rows(const __grid_constan
     }
     const bool new_v = a.mode == MV_COMPACT && a.v_rows != nullptr;
     const uint8_t * new_v_from = new_v ? a.v_rows + ((long long)layer * a.n + item) * a.keep_ld * a.vrb : nullptr;
-    for (long long j0 = (long long)blockIdx.x * MOVE_ROWS; j0 < count; j0 += (long long)gridDim.x * MOVE_ROWS) {
-        const int rows = (int)min((long long)MOVE_ROWS, count - j0);
+    for (long long j0 = (long long)blockIdx.x * a.per; j0 < count; j0 += (long long)gridDim.x * a.per) {
+        const int rows = (int)min((long long)a.per, count - j0);
         __syncthreads();
         if (threadIdx.x < rows) {
             const int j = (int)j0 + threadIdx.x;
@@ -473,7 +475,10 @@ int launch_move(move_args & a, const kvc_page_cache * c, const plan_ids & ids, c
     a.vrb = (long long)c->v_row_bytes;
     a.kdiv = kvc_make_divisor((uint32_t)(c->k_row_bytes / kp));
     a.vdiv = kvc_make_divisor((uint32_t)(c->v_row_bytes / vp));
-    const long long tiles = (most + MOVE_ROWS - 1) / MOVE_ROWS;
+    // a quarter of the rows per CTA, and again, while there are fewer CTAs than two per SM
+    a.per = MOVE_ROWS;
+    while (a.per > 2 && (most + a.per - 1) / a.per * items * c->n_layers < 2LL * sms) a.per /= 4;
+    const long long tiles = (most + a.per - 1) / a.per;
     const long long want = (16LL * sms * 8 + (long long)items * c->n_layers - 1) / ((long long)items * c->n_layers);
     const dim3 grid((unsigned)(tiles < want ? tiles : want), (unsigned)c->n_layers, (unsigned)items);
     switch (kp) {
