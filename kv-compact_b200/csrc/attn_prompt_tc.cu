@@ -3,21 +3,24 @@
 //
 //   S = Q K^T,  P = exp2(c S - c m),  O = P V,  out = O / l,  c = scale log2 e
 //
-// A CTA takes 128 rows of one KV head: floor(128 / g) tokens times the g query
+// A tile is 128 rows of one KV head: floor(128 / g) tokens times the g query
 // heads that share it, so that keys and values are loaded once for the group
-// and short prompts fill the tile. It walks the keys in steps of 128. Two CTAs
-// share an SM: while one's softmax warps work, the tensor cores run the other's
-// products, and one's start and end lie under the other's steps (two tiles in
-// one CTA, 256 rows: prompt_packed 93 us against 87, prompt_chunk 124 against
-// 111, prompt_long 501 against 508).
+// and short prompts fill the tile. A tile walks the keys in steps of 128; while
+// one tile's softmax warps work, the tensor cores run the other's products. The
+// two are two CTAs of one SM (NT = 1: one's start and end lie under the other's
+// steps, and work is dealt in smaller pieces), or, for long sequences that fill
+// the machine several times, in one CTA, which then loads keys and values once
+// for both (NT = 2). prompt_packed 87 us against 93, prompt_chunk 111 against
+// 124, prompt_long 508 against 501.
 //
-//   warps 0-3  softmax: a thread owns a row. S comes from TMEM, P goes back as
-//              fp16 over S's columns, from where it is the second product's A
-//              operand (no shared memory). The reference maximum m moves only
-//              when a row's maximum has grown by more than 2^8 in P, so O is
-//              rarely rescaled.
-//   warp 4     TMA: Q once, then K and V through a ring of slots
-//   warp 5     MMA issue
+//   warps 0-3 (, 4-7)  softmax of tile 0 (, 1): a thread owns a row. S comes
+//                      from TMEM, P goes back as fp16 over S's columns, from
+//                      where it is the second product's A operand (no shared
+//                      memory). The reference maximum m moves only when a
+//                      row's maximum has grown by more than 2^8 in P, so O is
+//                      rarely rescaled.
+//   then one warp      TMA: Q once, then K and V through one ring of slots
+//   and one            MMA issue
 //
 // Rows, statistics and O are 32-bit; P is rounded to fp16 (2^-12 relative, as
 // the output is). Bound by the exponentials (16 per clock and SM against 4,096
@@ -33,19 +36,20 @@ using namespace kvc_tc;
 using namespace kvc_attn_tc;
 
 constexpr int TM = 128, TN = 128;               // rows and keys of a tile
-constexpr int THREADS = 192;
 constexpr uint32_t POLLS = 1u << 22;            // bound of every wait
 constexpr float LOG2E = 1.4426950408889634f;
 
-template <int D>
+// NT tiles in a CTA.
+template <int D, int NT>
 struct cfg {
     static constexpr int HALVES = D / 64;                   // 64-value column blocks of 128 bytes a row
     static constexpr int BLOCK = TN * 128;                  // bytes of such a block (128 rows)
     static constexpr int TILE = HALVES * BLOCK;
-    static constexpr int SLOTS = D == 128 ? 2 : 4;          // ring of K and V tiles
-    static constexpr int SMEM = 1024 + TILE + SLOTS * TILE + 256;
-    static constexpr uint32_t S_COL = 0, O_COL = TN;        // TMEM: S, then O
-    static constexpr uint32_t COLS = 256;
+    static constexpr int THREADS = 128 * NT + 64;
+    static constexpr int SLOTS = NT == 2 ? (D == 128 ? 5 : 8) : (D == 128 ? 2 : 4);  // ring of K and V tiles
+    static constexpr int SMEM = 1024 + NT * TILE + SLOTS * TILE + 256;
+    static constexpr uint32_t S_COL = 0, O_COL = NT * 128;  // TMEM: S of tile t at t*128, O behind them at t*D
+    static constexpr uint32_t COLS = NT * 256;
 };
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void * map, int x, int y, int z, uint64_t * bar) {
@@ -54,29 +58,29 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void * map, int 
 }
 
 struct prompt_geom {
-    int tokens;                 // of a CTA: floor(128 / g)
+    int tokens;                 // of a tile: floor(128 / g)
     int tiles;                  // upper bound of the CTAs per KV head
 };
 
-template <int D>
-__global__ void __launch_bounds__(THREADS, 2) k_prompt_tc(const __grid_constant__ kvc_attn_args a,
+template <int D, int NT>
+__global__ void __launch_bounds__(cfg<D, NT>::THREADS, 3 - NT) k_prompt_tc(const __grid_constant__ kvc_attn_args a,
                                                           const __grid_constant__ prompt_geom G,
                                                           const __grid_constant__ CUtensorMap q_map,
                                                           const __grid_constant__ CUtensorMap k_map,
                                                           const __grid_constant__ CUtensorMap v_map) {
-    using C = cfg<D>;
+    using C = cfg<D, NT>;
     extern __shared__ uint8_t sm_raw[];
     uint8_t * sm = aligned_1024(sm_raw);
-    uint8_t * sq = sm;
-    uint8_t * ring = sq + C::TILE;
+    uint8_t * sq = sm;                                   // Q tiles
+    uint8_t * ring = sq + NT * C::TILE;
     uint64_t * bars = reinterpret_cast<uint64_t *>(ring + C::SLOTS * C::TILE);
     uint64_t * full = bars;                              // [SLOTS] by TMA
     uint64_t * empty = full + C::SLOTS;                  // [SLOTS] by the MMAs that read it
     uint64_t * q_full = empty + C::SLOTS;
-    uint64_t * s_full = q_full + 1;                      // S is in TMEM
-    uint64_t * p_full = s_full + 1;                      // P is, and O may be added to
-    uint64_t * o_full = p_full + 1;                      // the product has been added
-    uint64_t * v_fixed = o_full + 1;                     // the last V tile's rows past the end are zero
+    uint64_t * s_full = q_full + 1;                      // [2] S of a tile is in TMEM
+    uint64_t * p_full = s_full + 2;                      // [2] P is, and O may be added to
+    uint64_t * o_full = p_full + 2;                      // [2] the product has been added
+    uint64_t * v_fixed = o_full + 2;                     // the last V tile's rows past the end are zero
     uint32_t * slot = reinterpret_cast<uint32_t *>(v_fixed + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int h = blockIdx.x % a.Hkv;
@@ -84,7 +88,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_prompt_tc(const __grid_constant_
     // the CTA's token tile: the last ones of a sequence, which see most keys, first
     int s = -1, q0 = 0, nq = 0, k0 = 0, nk = 0, tok0 = 0;
     {
-        const int per = G.tokens;
+        const int per = NT * G.tokens;
         int want = blockIdx.x / a.Hkv, at = 0;
         for (int s0 = 0; s0 < a.n_seqs && s < 0; s0 += 32) {
             kvc_attn_seq x{};
@@ -111,20 +115,28 @@ __global__ void __launch_bounds__(THREADS, 2) k_prompt_tc(const __grid_constant_
         }
     }
     if (s < 0) return;                                   // past the last tile
-    // keys that the tile sees, in steps of 128
-    const int last_tok = min(tok0 + G.tokens, nq) - 1;
-    const int n = ((a.causal ? min(nk, max(0, last_tok + nk - nq + 1)) : nk) + TN - 1) / TN;
+    // keys that the tiles see, in steps of 128
+    int n_keys[NT], steps[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        const int first = tok0 + t * G.tokens, last = min(first + G.tokens, nq) - 1;
+        n_keys[t] = last < first ? 0 : a.causal ? min(nk, max(0, last + nk - nq + 1)) : nk;
+        steps[t] = (n_keys[t] + TN - 1) / TN;
+    }
+    const int n = max(steps[0], steps[NT - 1]);
 
-    if (warp == 5) tmem_alloc(slot, C::COLS);
+    if (warp == 4 * NT + 1) tmem_alloc(slot, C::COLS);
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::SLOTS; i++) {
             mbar_init(full + i, 1);
             mbar_init(empty + i, 1);
         }
         mbar_init(q_full, 1);
-        mbar_init(s_full, 1);
-        mbar_init(p_full, 4);
-        mbar_init(o_full, 1);
+        for (int t = 0; t < 2; t++) {
+            mbar_init(s_full + t, 1);
+            mbar_init(p_full + t, 4);
+            mbar_init(o_full + t, 1);
+        }
         mbar_init(v_fixed, 1);
         mbar_init_fence();
     }
@@ -133,13 +145,15 @@ __global__ void __launch_bounds__(THREADS, 2) k_prompt_tc(const __grid_constant_
     const uint32_t tmem = *slot;
 
     bool ok = true;                                      // false: a wait ran out; the rows become NaN
-    if (warp == 4) {
+    if (warp == 4 * NT) {
         // ---- loads: slot 2j holds K of step j, slot 2j + 1 its V
         const int last_rows = nk - (n - 1) * TN;         // valid rows of the last V tile
         if (lane == 0 && n > 0) {
-            mbar_arrive_expect_tx(q_full, C::HALVES * (uint32_t)(G.tokens * a.g * 128));
-            for (int x = 0; x < C::HALVES; x++)
-                tma_load_3d(smem_u32(sq + x * C::BLOCK), &q_map, 64 * x, h * a.g, q0 + tok0, q_full);
+            mbar_arrive_expect_tx(q_full, NT * C::HALVES * (uint32_t)(G.tokens * a.g * 128));
+            for (int t = 0; t < NT; t++)
+                for (int x = 0; x < C::HALVES; x++)
+                    tma_load_3d(smem_u32(sq + t * C::TILE + x * C::BLOCK), &q_map, 64 * x, h * a.g,
+                                q0 + tok0 + t * G.tokens, q_full);
             for (int i = 0; i < 2 * n && ok; i++) {
                 const int st = i % C::SLOTS;
                 ok = mbar_wait(empty + st, ((i / C::SLOTS) & 1) ^ 1, POLLS);
@@ -165,61 +179,72 @@ __global__ void __launch_bounds__(THREADS, 2) k_prompt_tc(const __grid_constant_
             __syncwarp();
             if (lane == 0 && there) mbar_arrive(v_fixed);
         }
-    } else if (warp == 5) {
+    } else if (warp == 4 * NT + 1) {
         // ---- products
         if (n > 0) {
             const uint32_t id_s = idesc_f16(TM, TN), id_o = idesc_f16(TM, D) | 1u << 16;      // V is N-major
             const bool fixed = nk - (n - 1) * TN < TN;
-            auto qk = [&](int j) {
-                const uint32_t qa = smem_u32(sq), ka = smem_u32(ring + (2 * j) % C::SLOTS * C::TILE);
+            auto qk = [&](int t, int j) {
+                const uint32_t qa = smem_u32(sq + t * C::TILE), ka = smem_u32(ring + (2 * j) % C::SLOTS * C::TILE);
 #pragma unroll
                 for (int k = 0; k < D / 16; k++) {
                     const uint32_t o = (k >> 2) * C::BLOCK + (k & 3) * 32;
-                    mma_f16_ss(tmem + C::S_COL, desc_k(qa + o), desc_k(ka + o), id_s, k > 0);
+                    mma_f16_ss(tmem + C::S_COL + t * TN, desc_k(qa + o), desc_k(ka + o), id_s, k > 0);
                 }
-                commit_mma(s_full);
-                commit_mma(empty + (2 * j) % C::SLOTS);
+                commit_mma(s_full + t);
             };
-            auto pv = [&](int j) {
+            auto pv = [&](int t, int j) {
                 const uint32_t va = smem_u32(ring + (2 * j + 1) % C::SLOTS * C::TILE);
 #pragma unroll
                 for (int k = 0; k < TN / 16; k++)
-                    mma_f16_ts(tmem + C::O_COL, tmem + C::S_COL + 8 * k, desc_n(va + k * 2048, C::BLOCK), id_o, j > 0 || k > 0);
-                commit_mma(o_full);
-                commit_mma(empty + (2 * j + 1) % C::SLOTS);
+                    mma_f16_ts(tmem + C::O_COL + t * D, tmem + C::S_COL + t * TN + 8 * k, desc_n(va + k * 2048, C::BLOCK),
+                               id_o, j > 0 || k > 0);
+                commit_mma(o_full + t);
             };
             auto wait_full = [&](int i) { ok = ok && mbar_wait(full + i % C::SLOTS, (i / C::SLOTS) & 1, POLLS); };
             ok = mbar_wait(q_full, 0, POLLS);
             wait_full(0);
             fence_after_sync();
-            if (ok) qk(0);
+            if (ok) {
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+                    if (steps[t] > 0) qk(t, 0);
+                commit_mma(empty + 0);
+            }
             for (int j = 0; j < n && ok; j++) {
                 wait_full(2 * j + 1);
                 if (j == n - 1 && fixed) ok = ok && mbar_wait(v_fixed, 0, POLLS);
-                ok = ok && mbar_wait(p_full, j & 1, POLLS);
-                if (!ok) break;
-                fence_after_sync();
-                pv(j);                                   // reads P before the next scores go over it: MMAs run in order
-                if (j + 1 < n) {
-                    wait_full(2 * j + 2);
-                    if (ok) qk(j + 1);
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    if (!ok) break;
+                    if (j < steps[t]) {
+                        ok = mbar_wait(p_full + t, j & 1, POLLS);
+                        if (!ok) break;
+                        fence_after_sync();
+                        pv(t, j);
+                    }
+                    if (t == NT - 1) commit_mma(empty + (2 * j + 1) % C::SLOTS);
+                    if (t == 0 && j + 1 < n) wait_full(2 * j + 2);
+                    if (j + 1 < steps[t] && ok) qk(t, j + 1);
+                    if (t == NT - 1 && j + 1 < n) commit_mma(empty + (2 * j + 2) % C::SLOTS);
                 }
             }
         }
         __syncwarp();
     } else {
         // ---- softmax: thread = row
-        const uint32_t lanes = (uint32_t)(32 * warp) << 16;
-        const uint32_t s_addr = tmem + lanes + C::S_COL, o_addr = tmem + lanes + C::O_COL;
-        const int r = threadIdx.x;
-        const int tok = tok0 + (int)a.by_group.div(r);
+        const int t = NT == 1 ? 0 : warp >> 2;
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+        const uint32_t s_addr = tmem + lanes + C::S_COL + t * TN, o_addr = tmem + lanes + C::O_COL + t * D;
+        const int r = threadIdx.x & 127;
+        const int tok = tok0 + t * G.tokens + (int)a.by_group.div(r);
         const bool real = r < G.tokens * a.g && tok < nq;
         const int see = !real ? 0 : a.causal ? min(nk, max(0, tok + nk - nq + 1)) : nk;      // keys 0 .. see-1
-        const int see_all = tok0 + nk - nq + 1;                                              // of the tile's first row
+        const int see_all = tok0 + t * G.tokens + nk - nq + 1;                               // of the tile's first row
         const float c = a.scale * LOG2E;
         float m = -INFINITY, l = 0.0f;
-        for (int j = 0; j < n; j++) {
-            ok = ok && mbar_wait(s_full, j & 1, POLLS);
+        for (int j = 0; j < steps[t]; j++) {
+            ok = ok && mbar_wait(s_full + t, j & 1, POLLS);
             if (!__all_sync(~0u, ok)) break;
             fence_after_sync();
             float x[TN];
@@ -252,7 +277,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_prompt_tc(const __grid_constant_
                 const float fr = move ? f : 1.0f;
                 m = mn;
                 l *= fr;
-                ok = ok && mbar_wait(o_full, (j - 1) & 1, POLLS);
+                ok = ok && mbar_wait(o_full + t, (j - 1) & 1, POLLS);
                 if (!__all_sync(~0u, ok)) break;
                 fence_after_sync();
 #pragma unroll 1
@@ -282,10 +307,10 @@ __global__ void __launch_bounds__(THREADS, 2) k_prompt_tc(const __grid_constant_
             tmem_wait_st();
             fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive(p_full);
+            if (lane == 0) mbar_arrive(p_full + t);
         }
         // ---- output
-        if (n > 0) ok = ok && mbar_wait(o_full, (n - 1) & 1, POLLS);
+        if (steps[t] > 0) ok = ok && mbar_wait(o_full + t, (steps[t] - 1) & 1, POLLS);
         ok = __all_sync(~0u, ok);
         fence_after_sync();
         const size_t row = (size_t)(q0 + tok) * a.Hq + h * a.g + (r - (int)a.by_group.div(r) * a.g);
@@ -294,7 +319,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_prompt_tc(const __grid_constant_
 #pragma unroll 1
         for (int i = 0; i < D; i += 32) {
             float o[32];
-            if (n > 0) {
+            if (steps[t] > 0) {
                 ld32(o_addr + i, reinterpret_cast<uint32_t *>(o));
                 tmem_wait_ld();
             } else {
@@ -319,11 +344,11 @@ __global__ void __launch_bounds__(THREADS, 2) k_prompt_tc(const __grid_constant_
     }
     __syncthreads();
     // copies in flight land before the CTA ends (only where a wait ran out can there be any)
-    if (warp == 4 && lane < C::SLOTS && !ok) {
+    if (warp == 4 * NT && lane < C::SLOTS && !ok) {
         mbar_wait(full + lane, 0, POLLS);
         mbar_wait(full + lane, 1, POLLS);
     }
-    if (warp == 5) {
+    if (warp == 4 * NT + 1) {
         fence_after_sync();
         tmem_free(tmem, C::COLS);
     }
@@ -340,16 +365,17 @@ bool rows_map(CUtensorMap * m, const void * base, int d, int heads, int tokens, 
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D>
-int launch(const kvc_attn_args & a, const prompt_geom & G, const CUtensorMap * maps, cudaStream_t st) {
+template <int D, int NT>
+int launch(const kvc_attn_args & a, prompt_geom G, const CUtensorMap * maps, cudaStream_t st) {
     static std::atomic<bool> set[64];
     int dev = 0;
     KVC_CUDA(cudaGetDevice(&dev));
     if (!set[dev & 63].load(std::memory_order_relaxed)) {
-        KVC_CUDA(cudaFuncSetAttribute(k_prompt_tc<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, cfg<D>::SMEM));
+        KVC_CUDA(cudaFuncSetAttribute(k_prompt_tc<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, cfg<D, NT>::SMEM));
         set[dev & 63].store(true, std::memory_order_relaxed);
     }
-    k_prompt_tc<D><<<(unsigned)G.tiles * (unsigned)a.Hkv, THREADS, cfg<D>::SMEM, st>>>(a, G, maps[0], maps[1], maps[2]);
+    G.tiles = a.n_total / (NT * G.tokens) + a.n_seqs;    // each sequence's tiles, its last one perhaps partial
+    k_prompt_tc<D, NT><<<(unsigned)G.tiles * (unsigned)a.Hkv, cfg<D, NT>::THREADS, cfg<D, NT>::SMEM, st>>>(a, G, maps[0], maps[1], maps[2]);
     g_serve_launches++;
     KVC_CUDA(cudaGetLastError());
     return KVC_OK;
@@ -375,7 +401,6 @@ bool kvc_attn_prompt_tc_ok(const kvc_attn_args & a) {
 int kvc_launch_attn_prompt_tc(const kvc_attn_args & a, cudaStream_t st) {
     prompt_geom G;
     G.tokens = TM / a.g;
-    G.tiles = a.n_total / G.tokens + a.n_seqs;           // each sequence's tiles, its last one perhaps partial
     CUtensorMap maps[3];
     if (!rows_map(&maps[0], a.q, a.dk, a.Hq, a.n_total, a.q_head * 2, a.q_stride * 2, a.g, G.tokens) ||
         !rows_map(&maps[1], a.K, a.dk, a.Hkv, a.n_keys, a.k_hb, a.k_rb, 1, TN) ||
@@ -383,5 +408,8 @@ int kvc_launch_attn_prompt_tc(const kvc_attn_args & a, cudaStream_t st) {
         fprintf(stderr, "[kvc] cuTensorMapEncodeTiled failed for a prompt of %d rows\n", a.n_total);
         return KVC_ERR_CUDA;
     }
-    return (a.dk > 64 || a.dv > 64) ? launch<128>(a, G, maps, st) : launch<64>(a, G, maps, st);
+    // two tiles in a CTA for sequences of 4,096 queries and more on average that make 4 CTAs per SM
+    const bool two = a.n_total / a.n_seqs >= 4096 && (long long)a.n_total / (2 * G.tokens) * a.Hkv >= 4LL * kvc_serve_device();
+    if (a.dk > 64 || a.dv > 64) return two ? launch<128, 2>(a, G, maps, st) : launch<128, 1>(a, G, maps, st);
+    return two ? launch<64, 2>(a, G, maps, st) : launch<64, 1>(a, G, maps, st);
 }
