@@ -147,50 +147,51 @@ __device__ __forceinline__ uint32_t code_word(const raw_block & r, bool odd, int
     return odd || type == KV_TYPE_Q4_1 ? r.w[i + 1] : __funnelshift_r(r.w[i], r.w[i + 1], 16);
 }
 
-// 32 values of a block over 2^e as two fp16 pieces, 16 chunks of two values each.
-__device__ __forceinline__ void block_values(const raw_block & r, bool odd, int type, float up, uint32_t hi[16], uint32_t lo[16]) {
+// 32 values of a block over 2^e as two fp16 pieces, written as 16-byte chunks (8 values) through put(chunk, hi, lo).
+template <int TYPE, typename F>
+__device__ __forceinline__ void block_values(const raw_block & r, bool odd, float up, F && put) {
     uint32_t d, m;
-    block_head(r, odd, type, d, m);
-    const float fd = half_of(d) * up;                    // a power of two: exact but for tiny scales
-    if (type == KV_TYPE_Q8_0) {
-        const uint32_t d2 = pack(fd, fd);
+    block_head(r, odd, TYPE, d, m);
+    const float fd = half_of(d) * up, fm = half_of(m) * up;     // a power of two: exact but for tiny scales
+    const uint32_t d2 = pack(fd, fd);
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const uint32_t w = code_word(r, odd, type, i) ^ 0x80808080u;
-            const uint32_t c0 = h2add(__byte_perm(w, 0x64646464u, 0x4140), 0xE480E480u);   // 1024 + 128 + code, less 1152
-            const uint32_t c1 = h2add(__byte_perm(w, 0x64646464u, 0x4342), 0xE480E480u);
-            hi[2 * i] = h2mul(c0, d2);
-            hi[2 * i + 1] = h2mul(c1, d2);
-            lo[2 * i] = h2fma(c0, d2, hi[2 * i] ^ 0x80008000u);                            // exact
-            lo[2 * i + 1] = h2fma(c1, d2, hi[2 * i + 1] ^ 0x80008000u);
-        }
-    } else {
-        // a byte holds values 2i (low) and 2i + 1 (high): 0x6400 | n is 1024 + n, 0x6400 | 16 n is 1024 + 16 n
-        const uint32_t d2 = pack(fd, fd);
-        const float fm = half_of(m) * up;
+    for (int c = 0; c < 4; c++) {
+        uint32_t hi[4], lo[4];
+        if (TYPE == KV_TYPE_Q8_0) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint32_t w = code_word(r, odd, type, i);
+            for (int i = 0; i < 2; i++) {
+                const uint32_t w = code_word(r, odd, TYPE, 2 * c + i) ^ 0x80808080u;
+                const uint32_t c0 = h2add(__byte_perm(w, 0x64646464u, 0x4140), 0xE480E480u);   // 1024 + 128 + code, less 1152
+                const uint32_t c1 = h2add(__byte_perm(w, 0x64646464u, 0x4342), 0xE480E480u);
+                hi[2 * i] = h2mul(c0, d2);
+                hi[2 * i + 1] = h2mul(c1, d2);
+                lo[2 * i] = h2fma(c0, d2, hi[2 * i] ^ 0x80008000u);                            // exact
+                lo[2 * i + 1] = h2fma(c1, d2, hi[2 * i + 1] ^ 0x80008000u);
+            }
+        } else {
+            // a byte holds values 2i (low) and 2i + 1 (high): 0x6400 | n is 1024 + n, 0x6400 | 16 n is 1024 + 16 n
+            const uint32_t w = code_word(r, odd, TYPE, c);
 #pragma unroll
             for (int b = 0; b < 4; b++) {
                 const uint32_t n = __byte_perm(w, 0x64646464u, 0x4040 | b << 8 | b) & 0x64F0640Fu;
-                if (type == KV_TYPE_Q4_0) {              // (1024 + n0) - 1032, (1024 + 16 n1) / 16 - 72
-                    const uint32_t c = h2fma(n, 0x2C003C00u, 0xD480E408u);
-                    hi[4 * i + b] = h2mul(c, d2);
-                    lo[4 * i + b] = h2fma(c, d2, hi[4 * i + b] ^ 0x80008000u);               // exact
+                if (TYPE == KV_TYPE_Q4_0) {              // (1024 + n0) - 1032, (1024 + 16 n1) / 16 - 72
+                    const uint32_t q = h2fma(n, 0x2C003C00u, 0xD480E408u);
+                    hi[b] = h2mul(q, d2);
+                    lo[b] = h2fma(q, d2, hi[b] ^ 0x80008000u);                                 // exact
                 } else {
-                    const uint32_t c = h2fma(n, 0x2C003C00u, 0xD400E400u);
-                    __half2 hc, hh;
-                    memcpy(&hc, &c, 4);
-                    const float2 x = __half22float2(hc);
+                    const uint32_t q = h2fma(n, 0x2C003C00u, 0xD400E400u);
+                    __half2 hq, hh;
+                    memcpy(&hq, &q, 4);
+                    const float2 x = __half22float2(hq);
                     const float v0 = fmaf(x.x, fd, fm), v1 = fmaf(x.y, fd, fm);
-                    hi[4 * i + b] = pack(v0, v1);
-                    memcpy(&hh, &hi[4 * i + b], 4);
+                    hi[b] = pack(v0, v1);
+                    memcpy(&hh, &hi[b], 4);
                     const float2 f = __half22float2(hh);
-                    lo[4 * i + b] = pack(v0 - f.x, v1 - f.y);
+                    lo[b] = pack(v0 - f.x, v1 - f.y);
                 }
             }
         }
+        put(c, make_uint4(hi[0], hi[1], hi[2], hi[3]), make_uint4(lo[0], lo[1], lo[2], lo[3]));
     }
 }
 
@@ -274,15 +275,32 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
             const int rows_here = (int)min((long long)TM, (long long)S.nq * a.g - r0);
             {
                 // Q: two threads per row
+                const bool q_pairs = (reinterpret_cast<uintptr_t>(a.q) & (QP == 2 ? 7 : 3)) == 0 && (a.q_stride & 1) == 0;
                 const int row = threadIdx.x >> 1, part = threadIdx.x & 1;
                 const int i = (int)a.by_group.div(r0 + row);
                 const long long at = (long long)(S.q0 + i) * a.q_stride + (long long)(h * a.g + (r0 + row - i * a.g)) * a.q_head;
+                // this thread's half of the row, pairs of values; read at once, so that the latencies overlap
+                float2 v[D / 4];
+#pragma unroll
+                for (int k = 0; k < D / 4; k++) {
+                    const int d = part * (D / 2) + 2 * k;
+                    v[k] = make_float2(0.0f, 0.0f);
+                    if (row < rows_here && d < a.dk) {
+                        if (QP == 2) {
+                            const float * p = reinterpret_cast<const float *>(a.q) + at + d;
+                            v[k] = q_pairs ? *reinterpret_cast<const float2 *>(p) : make_float2(p[0], p[1]);
+                        } else {
+                            const __half * p = reinterpret_cast<const __half *>(a.q) + at + d;
+                            v[k] = q_pairs ? __half22float2(*reinterpret_cast<const __half2 *>(p))
+                                           : make_float2(__half2float(p[0]), __half2float(p[1]));
+                        }
+                    }
+                }
                 float up = 1.0f;
                 if (QP == 2) {
                     float top = 0.0f;
-                    if (row < rows_here)
-                        for (int d = part * (D / 2); d < (part + 1) * (D / 2); d++)
-                            if (d < a.dk) top = fmaxf(top, fabsf(reinterpret_cast<const float *>(a.q)[at + d]));
+#pragma unroll
+                    for (int k = 0; k < D / 4; k++) top = fmaxf(top, fmaxf(fabsf(v[k].x), fabsf(v[k].y)));
                     top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
                     float down = 1.0f;
                     // largest value of the row in [2^13, 2^14): both pieces normal numbers
@@ -293,26 +311,20 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                     }
                     if (part == 0) X.mul[row] = down;
                 }
-#pragma unroll 2
-                for (int c = part * (D / 16); c < (part + 1) * (D / 16); c++) {          // chunks of 8 values
-                    float v[8];
 #pragma unroll
-                    for (int k = 0; k < 8; k++) {
-                        v[k] = 0.0f;
-                        if (row < rows_here && 8 * c + k < a.dk)
-                            v[k] = QP == 2 ? reinterpret_cast<const float *>(a.q)[at + 8 * c + k] * up
-                                           : __half2float(reinterpret_cast<const __half *>(a.q)[at + 8 * c + k]);
-                    }
+                for (int c = 0; c < D / 16; c++) {       // chunks of 8 values
                     uint32_t hi[4], lo[4];
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
-                        hi[k] = pack(v[2 * k], v[2 * k + 1]);
+                        const float x = v[4 * c + k].x * up, y = v[4 * c + k].y * up;
+                        hi[k] = pack(x, y);
                         __half2 hh;
                         memcpy(&hh, &hi[k], 4);
                         const float2 f = __half22float2(hh);
-                        lo[k] = pack(v[2 * k] - f.x, v[2 * k + 1] - f.y);
+                        lo[k] = pack(x - f.x, y - f.y);
                     }
-                    uint8_t * dst = sq + (c >> 3) * C::QBLOCK + swizzled(row, c & 7);
+                    const int chunk = part * (D / 16) + c;
+                    uint8_t * dst = sq + (chunk >> 3) * C::QBLOCK + swizzled(row, chunk & 7);
                     *reinterpret_cast<uint4 *>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                     if (QP == 2)
                         *reinterpret_cast<uint4 *>(dst + C::HALVES * C::QBLOCK) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
@@ -334,12 +346,13 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                 const float2 b2 = make_float2(back, back), f2 = make_float2(f, f);
                 const bool moved = __any_sync(~0u, f != 1.0f);
 #pragma unroll
-                for (int c = 0; c < D; c += 16) {
-                    uint32_t o[16];
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t o[32];
                     tmem_ld16_nowait(o_addr + c, o);
+                    tmem_ld16_nowait(o_addr + c + 16, o + 16);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int k = 0; k < 8; k++) {
+                    for (int k = 0; k < 16; k++) {
                         float2 & x = O[c / 2 + k];
                         x = fma2(make_float2(__uint_as_float(o[2 * k]), __uint_as_float(o[2 * k + 1])), b2, x);
                     }
@@ -417,11 +430,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                 int R = HIDDEN;
                 float sum = 0.0f;
                 if (KP == 2 || own) {
+                    const int it = items + 2 * i + 1;    // the exponents are written with V
+                    await(X.full + it % C::SLOTS, (it / C::SLOTS) & 1);
                     const int2 e2 = *reinterpret_cast<const int2 *>(&I.e[2 * lane]);
                     R = __reduce_max_sync(~0u, max(e2.x, e2.y));
                     if (own) {
-                        const int it = items + 2 * i + 1;
-                        await(X.full + it % C::SLOTS, (it / C::SLOTS) & 1);
                         uint8_t * vt = ring + (it % C::SLOTS) * C::SLOT;
                         if (r == 0) X.bad[t] = 0;
                         const int least = __reduce_min_sync(~0u, min(e2.x > HIDDEN ? e2.x : INT_MAX, e2.y > HIDDEN ? e2.y : INT_MAX));
@@ -672,95 +685,99 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                 const int part = tid & 1;
                 const int kbb = kvc_block_size(a.k_type), vbb = kvc_block_size(a.v_type);
                 const int nbk = a.dk >> 5, nbv = a.dv >> 5;
-                raw_block K[PER], V[PER];
+                raw_block K[PER], V[PER], R[PER];
                 uint32_t odd_k = 0, odd_v = 0;
                 // an absent row reads the pool's first one: every address is one of the pool's
-                auto read = [&](int row) {
-                    odd_k = odd_v = 0;
-                    const long long at = row < 0 ? 0 : row;
+                auto read = [&](raw_block * R, uint32_t & odd, const uint8_t * base, long long rb, long long hb, int size, int nb,
+                                int type, int row) {
+                    odd = 0;
+                    const uint8_t * at = base + (row < 0 ? 0 : row) * rb + (long long)h * hb;
 #pragma unroll
                     for (int b = 0; b < PER; b++) {
                         const int bb = part * PER + b;
-                        const uint8_t * pk = a.K + at * a.k_rb + (long long)h * a.k_hb + (bb < nbk ? bb : 0) * kbb;
-                        const uint8_t * pv = a.V + at * a.v_rb + (long long)h * a.v_hb + (bb < nbv ? bb : 0) * vbb;
-                        odd_k |= (uint32_t)((uintptr_t)pk >> 1 & 1) << b;
-                        odd_v |= (uint32_t)((uintptr_t)pv >> 1 & 1) << b;
-                        read_block(K[b], pk, a.k_type);
-                        read_block(V[b], pv, a.v_type);
+                        const uint8_t * p = at + (bb < nb ? bb : 0) * size;
+                        odd |= (uint32_t)((uintptr_t)p >> 1 & 1) << b;
+                        read_block(R[b], p, type);
                     }
                 };
+                // one side of tile i from its raw blocks: two pieces over 2^e, e the exponent of the row's largest finite
+                // scale or minimum, which is returned
+                auto convert = [&](uint32_t odd, int type, int nb, int it, bool live) {
+                    uint32_t top = 0;
+#pragma unroll
+                    for (int b = 0; b < PER; b++)
+                        if (part * PER + b < nb) {
+                            uint32_t d, m;
+                            block_head(R[b], (odd >> b) & 1, type, d, m);
+                            d &= 0x7FFFu, m &= 0x7FFFu;
+                            top = max(top, max(d < 0x7C00u ? d : 0u, m < 0x7C00u ? m : 0u));
+                        }
+                    top = max(top, __shfl_xor_sync(~0u, top, 1));
+                    const int e = max((int)(top >> 10), 1) - 15;
+                    const float up = __int_as_float((127 - e) << 23);
+                    await(X.empty + it % C::SLOTS, ((it / C::SLOTS) & 1) ^ 1);
+                    uint8_t * dst = ring + (it % C::SLOTS) * C::SLOT;
+#pragma unroll
+                    for (int b = 0; b < PER; b++) {
+                        const int bb = part * PER + b;
+                        uint8_t * at = dst + (bb >> 1) * C::KBLOCK;
+                        auto put = [&](int c, uint4 hi, uint4 lo) {
+                            uint8_t * p = at + swizzled(key, (bb & 1) * 4 + c);
+                            *reinterpret_cast<uint4 *>(p) = hi;
+                            *reinterpret_cast<uint4 *>(p + C::PIECE) = lo;
+                        };
+                        const bool o = (odd >> b) & 1;
+                        if (!live || bb >= nb) {
+#pragma unroll
+                            for (int c = 0; c < 4; c++) put(c, make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0));
+                        } else if (type == KV_TYPE_Q8_0) {
+                            block_values<KV_TYPE_Q8_0>(R[b], o, up, put);
+                        } else if (type == KV_TYPE_Q4_0) {
+                            block_values<KV_TYPE_Q4_0>(R[b], o, up, put);
+                        } else {
+                            block_values<KV_TYPE_Q4_1>(R[b], o, up, put);
+                        }
+                    }
+                    return e;
+                };
+                auto read_k = [&](int row) { read(K, odd_k, a.K, a.k_rb, a.k_hb, kbb, nbk, a.k_type, row); };
+                auto read_v = [&](int row) { read(V, odd_v, a.V, a.v_rb, a.v_hb, vbb, nbv, a.v_type, row); };
                 int page = page_of(0);
                 int row = place(0, page);
                 float bias = bias_of(row);
-                read(row);
+                read_k(row);
+                read_v(row);
                 page = page_of(1);
                 for (int i = 0; i < n; i++) {
                     const bool live = row >= 0 && bias != -INFINITY;
                     const float bias_now = bias;
-                    const int row_next = place(i + 1, page);
-                    bias = bias_of(row_next);
+                    row = place(i + 1, page);
+                    bias = bias_of(row);
                     page = page_of(i + 2);
-                    for (int side = 0; side < 2; side++) {
-                        const int it = items + 2 * i + side, type = side ? a.v_type : a.k_type, nb = side ? nbv : nbk;
-                        const uint32_t odd = side ? odd_v : odd_k;
-                        // the exponent of the row's largest finite scale (or minimum)
-                        uint32_t top = 0;
+#pragma unroll 1
+                    for (int side = 0; side < 2; side++) {       // one body for both sides: the loop has to stay in the instruction cache
 #pragma unroll
                         for (int b = 0; b < PER; b++)
-                            if (part * PER + b < nb) {
-                                uint32_t d, m;
-                                block_head(side ? V[b] : K[b], (odd >> b) & 1, type, d, m);
-                                d &= 0x7FFFu, m &= 0x7FFFu;
-                                top = max(top, max(d < 0x7C00u ? d : 0u, m < 0x7C00u ? m : 0u));
-                            }
-                        top = max(top, __shfl_xor_sync(~0u, top, 1));
-                        const int e = max((int)(top >> 10), 1) - 15;
-                        const float up = __int_as_float((127 - e) << 23);
-                        await(X.empty + it % C::SLOTS, ((it / C::SLOTS) & 1) ^ 1);
-                        uint8_t * dst = ring + (it % C::SLOTS) * C::SLOT;
 #pragma unroll
-                        for (int b = 0; b < PER; b++) {
-                            const int bb = part * PER + b;
-                            uint32_t hi[16], lo[16];
-                            if (live && bb < nb) {
-                                block_values(side ? V[b] : K[b], (odd >> b) & 1, type, up, hi, lo);
-                            } else {
-#pragma unroll
-                                for (int k = 0; k < 16; k++) hi[k] = lo[k] = 0;
-                            }
-#pragma unroll
-                            for (int c = 0; c < 4; c++) {
-                                uint8_t * d = dst + (bb >> 1) * C::KBLOCK + swizzled(key, (bb & 1) * 4 + c);
-                                *reinterpret_cast<uint4 *>(d) = make_uint4(hi[4 * c], hi[4 * c + 1], hi[4 * c + 2], hi[4 * c + 3]);
-                                *reinterpret_cast<uint4 *>(d + C::PIECE) = make_uint4(lo[4 * c], lo[4 * c + 1], lo[4 * c + 2], lo[4 * c + 3]);
-                            }
-                        }
+                            for (int u = 0; u < 9; u++) R[b].w[u] = side ? V[b].w[u] : K[b].w[u];
+                        const uint32_t odd = side ? odd_v : odd_k;
+                        // the next tile's K comes in under this one's V, its V under the next K
+                        if (side == 0) read_k(row);
+                        else read_v(row);
+                        const int it = items + 2 * i + side;
+                        const int e = convert(odd, side ? a.v_type : a.k_type, side ? nbv : nbk, it, live);
                         if (part == 0) {
                             tile_info & I = X.info[i & 7];
                             if (side == 0) {
                                 I.f[key] = a.scale * scalbnf(1.0f, e);
                                 I.b[key] = live ? bias_now : -INFINITY;
+                            } else {
+                                I.e[key] = live ? e * (1 << 23) : HIDDEN;
                             }
-                        }
-                        if (side == 0) {
-                            // V's exponent is read with the scores: it has to be there with K
-                            uint32_t tv = 0;
-#pragma unroll
-                            for (int b = 0; b < PER; b++)
-                                if (part * PER + b < nbv) {
-                                    uint32_t d, m;
-                                    block_head(V[b], (odd_v >> b) & 1, a.v_type, d, m);
-                                    d &= 0x7FFFu, m &= 0x7FFFu;
-                                    tv = max(tv, max(d < 0x7C00u ? d : 0u, m < 0x7C00u ? m : 0u));
-                                }
-                            tv = max(tv, __shfl_xor_sync(~0u, tv, 1));
-                            if (part == 0) X.info[i & 7].e[key] = live ? (max((int)(tv >> 10), 1) - 15) * (1 << 23) : HIDDEN;
                         }
                         fence_smem_to_async();
                         mbar_arrive(X.full + it % C::SLOTS);
                     }
-                    row = row_next;
-                    if (i + 1 < n) read(row);
                 }
             }
             // (the softmax warps' barriers of the join are theirs alone)
