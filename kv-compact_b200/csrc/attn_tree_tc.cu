@@ -889,7 +889,17 @@ bool block_type(int t) { return t == KV_TYPE_Q8_0 || t == KV_TYPE_Q4_0 || t == K
 bool kvc_attn_tree_tc_plan(kvc_attn_args * a, int sms, long long * blocks) {
     const int top = a->dk > a->dv ? a->dk : a->dv;
     const long long rows = (long long)a->max_q * a->g;
-    if (rows < 24 || top > 128 || a->dk % 32 || a->dv % 32) return false;
+    // k_tree_mma takes 32 rows at a time and its time grows with them; this
+    // kernel's hardly does up to 128 rows, but putting two fp16 pieces of 128
+    // values into the tiles costs it most. 43,000 keys x 8 heads, us here / there:
+    //   rows                 32         36         64         80
+    //   F16, d 64         73 / 72    73 / 99   77 / 105   78 / 171
+    //   Q8_0, d 64       106 / 71  107 / 108  112 / 113  111 / 206
+    //   F16, d 128      103 / 104  103 / 144  108 / 156  109 / 229
+    //   Q8_0, d 128     222 / 117  222 / 164  227 / 175  226 / 297
+    //   Q4_0, d 128     178 / 97   180 / 148  189 / 156  190 / 286
+    const long long few = a->k_type != KV_TYPE_F16 && top > 64 ? 64 : 32;
+    if (rows <= few || top > 128 || a->dk % 32 || a->dv % 32) return false;
     if (a->k_type == KV_TYPE_F16 && a->v_type == KV_TYPE_F16) {
         // 16-byte pieces of a head's part of a row
         if (((uintptr_t)a->K | (uintptr_t)a->V | (uintptr_t)a->k_rb | (uintptr_t)a->v_rb) & 15) return false;

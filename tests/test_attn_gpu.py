@@ -324,6 +324,114 @@ def test_tree_refuses_a_small_workspace(kvc):
     assert t.fn(cache, desc, ws + 4, size, None) == -13
 
 
+def many_rows(**kw):
+    """Sequences with enough nodes that the kernels for many query rows take them, at head size d too."""
+    return dict(dict(lens=[200, 0, 70, 513], nodes=[24, 40, 1, 33], hkv=2, g=4, page=16, beta=True), **kw)
+
+
+@pytest.mark.parametrize("qt", [torch.float16, torch.float32])
+@pytest.mark.parametrize("vt", KINDS)
+@pytest.mark.parametrize("kt", KINDS)
+def test_tree_many_rows_types(kvc, kt, vt, qt):
+    tree_check(kvc, **many_rows(kt=kt, vt=vt, qt=qt, seed=kt * 10 + vt))
+
+
+@pytest.mark.parametrize("dk,dv", [(32, 64), (64, 128), (128, 32), (96, 96), (128, 128)])
+@pytest.mark.parametrize("kind", [R.F16, R.Q8_0, R.Q4_0, R.Q4_1])
+@pytest.mark.parametrize("qt", [torch.float16, torch.float32])
+def test_tree_many_rows_head_sizes(kvc, dk, dv, kind, qt):
+    tree_check(kvc, **many_rows(dk=dk, dv=dv, kt=kind, vt=kind, qt=qt, seed=dk + dv))
+
+
+@pytest.mark.parametrize("rows", [9, 16, 17, 32, 33, 64, 65, 127, 128, 129, 260])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("kind", [R.F16, R.Q8_0])
+def test_tree_row_counts(kvc, rows, d, kind):
+    """Each number of query rows on either side of a kernel's rows, with one head to a KV head."""
+    tree_check(kvc, lens=[300, 40], nodes=[rows, 3], hkv=2, g=1, dk=d, dv=d, kt=kind, vt=kind, page=24, seed=rows)
+
+
+@pytest.mark.parametrize("page", [1, 7, 64, 100, 256])
+@pytest.mark.parametrize("kind", [R.F16, R.Q8_0])
+def test_tree_many_rows_pages(kvc, page, kind):
+    tree_check(kvc, **many_rows(page=page, kt=kind, vt=kind, hkv=3, g=5, seed=page))
+
+
+@pytest.mark.parametrize("kind", [R.F16, R.Q8_0, R.Q4_1])
+@pytest.mark.parametrize("qt", [torch.float16, torch.float32])
+def test_tree_many_rows_that_see_nothing(kvc, kind, qt):
+    t = tree_check(kvc, lens=[0, 20], nodes=[30, 2], kt=kind, vt=kind, qt=qt, mask="none")
+    assert float(t.out[:30].abs().max()) == 0.0 and bool((t.lse[:30] == -math.inf).all())
+    t = tree_check(kvc, **many_rows(kt=kind, vt=kind, qt=qt, edit=lambda c, q: c.beta.fill_(-math.inf)))
+    assert float(t.out.abs().max()) == 0.0 and bool((t.lse == -math.inf).all())
+    low = torch.finfo(torch.float32).min
+    tree_check(kvc, **many_rows(kt=kind, vt=kind, qt=qt, edit=lambda c, q: c.beta.fill_(low)))
+
+
+@pytest.mark.parametrize("kind", [R.F16, R.Q8_0, R.Q4_0, R.Q4_1])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("qt", [torch.float16, torch.float32])
+def test_tree_many_rows_hidden_rows_may_hold_anything(kvc, kind, bad, qt):
+    """As above where 128 query rows share a tile: rows behind beta, the last node's own row, free pages."""
+    def edit(c, q):
+        rows = c.rows(0)
+        hidden = [int(rows[i]) for i in (0, 5, 63, 64, 130)]
+        for r in hidden:
+            c.beta[0, r // c.page, :, r % c.page] = -math.inf
+        used = torch.cat([c.rows(i) for i in range(3)])
+        free = sorted(set(range(c.n_pages * c.page)) - set(used.tolist()))
+        for store, t in ((c.K, c.kt), (c.V, c.vt)):
+            for r in hidden + c.rows(0)[-1:].tolist() + free:
+                if t == R.F16:
+                    store[0, r].view(torch.float16).fill_(bad)
+                else:
+                    b = store[0, r].view(-1, R.BLOCK[t])
+                    b[:, :2] = torch.tensor([bad], dtype=torch.float16).view(torch.uint8).to(b.device)
+    nodes = [40, 3, 20]
+    c, q, t, (out, lse) = tree_case(kvc, lens=[150, 20, 64], nodes=nodes, kt=kind, vt=kind, beta=True, page=16, qt=qt, edit=edit)
+    used = torch.cat([c.rows(i) for i in range(3)])
+    K, V = (R.decode(x[0][used], kind).nan_to_num(0.0, 0.0, 0.0) for x in (c.K, c.V))
+    t.run()
+    torch.cuda.synchronize()
+    ok = torch.ones(sum(nodes), dtype=torch.bool, device="cuda")
+    ok[nodes[0] - 1] = False                           # only the last node sees the bad row of its own
+    o_tol, l_tol = bounds(q, K.view(-1, c.hkv, c.dk), V, float(c.beta[c.beta.isfinite()].abs().max()), kind,
+                          qt == torch.float16, c.dk ** -0.5)
+    check(t.out[ok], out[ok], o_tol, "out")
+    check(t.lse[ok], lse[ok], l_tol, "lse")
+    assert not bool(torch.isfinite(t.out[nodes[0] - 1]).all())
+
+
+def test_tree_many_rows_large_and_small_scales(kvc):
+    for size in (1e-6, 1e-2, 3e3):
+        def edit(c, q):
+            for store, t in ((c.K, c.kt), (c.V, c.vt)):
+                b = store[0].view(-1, R.BLOCK[t])
+                d = b[:, :2].contiguous().view(torch.float16).float() * size
+                b[:, :2] = d.half().view(torch.uint8)
+            q.mul_(1.0 / size)
+        for kind in (R.Q8_0, R.Q4_1):
+            tree_check(kvc, lens=[100], nodes=[36], kt=kind, vt=kind, qt=torch.float32, edit=edit, seed=11)
+
+
+def test_tree_many_rows_bad_pages(kvc):
+    for kt in (R.F16, R.Q8_0):
+        c, q, t, _ = tree_case(kvc, lens=[200], nodes=[36], hkv=2, page=16, kt=kt, vt=kt, qt=torch.float32, beta=True,
+                               mask=None)
+        c.table[0, 1], c.table[0, 4] = -1, c.n_pages
+        t.run()
+        torch.cuda.synchronize()
+        n = int(c.seq_len[0])
+        keep = [r for r in range(n) if r // 16 not in (1, 4)]
+        table = c.table[0].tolist()
+        rows = torch.tensor([table[r // 16] * 16 + r % 16 for r in keep], device="cuda")
+        K, V = R.decode(c.K[0][rows], kt).view(-1, 2, 64), R.decode(c.V[0][rows], kt).view(-1, 2, 64)
+        for h in range(q.shape[1]):
+            see = torch.ones(36, len(keep), dtype=torch.bool, device="cuda")
+            o, w = R.attend(q[:, h], K[:, h // 4], V[:, h // 4], c.beta[0, rows // 16, h // 4, rows % 16], see, 64 ** -0.5)
+            assert float((t.out[:, h].double() - o).abs().max()) < 1e-4 and float((t.lse[:, h].double() - w).abs().max()) < 1e-4
+
+
 # ---- prompts ------------------------------------------------------------------------------
 
 def prompt_case(new, past, hkv=2, g=4, dk=64, dv=64, dtype=torch.float16, causal=True, seed=0, wide=False, scale=None, edit=None):
@@ -402,6 +510,32 @@ def test_prompt_groups(kvc, g):
 def test_prompt_many_sequences(kvc):
     new = [(i * 29) % 50 for i in range(90)]
     prompt_check(kvc, new, [(i * 7) % 13 for i in range(90)], hkv=2, g=2)
+
+
+@pytest.mark.parametrize("d,causal", [(64, True), (128, True), (64, False)])
+def test_prompt_long_sequence(kvc, d, causal):
+    """One sequence long enough that a CTA takes two tiles; some rows of some heads against the definition."""
+    gen = torch.Generator().manual_seed(d)
+    n, past, hkv, g = 4801, 77, 8, 4
+    rnd = lambda *s: torch.randn(*s, generator=gen).to("cuda", torch.float16)  # noqa: E731
+    q, k, v = rnd(n, hkv * g, d), rnd(n + past, hkv, d), rnd(n + past, hkv, d)
+    cu = lambda x: torch.tensor([0, x], dtype=torch.int32, device="cuda")  # noqa: E731
+    p = attn.Prompt(kvc, q, k, v, cu(n), cu(n + past), scale=d ** -0.5, causal=causal)
+    p.out.fill_(7.0)
+    p.run()
+    torch.cuda.synchronize()
+    at = torch.tensor([0, 1, 31, 32, 63, 64, 65, 2047, 2048, 4735, 4736, 4767, 4768, 4799, 4800], device="cuda")
+    j = torch.arange(n + past, device="cuda")[None]
+    see = (j <= at[:, None] + past) if causal else (j >= 0).expand(len(at), -1)
+    o_tol, l_tol = bounds(q, k.double(), v.double(), 0.0, R.F16, True, d ** -0.5)
+    for h in (0, 3, 13, 31):
+        o, w = R.attend(q[at, h], k[:, h // g].double(), v[:, h // g].double(), None, see, d ** -0.5)
+        check(p.out[at, h], o, o_tol, "out")
+        check(p.lse[at, h], w, l_tol, "lse")
+    first = p.out.clone()
+    p.run()
+    torch.cuda.synchronize()
+    assert torch.equal(first, p.out) and bool(torch.isfinite(p.lse).all())
 
 
 def test_prompt_fewer_keys_than_queries(kvc):
