@@ -236,10 +236,6 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void * map, int 
                  :: "r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar)) : "memory");
 }
 
-__device__ __forceinline__ void arrive(uint64_t * bar, int count) {
-    asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0], %1;" :: "r"(smem_addr(bar)), "r"(count) : "memory");
-}
-
 // One slot of the shared region: a unit's query fragments in two pieces (in the
 // loop), or a warp's output, maxima and sums (when the warps of a unit are joined).
 constexpr int slot_bytes(int db, int nb) { return db * nb * 1024 + nb * 512; }
@@ -886,22 +882,19 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
 
         int turn = sub;                                  // groups until this warp's next one
         for (int i = lo; i < hi; i++) {
-            const int keys = min(KT, q.ln - i * KT), groups = (keys + KEYS - 1) / KEYS;
-            if (active && turn < groups) {
-                await(full + c_stage, c_phase);
-                const uint8_t * st = ring + (size_t)c_stage * G.stage_bytes;
-                const uint8_t * sv = st + KT * G.kp;
-                const uint32_t missing = tma ? bad[c_stage] : 0;
-                // the first reader of a unit also counts for the warps that have nothing of this tile, which pass it by
-                const int arrivals = 1 + (turn ? 0 : max(nsub - groups, 0) + (unit ? 0 : NW - units * nsub));
-                for (; turn < groups; turn += nsub)
-                    group(i * KT + KEYS * turn, KEYS * turn, st + KEYS * turn * G.kp + k_off + hc * (int)a.k_hb,
-                          sv + KEYS * turn * G.vp + v_off + hc * (int)a.v_hb,
+            await(full + c_stage, c_phase);
+            const uint8_t * st = ring + (size_t)c_stage * G.stage_bytes;
+            const uint8_t * sv = st + KT * G.kp;
+            const uint32_t missing = tma ? bad[c_stage] : 0;
+            const int keys = min(KT, q.ln - i * KT);
+            for (int k = 0; k < keys; k += KEYS) {
+                if (active && turn == 0)
+                    group(i * KT + k, k, st + k * G.kp + k_off + hc * (int)a.k_hb, sv + k * G.vp + v_off + hc * (int)a.v_hb,
                           reinterpret_cast<const float *>(sv + KT * G.vp), missing);
-                __syncwarp();
-                if (lane == 0) arrive(empty + c_stage, arrivals);
+                turn = turn == 0 ? nsub - 1 : turn - 1;
             }
-            turn -= groups;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty + c_stage);
             step(c_stage, c_phase);
             if (f_tile == tile + G.stages - G.lag) fill();
             tile++;

@@ -138,6 +138,19 @@ def test_tree_lengths(kvc, n, qt):
     tree_check(kvc, lens=[n], nodes=[1], hkv=8, g=4, dk=128, dv=128, page=16, qt=qt, beta=True, seed=n)
 
 
+@pytest.mark.parametrize("hkv", [1, 3, 5, 8, 11])
+@pytest.mark.parametrize("kind,qt,page", [(R.Q8_0, torch.float32, 64), (R.F16, torch.float16, 32), (R.Q4_1, torch.float32, 5)])
+def test_tree_long(kvc, hkv, kind, qt, page):
+    """Stretches of many tiles per CTA, so that its ring of tiles turns several times, with warps to spare or not."""
+    tree_check(kvc, lens=[30000, 25000 // hkv], nodes=[1, 1], hkv=hkv, g=2, dk=128, dv=128, kt=kind, vt=kind, qt=qt, page=page,
+               beta=True, seed=hkv)
+
+
+@pytest.mark.parametrize("kind,qt", [(R.Q8_0, torch.float32), (R.F16, torch.float16), (R.F16, torch.float32)])
+def test_tree_many_rows_long(kvc, kind, qt):
+    tree_check(kvc, lens=[60000], nodes=[35], hkv=3, g=2, dk=128, dv=128, kt=kind, vt=kind, qt=qt, page=64, beta=True)
+
+
 @pytest.mark.parametrize("nodes", [[2], [33], [64, 1, 30], [100], [0, 5, 0]])
 @pytest.mark.parametrize("g", [1, 4])
 def test_tree_nodes(kvc, nodes, g):
