@@ -4,7 +4,9 @@
 ``Prompt`` and ``Tree`` hold the tensors and buffers of one call shape;
 ``run()`` queues the kernels on the current stream of the tensors' device and
 returns the output without waiting. The tensors are read at every run, so a
-program refills them in place (or captures the run into a graph).
+program refills them in place (or captures the run into a graph). Runs of one
+object write its output and workspace: order them, or make an object for each
+stream. Its tensors must live until the queued work is done.
 """
 import ctypes
 from ctypes import Structure, c_float, c_int, c_longlong, c_void_p

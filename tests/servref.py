@@ -41,7 +41,7 @@ def decode(raw, kind):
         return raw.view(torch.float32).double()
     if kind == F16:
         return raw.view(torch.float16).double()
-    b = raw.view(raw.shape[0], -1, BLOCK[kind])
+    b = raw.view(raw.shape[0], raw.shape[1] // BLOCK[kind], BLOCK[kind])
     d = b[..., :2].contiguous().view(torch.float16).double()
     if kind == Q8_0:
         return (b[..., 2:].contiguous().view(torch.int8).double() * d).flatten(1)

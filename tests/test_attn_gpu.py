@@ -445,6 +445,98 @@ def test_tree_many_rows_bad_pages(kvc):
             assert float((t.out[:, h].double() - o).abs().max()) < 1e-4 and float((t.lse[:, h].double() - w).abs().max()) < 1e-4
 
 
+@pytest.mark.parametrize("kind", [R.F32, R.F16, R.Q8_0])
+@pytest.mark.parametrize("nodes", [[2, 2, 1], [40, 40, 3]])
+def test_tree_one_sequence_read_twice(kvc, kind, nodes):
+    """Several entries over one sequence (the same slot more than once)."""
+    tree_check(kvc, lens=[300 - nodes[0], 20 - nodes[1] % 20, 7], nodes=nodes, seqs=[0, 0, 0], kt=kind, vt=kind, beta=True)
+
+
+@pytest.mark.parametrize("kind", [R.F32, R.F16, R.Q8_0])
+@pytest.mark.parametrize("nodes", [6, 40])
+def test_tree_shorter_than_its_nodes(kvc, kind, nodes):
+    """A sequence with fewer rows than the entry has nodes: the rows belong to the last nodes."""
+    tree_check(kvc, lens=[3 - nodes, 50], nodes=[nodes, 2], kt=kind, vt=kind, qt=torch.float32, beta=True)
+
+
+@pytest.mark.parametrize("kind", [R.F32, R.F16, R.Q8_0])
+@pytest.mark.parametrize("qt", [torch.float16, torch.float32])
+@pytest.mark.parametrize("nodes", [[1, 3], [40, 3]])
+def test_tree_a_bad_query_spoils_its_own_rows(kvc, kind, qt, nodes):
+    for bad in (math.nan, math.inf):
+        c, q, t, (out, lse) = tree_case(kvc, lens=[90, 33], nodes=nodes, kt=kind, vt=kind, qt=qt, beta=True)
+        q[1, 5] = bad
+        t.run()
+        torch.cuda.synchronize()
+        ok = torch.ones(q.shape[:2], dtype=torch.bool, device="cuda")
+        ok[1, 5] = False
+        used = torch.cat([c.rows(0), c.rows(1)])
+        K, V = (R.decode(x[0][used], kind) for x in (c.K, c.V))
+        good = torch.where(ok[..., None], q, torch.zeros_like(q))
+        o_tol, l_tol = bounds(good, K.view(-1, c.hkv, c.dk), V, float(c.beta.abs().max()), kind, qt == torch.float16, c.dk ** -0.5)
+        check(t.out[ok], out[ok], o_tol, "out")
+        check(t.lse[ok], lse[ok], l_tol, "lse")
+
+
+@pytest.mark.parametrize("kt,vt", [(R.Q8_0, R.Q8_0), (R.Q4_0, R.Q8_0), (R.Q4_1, R.Q4_0)])
+@pytest.mark.parametrize("nodes", [[1, 2], [40, 2]])
+def test_tree_rows_of_odd_blocks(kvc, kt, vt, nodes):
+    """Rows whose size is no multiple of four bytes."""
+    for hkv in (1, 3):
+        tree_check(kvc, lens=[90, 20], nodes=nodes, hkv=hkv, dk=32, dv=32, kt=kt, vt=vt, qt=torch.float32, page=7, beta=True)
+
+
+@pytest.mark.parametrize("kind", [R.F32, R.F16, R.Q4_0])
+def test_tree_more_heads_than_workers(kvc, kind):
+    tree_check(kvc, lens=[70, 0], nodes=[1, 0], hkv=320, g=1, dk=32, dv=32, kt=kind, vt=kind)
+    tree_check(kvc, lens=[70, 0], nodes=[40, 0], hkv=160, g=1, dk=32, dv=32, kt=kind, vt=kind)
+
+
+def test_tree_calls_side_by_side(kvc):
+    """Two calls over one cache on two streams, each with its own workspace; a graph next to them."""
+    c, q, t, (out, _) = tree_case(kvc, lens=[5000, 300], nodes=[2, 40], qt=torch.float32, hkv=4)
+    t.run()
+    torch.cuda.synchronize()
+    want = t.out.clone()
+    dev = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    calls = [attn.Tree(kvc, c.handle(kvc), q, dev([0, 2, 42]), dev([0, 1]), mask=t._keep[3], max_nodes=40, scale=64 ** -0.5)
+             for _ in range(3)]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        calls[2].run()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for s, u in zip(streams, calls):
+            with torch.cuda.stream(s):
+                u.run()
+        g.replay()
+    torch.cuda.synchronize()
+    for u in calls:
+        assert torch.equal(u.out, want)
+
+
+@pytest.mark.parametrize("kind,page,nodes", [(R.F16, 16, [1, 2]), (R.F16, 16, [40, 2]), (R.F16, 5, [1, 2]), (R.F32, 16, [1, 2])])
+def test_tree_far_rows(kvc, kind, page, nodes):
+    """Pages more than 4 GiB into the pool."""
+    c, q, t, (out, lse) = tree_case(kvc, lens=[200, 33], nodes=nodes, hkv=8, dk=128, dv=128, kt=kind, vt=kind, page=page,
+                                    qt=torch.float32)
+    t.run()
+    torch.cuda.synchronize()
+    rb, rows = c.K.shape[2], c.K.shape[1]
+    far = (-(-(2 ** 32 + 2 ** 20) // rb) // page + 1) * page
+    K, V = (torch.empty(1, far + rows, rb, dtype=torch.uint8, device="cuda") for _ in range(2))
+    K[:, far:], V[:, far:] = c.K, c.V
+    c.K, c.V = K, V
+    c.table[c.table >= 0] += far // page
+    c.ref = torch.zeros((far + rows) // page, dtype=torch.int32, device="cuda")
+    u = attn.Tree(kvc, c.handle(kvc), q, t._keep[1], t._keep[2], mask=t._keep[3], max_nodes=max(nodes), scale=128 ** -0.5)
+    u.run()
+    torch.cuda.synchronize()
+    assert torch.equal(u.out, t.out) and torch.equal(u.lse, t.lse)
+    assert float((u.out.double() - out).abs().max()) < 1e-4
+
+
 # ---- prompts ------------------------------------------------------------------------------
 
 def prompt_case(new, past, hkv=2, g=4, dk=64, dv=64, dtype=torch.float16, causal=True, seed=0, wide=False, scale=None, edit=None):
@@ -616,6 +708,48 @@ def test_prompt_on_a_stream_and_in_a_graph(kvc):
     g.replay()
     torch.cuda.synchronize()
     assert torch.equal(p.out, want) and float((want.double() - out).abs().max()) < 2 * 2.0 ** -11 * 5
+
+
+@pytest.mark.parametrize("n,d", [(300, 64), (70, 24)])
+def test_prompt_far_rows(kvc, n, d):
+    """Strides that put the last rows more than 2^31 elements behind the first."""
+    wide = torch.empty(n, 2 ** 31 // n // 8 * 8 + 4096, dtype=torch.float16, device="cuda")
+    gen = torch.Generator().manual_seed(n)
+    q, k, v = (wide[:, i * 8 * d:i * 8 * d + h * d].unflatten(1, (h, d)) for i, h in ((0, 8), (1, 2), (2, 2)))
+    for x in (q, k, v):
+        x.copy_(torch.randn(x.shape, generator=gen))
+    cu = torch.tensor([0, n // 2, n], dtype=torch.int32, device="cuda")
+    far, near = attn.Prompt(kvc, q, k, v, cu), attn.Prompt(kvc, q.contiguous(), k.contiguous(), v.contiguous(), cu)
+    far.run()
+    near.run()
+    torch.cuda.synchronize()
+    assert torch.equal(far.out, near.out) and bool(torch.isfinite(far.out).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_prompt_a_bad_query_spoils_its_own_rows(kvc, dtype):
+    q, k, v, cu_q, cu_k, scale, out, lse = prompt_case([140, 20], [3, 0], dk=128, dv=128, dtype=dtype)
+    q[77, 3] = math.nan
+    p = attn.Prompt(kvc, q, k, v, cu_q, cu_k, scale=scale)
+    p.run()
+    torch.cuda.synchronize()
+    ok = torch.ones(q.shape[:2], dtype=torch.bool, device="cuda")
+    ok[77, 3] = False
+    q = torch.where(ok[..., None], q, torch.zeros_like(q))
+    o_tol, l_tol = bounds(q, k.double(), v.double(), 0.0, R.F16, dtype == torch.float16, scale)
+    check(p.out[ok], out[ok], o_tol, "out")
+    check(p.lse[ok], lse[ok], l_tol, "lse")
+
+
+def test_prompt_shared_heads_by_stride(kvc):
+    """Keys and values expanded over the KV heads (a head stride of 0)."""
+    q, k, v, cu_q, cu_k, scale, out, lse = prompt_case([90, 9], [0, 0], hkv=1, g=4)
+    p = attn.Prompt(kvc, q, k.expand(-1, 4, -1), v.expand(-1, 4, -1), cu_q, cu_k, scale=scale)
+    p.run()
+    torch.cuda.synchronize()
+    o_tol, l_tol = bounds(q, k.double(), v.double(), 0.0, R.F16, True, scale)
+    check(p.out, out, o_tol, "out")
+    check(p.lse, lse, l_tol, "lse")
 
 
 def test_wrappers_check_their_tensors(kvc):
