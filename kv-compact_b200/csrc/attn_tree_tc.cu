@@ -23,6 +23,12 @@
 //                    is put into the swizzled tiles
 //   warp 12          MMA issue (one thread); 13-15 idle (register shares go by
 //                    warp group)
+//
+// Bound by latency inside a CTA: two softmax warps per scheduler, whose chain per
+// tile (scores, maximum, exponentials, P, sums) the other stream half hides, and
+// for block codes the conversion. Trees of 16 to 60 nodes on 26,122 F16 keys (8
+// heads of 4 query heads, 128 values) 122 us, 0.9 TB/s of rows; 25 nodes on
+// 30,000 Q4_0 / Q4_1 keys (4 heads of 8, 64 values, F32 queries) 90 us.
 #include "attn.h"
 #include "attn_tc.h"
 #include "attn_tree.h"
