@@ -6,8 +6,7 @@
 //   x_ij = scale q_i.k_j (+ beta_j),  m = max_j x_ij,  l = sum_j exp(x_ij - m),
 //   out_i = (sum_j exp(x_ij - m) v_j) / l,  lse_i = m + log l
 //
-// in one pass over the keys with a running m, l and sum. 160,000 Q8_0 keys of 8
-// heads, 4 query rows each, 128 values: 1.41 ms here, 0.14 ms in k_tree_mma.
+// in one pass over the keys with a running m, l and sum.
 #include "attn.h"
 #include "attn_tc.h"
 
@@ -19,20 +18,72 @@ constexpr int RB = 8, TILE = 128;        // query rows and keys per CTA and step
 constexpr int WARPS = 4, THREADS = 32 * WARPS, WK = 32;
 static_assert(TILE == WARPS * WK, "a tile is one key per lane");
 
+// A shared-memory row of `d` values: whole float4s, an odd number of them, so that 8 lanes reading 8 rows hit all banks.
+__host__ __device__ constexpr int simt_pitch(int d) { return 4 * (((d + 3) / 4) | 1); }
+
+// 32 stored rows (this lane's is `row`; only those in `live` are read, the others become zeros) as fp32 into a warp's
+// shared memory, d values each and zeros up to whole float4s. `direct`: fp32 rows on 16-byte boundaries, whose copies are
+// all in flight at once; else 8 rows' elements at a time.
+__device__ __forceinline__ void simt_load(float * buf, int pitch, const uint8_t * base, long long rb, int type, int d,
+                                          long long row, unsigned live, bool direct, int lane) {
+    const int d4 = (d + 3) & ~3;
+    if (direct) {
+        for (int k = 0; k < WK; k++) {
+            const long long rk = __shfl_sync(~0u, row, k);
+            const float * p = reinterpret_cast<const float *>(base + ((live >> k) & 1u ? rk : 0) * rb);
+            for (int e = 4 * lane; e < d; e += 128) {
+                if ((live >> k) & 1u)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                                 :: "r"((uint32_t)__cvta_generic_to_shared(buf + k * pitch + e)), "l"(p + e) : "memory");
+                else
+                    *reinterpret_cast<float4 *>(buf + k * pitch + e) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        return;
+    }
+    for (int k0 = 0; k0 < WK; k0 += 8) {
+        if (!((live >> k0) & 0xFFu)) {
+            for (int e = lane; e < 8 * d4; e += 32) buf[(k0 + e / d4) * pitch + e % d4] = 0.0f;
+            continue;
+        }
+        long long at[8];
+#pragma unroll
+        for (int u = 0; u < 8; u++) at[u] = __shfl_sync(~0u, row, k0 + u) * rb;
+        for (int e = lane; e < d4; e += 32) {
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) v[u] = e < d && ((live >> (k0 + u)) & 1u) ? attn_elem(base + at[u], type, e) : 0.0f;
+#pragma unroll
+            for (int u = 0; u < 8; u++) buf[(k0 + u) * pitch + e] = v[u];
+        }
+    }
+}
+
 // One CTA: 8 query rows of one KV head against its stretch of the keys. A
-// warp takes 32 keys of a tile, decodes their K rows into its own shared
-// memory, scores one key per lane, then does the same with V with one output
-// dimension per lane: no barrier inside the loop. Bound by the shared-memory
-// reads of the two products (9 words per 8 multiply-adds).
+// warp takes 32 keys of a tile, brings their K rows as fp32 into its own shared
+// memory, scores one key per lane, then does the same with V with up to 4
+// neighbouring output dimensions per lane (8 in two runs): no barrier inside
+// the loop. All shared-memory reads are of four values, 12 wavefronts for the
+// 32 multiply-adds that a lane makes with them. Bound by a warp's wait for its
+// rows (12 warps per SM at 128 values): 43,000 F32 keys of 8 heads, 4 query rows
+// each, 128 values, 162 us (2.2 TB/s of rows); rows brought one by one and single
+// values read from shared memory: 432 us.
 template <int DV_LANES>
 __global__ void __launch_bounds__(THREADS) k_attn_simt(const __grid_constant__ kvc_attn_args a) {
-    extern __shared__ float sm[];
-    const int pitch = max(a.dk, a.dv) | 1;               // odd: a column read hits 32 banks
+    extern __shared__ __align__(16) float sm[];
+    constexpr int VEC = DV_LANES < 4 ? DV_LANES : 4;     // neighbouring output dimensions of a lane
+    const int pitch = simt_pitch(max(a.dk, a.dv)), dk4 = (a.dk + 3) & ~3;
+    // fp32 rows that can be copied 16 bytes at a time
+    auto aligned = [](const uint8_t * p, long long rb, long long hb, int type, int d) {
+        return type == KV_TYPE_F32 && (((uintptr_t)p | (uintptr_t)rb | (uintptr_t)hb) & 15) == 0 && d % 4 == 0;
+    };
+    const bool k_direct = aligned(a.K, a.k_rb, a.k_hb, a.k_type, a.dk), v_direct = aligned(a.V, a.v_rb, a.v_hb, a.v_type, a.dv);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     float * qs = sm;                                     // [RB][dk]
-    float * ps = qs + RB * a.dk + warp * (RB * WK);      // [RB][32] of this warp
-    float * buf = qs + RB * a.dk + WARPS * RB * WK + (size_t)warp * WK * pitch;
-    float * joinO = qs + RB * a.dk + WARPS * RB * WK;    // reused after the loop: [WARPS][RB][dv] (dv <= pitch, RB <= 32)
+    float * ps = qs + RB * dk4 + warp * (RB * WK);       // [32][RB] of this warp
+    float * buf = qs + RB * dk4 + WARPS * RB * WK + (size_t)warp * WK * pitch;
+    float * joinO = qs + RB * dk4 + WARPS * RB * WK;    // reused after the loop: [WARPS][RB][dv] (dv <= pitch, RB <= 32)
     __shared__ float s_m[WARPS][RB], s_l[WARPS][RB];
     const int h = blockIdx.y % a.Hkv, w = blockIdx.x;
     const int n_blocks = (int)(((long long)a.max_q * a.g + RB - 1) / RB);
@@ -42,10 +93,10 @@ __global__ void __launch_bounds__(THREADS) k_attn_simt(const __grid_constant__ k
         const int r0 = qb * RB;
         const int nr = (int)min((long long)RB, (long long)q.nq * a.g - r0);
         __syncthreads();
-        for (int e = threadIdx.x; e < RB * a.dk; e += THREADS) {
-            const int r = e / a.dk, d = e - r * a.dk;
+        for (int e = threadIdx.x; e < RB * dk4; e += THREADS) {
+            const int r = e / dk4, d = e - r * dk4;
             float v = 0.0f;
-            if (r < nr) {
+            if (r < nr && d < a.dk) {
                 const int i = (int)a.by_group.div(r0 + r);
                 const long long at = (long long)(q.q0 + i) * a.q_stride + (long long)(h * a.g + (r0 + r - i * a.g)) * a.q_head + d;
                 v = a.q_type == KV_TYPE_F16 ? __half2float(reinterpret_cast<const __half *>(a.q)[at])
@@ -78,31 +129,27 @@ __global__ void __launch_bounds__(THREADS) k_attn_simt(const __grid_constant__ k
             const bool there = row >= 0 && bias != -INFINITY;
             const unsigned live = __ballot_sync(~0u, there);
             if (!live) continue;
-            for (int k = 0; k < WK; k++) {
-                const long long rk = __shfl_sync(~0u, row, k);
-                const bool ok = (live >> k) & 1u;
-                const uint8_t * p = a.K + (ok ? rk : 0) * a.k_rb + (long long)h * a.k_hb;
-                for (int d = lane; d < a.dk; d += 32) buf[k * pitch + d] = ok ? attn_elem(p, a.k_type, d) : 0.0f;
-            }
+            simt_load(buf, pitch, a.K + (long long)h * a.k_hb, a.k_rb, a.k_type, a.dk, row, live, k_direct, lane);
             __syncwarp();
             float x[RB];
 #pragma unroll
             for (int r = 0; r < RB; r++) x[r] = 0.0f;
-            for (int d = 0; d < a.dk; d++) {
-                const float kv = buf[lane * pitch + d];
+#pragma unroll 4
+            for (int d = 0; d < dk4; d += 4) {
+                const float4 kv = *reinterpret_cast<const float4 *>(buf + lane * pitch + d);
 #pragma unroll
-                for (int r = 0; r < RB; r++) x[r] = fmaf(qs[r * a.dk + d], kv, x[r]);
+                for (int r = 0; r < RB; r++) {
+                    const float4 qv = *reinterpret_cast<const float4 *>(qs + r * dk4 + d);
+                    x[r] = fmaf(qv.w, kv.w, fmaf(qv.z, kv.z, fmaf(qv.y, kv.y, fmaf(qv.x, kv.x, x[r]))));
+                }
             }
             __syncwarp();
-            for (int k = 0; k < WK; k++) {
-                const long long rk = __shfl_sync(~0u, row, k);
-                const bool ok = (live >> k) & 1u;
-                const uint8_t * p = a.V + (ok ? rk : 0) * a.v_rb + (long long)h * a.v_hb;
-                for (int d = lane; d < a.dv; d += 32) buf[k * pitch + d] = ok ? attn_elem(p, a.v_type, d) : 0.0f;
-            }
+            simt_load(buf, pitch, a.V + (long long)h * a.v_hb, a.v_rb, a.v_type, a.dv, row, live, v_direct, lane);
+            bool some = false;                           // a key that some rows see and others do not
 #pragma unroll
             for (int r = 0; r < RB; r++) {
                 const bool sees = there && r < nr && attn_sees(a, q, (int)a.by_group.div(r0 + r), j);
+                some |= there && r < nr && !sees;
                 const float xr = sees ? fmaf(x[r], a.scale, bias) : -INFINITY;
                 float mt = xr;
 #pragma unroll
@@ -115,20 +162,50 @@ __global__ void __launch_bounds__(THREADS) k_attn_simt(const __grid_constant__ k
                 l[r] = l[r] * f + p;                     // per lane; summed over the lanes at the end
 #pragma unroll
                 for (int c = 0; c < DV_LANES; c++) o[r][c] *= f;
-                ps[r * WK + lane] = p;
+                ps[lane * RB + r] = p;
             }
+            some = __any_sync(~0u, some);
             __syncwarp();
+#pragma unroll 2
             for (int k = 0; k < WK; k++) {
-                float v[DV_LANES];
+                float v[DV_LANES], p[RB];
 #pragma unroll
-                for (int c = 0; c < DV_LANES; c++) v[c] = lane + 32 * c < a.dv ? buf[k * pitch + lane + 32 * c] : 0.0f;
-#pragma unroll
-                for (int r = 0; r < RB; r++) {
-                    const float p = ps[r * WK + k];
-                    if (p != 0.0f) {                     // a hidden row's V may be anything
-#pragma unroll
-                        for (int c = 0; c < DV_LANES; c++) o[r][c] = fmaf(p, v[c], o[r][c]);
+                for (int c = 0; c < DV_LANES; c += VEC) {
+                    const int d = VEC * lane + 32 * c;
+                    const float * at = buf + k * pitch + d;
+                    const bool in = d < a.dv;
+                    if (VEC == 4) {
+                        const float4 w4 = in ? *reinterpret_cast<const float4 *>(at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        v[c] = w4.x;
+                        v[c + 1] = w4.y;
+                        v[c + VEC - 2] = w4.z;
+                        v[c + VEC - 1] = w4.w;
+                    } else {
+                        const float2 w2 = in ? *reinterpret_cast<const float2 *>(at) : make_float2(0.0f, 0.0f);
+                        v[c] = w2.x;
+                        v[c + 1] = w2.y;
                     }
+                }
+#pragma unroll
+                for (int r = 0; r < RB; r += 4) {
+                    const float4 p4 = *reinterpret_cast<const float4 *>(ps + k * RB + r);
+                    p[r] = p4.x;
+                    p[r + 1] = p4.y;
+                    p[r + 2] = p4.z;
+                    p[r + 3] = p4.w;
+                }
+                if (some) {                              // what a row does not see may be anything
+#pragma unroll
+                    for (int r = 0; r < RB; r++)
+                        if (p[r] != 0.0f) {
+#pragma unroll
+                            for (int c = 0; c < DV_LANES; c++) o[r][c] = fmaf(p[r], v[c], o[r][c]);
+                        }
+                } else {
+#pragma unroll
+                    for (int r = 0; r < RB; r++)
+#pragma unroll
+                        for (int c = 0; c < DV_LANES; c++) o[r][c] = fmaf(p[r], v[c], o[r][c]);
                 }
             }
             __syncwarp();
@@ -146,8 +223,10 @@ __global__ void __launch_bounds__(THREADS) k_attn_simt(const __grid_constant__ k
                 s_l[warp][r] = l[r];
             }
 #pragma unroll
-            for (int c = 0; c < DV_LANES; c++)
-                if (lane + 32 * c < a.dv) joinO[((size_t)warp * RB + r) * a.dv + lane + 32 * c] = o[r][c];
+            for (int c = 0; c < DV_LANES; c++) {
+                const int d = VEC * lane + 32 * (c & ~(VEC - 1)) + (c & (VEC - 1));
+                if (d < a.dv) joinO[((size_t)warp * RB + r) * a.dv + d] = o[r][c];
+            }
         }
         __syncthreads();
         float * part = slot >= 0 ? attn_part(a, qb, h, w, slot) : nullptr;
@@ -302,8 +381,8 @@ __global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ kvc_a
 }
 
 size_t simt_smem(int dk, int dv) {
-    const int pitch = (dk > dv ? dk : dv) | 1;
-    return (size_t)(RB * dk + WARPS * RB * WK + WARPS * WK * pitch) * sizeof(float);
+    const int pitch = simt_pitch(dk > dv ? dk : dv);
+    return (size_t)(RB * ((dk + 3) & ~3) + WARPS * RB * WK + WARPS * WK * pitch) * sizeof(float);
 }
 
 template <int C>
