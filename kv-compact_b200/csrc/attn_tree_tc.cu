@@ -280,25 +280,48 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
             const int qb = S.qb, r0 = qb * TM;
             const int rows_here = (int)min((long long)TM, (long long)S.nq * a.g - r0);
             {
-                // Q: two threads per row
-                const bool q_pairs = (reinterpret_cast<uintptr_t>(a.q) & (QP == 2 ? 7 : 3)) == 0 && (a.q_stride & 1) == 0;
+                // Q: two threads per row, in 16-byte pieces where they are aligned, all of them on their way at once
+                constexpr int SIZE = QP == 2 ? 4 : 2, PIECES = D / 2 * SIZE / 16;
+                const bool whole = ((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)(a.q_stride * SIZE)) & 15) == 0;
                 const int row = threadIdx.x >> 1, part = threadIdx.x & 1;
                 const int i = (int)a.by_group.div(r0 + row);
                 const long long at = (long long)(S.q0 + i) * a.q_stride + (long long)(h * a.g + (r0 + row - i * a.g)) * a.q_head;
-                // this thread's half of the row, pairs of values; read at once, so that the latencies overlap
+                const uint8_t * src = reinterpret_cast<const uint8_t *>(a.q) + (at + part * (D / 2)) * SIZE;
+                const int values = row < rows_here ? a.dk - part * (D / 2) : 0;      // of this thread's half
+                uint4 raw[PIECES];
+                if (whole) {
+#pragma unroll
+                    for (int k = 0; k < PIECES; k++)
+                        raw[k] = 16 / SIZE * k < values ? *reinterpret_cast<const uint4 *>(src + 16 * k) : make_uint4(0, 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < PIECES; k++) {
+                        uint32_t x[4] = {0, 0, 0, 0};
+                        if (16 / SIZE * k < values) {
+#pragma unroll
+                            for (int u = 0; u < 4; u++) {
+                                const uint8_t * p = src + 16 * k + 4 * u;
+                                if (QP == 2) x[u] = *reinterpret_cast<const uint32_t *>(p);
+                                else x[u] = *reinterpret_cast<const uint16_t *>(p) | (uint32_t)*reinterpret_cast<const uint16_t *>(p + 2) << 16;
+                            }
+                        }
+                        raw[k] = make_uint4(x[0], x[1], x[2], x[3]);
+                    }
+                }
                 float2 v[D / 4];
 #pragma unroll
-                for (int k = 0; k < D / 4; k++) {
-                    const int d = part * (D / 2) + 2 * k;
-                    v[k] = make_float2(0.0f, 0.0f);
-                    if (row < rows_here && d < a.dk) {
+                for (int k = 0; k < PIECES; k++) {
+                    const uint32_t x[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
                         if (QP == 2) {
-                            const float * p = reinterpret_cast<const float *>(a.q) + at + d;
-                            v[k] = q_pairs ? *reinterpret_cast<const float2 *>(p) : make_float2(p[0], p[1]);
+                            float2 & y = v[2 * k + u / 2];
+                            if (u & 1) y.y = __uint_as_float(x[u]);
+                            else y.x = __uint_as_float(x[u]);
                         } else {
-                            const __half * p = reinterpret_cast<const __half *>(a.q) + at + d;
-                            v[k] = q_pairs ? __half22float2(*reinterpret_cast<const __half2 *>(p))
-                                           : make_float2(__half2float(p[0]), __half2float(p[1]));
+                            __half2 hh;
+                            memcpy(&hh, &x[u], 4);
+                            v[(4 * k + u) % (D / 4)] = __half22float2(hh);
                         }
                     }
                 }
@@ -337,7 +360,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                 }
                 fence_smem_to_async();
             }
-            __syncthreads();                             // Q is there
+            group_sync(4, 288);                          // Q is there: these warps and the one that issues the products
             const float mul = QP == 2 ? X.mul[r] : 1.0f;
             const bool real = r < rows_here;
             const int node = (int)a.by_group.div(r0 + r);
@@ -634,7 +657,6 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                 const uint32_t p = a.by_page.div((uint32_t)row);
                 return a.beta[((size_t)p * a.Hkv + h) * a.page + (row - (int)p * a.page)];
             };
-            __syncthreads();                             // (Q is there)
             if constexpr (KP == 1) {
                 const int chunk = tid & 7, first = tid >> 3;
                 int page = page_of(0);
@@ -659,7 +681,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                     row = place(i + 1, page);
                     bias = bias_of(row);
                     page = page_of(i + 2);
-                    group_sync(4, 128);
+                    group_sync(5, 128);
                     for (int side = 0; side < 2; side++) {
                         const int it = items + 2 * i + side;
                         await(X.empty + it % C::SLOTS, ((it / C::SLOTS) & 1) ^ 1);
@@ -792,8 +814,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
         reg_less<REG_MMA>();
         // ---- products
         each(kvc_int<0>{}, [&](const segment & S, int n) {
-            __syncthreads();                             // Q is there
             if (warp == 12) {
+                group_sync(4, 288);                      // Q is there
                 fence_after_sync();
                 constexpr uint32_t ID_S = (1u << 4) | ((uint32_t)(TN >> 3) << 17) | ((uint32_t)(TM >> 4) << 24);
                 constexpr uint32_t ID_O = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(TM >> 4) << 24);
