@@ -410,17 +410,23 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                     }
                 }
                 // x of columns c .. c+15 from v; `show`: the keys that count
-                auto scores = [&](auto masked, int c, unsigned long long show, const uint32_t v[16], float x[16]) {
+                auto scores = [&](auto masked, int c, unsigned long long show, const uint32_t v[16], float2 x[8]) {
 #pragma unroll
                     for (int k = 0; k < 16; k += 4) {
                         const float4 f = *reinterpret_cast<const float4 *>(&I.f[c + k]);
                         const float4 b = *reinterpret_cast<const float4 *>(&I.b[c + k]);
-                        const float fk[4] = {f.x, f.y, f.z, f.w}, bk[4] = {b.x, b.y, b.z, b.w};
+                        const float2 fk[2] = {make_float2(f.x, f.y), make_float2(f.z, f.w)};
+                        const float2 bk[2] = {make_float2(b.x, b.y), make_float2(b.z, b.w)};
 #pragma unroll
-                        for (int u = 0; u < 4; u++) {
-                            const float s = __uint_as_float(v[k + u]);
-                            x[k + u] = fmaf(QP == 2 ? s * mul : s, fk[u], bk[u]);      // hidden rows: S = 0 and beta = -inf
-                            if (decltype(masked)::value && !((show >> (c + k + u)) & 1)) x[k + u] = -INFINITY;
+                        for (int u = 0; u < 2; u++) {
+                            float2 s = make_float2(__uint_as_float(v[k + 2 * u]), __uint_as_float(v[k + 2 * u + 1]));
+                            if (QP == 2) s = mul2(s, make_float2(mul, mul));
+                            float2 & y = x[k / 2 + u];
+                            y = fma2(s, fk[u], bk[u]);   // hidden rows: S = 0 and beta = -inf
+                            if (decltype(masked)::value) {
+                                if (!((show >> (c + k + 2 * u)) & 1)) y.x = -INFINITY;
+                                if (!((show >> (c + k + 2 * u + 1)) & 1)) y.y = -INFINITY;
+                            }
                         }
                     }
                 };
@@ -434,11 +440,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                         tmem_wait_ld();
 #pragma unroll
                         for (int u = 0; u < 2; u++) {
-                            float x[16];
+                            float2 x[8];
                             scores(masked, c + 16 * u, vis, v[u], x);
 #pragma unroll
-                            for (int k = 0; k < 16; k += 4)
-                                top = fmaxf(fmaxf(top, fmaxf(x[k], x[k + 1])), fmaxf(x[k + 2], x[k + 3]));
+                            for (int k = 0; k < 8; k += 2)
+                                top = fmaxf(fmaxf(top, fmaxf(x[k].x, x[k].y)), fmaxf(x[k + 1].x, x[k + 1].y));
                         }
                     }
                 };
@@ -458,6 +464,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                 // no finite numbers, or far above the others', are added value by value
                 int R = HIDDEN;
                 float sum = 0.0f;
+                float2 sums = make_float2(0.0f, 0.0f);
                 if (KP == 2 || own) {
                     const int it = items + 2 * i + 1;    // the exponents are written with V
                     await(X.full + it % C::SLOTS, (it / C::SLOTS) & 1);
@@ -524,7 +531,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                     tmem_ld16_nowait(s_addr, v);
 #pragma unroll 1
                     for (int c = 0; c < TN; c += 16) {
-                        float x[16];
+                        float2 x[8];
                         tmem_wait_ld();
                         scores(masked, c, vis, v, x);
                         if (c + 16 < TN) tmem_ld16_nowait(s_addr + c + 16, v);     // under the exponentials
@@ -536,21 +543,22 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                         uint32_t p0[8], p1[8];
 #pragma unroll
                         for (int k = 0; k < 8; k++) {
-                            float p[2];
-#pragma unroll
-                            for (int u = 0; u < 2; u++) {
-                                const int q = 2 * k + u;
-                                p[u] = ex2((x[q] - base) * LOG2E);
-                                sum += p[u];
-                                const int ek = q % 4 == 0 ? e[q / 4].x : q % 4 == 1 ? e[q / 4].y : q % 4 == 2 ? e[q / 4].z : e[q / 4].w;
-                                p[u] *= KP == 2 ? __int_as_float(max(ek + up_bits, 0)) : (float)(1 << P_SHIFT);
+                            const float2 y = mul2(add2(x[k], make_float2(-base, -base)), make_float2(LOG2E, LOG2E));
+                            float2 p = make_float2(ex2(y.x), ex2(y.y));
+                            sums = add2(sums, p);
+                            float2 up = make_float2((float)(1 << P_SHIFT), (float)(1 << P_SHIFT));
+                            if (KP == 2) {
+                                const int4 & ek = e[k / 2];
+                                up.x = __int_as_float(max((k & 1 ? ek.z : ek.x) + up_bits, 0));
+                                up.y = __int_as_float(max((k & 1 ? ek.w : ek.y) + up_bits, 0));
                             }
-                            p0[k] = pack(p[0], p[1]);
+                            p = mul2(p, up);
+                            p0[k] = pack(p.x, p.y);
                             if (QP == 2) {
                                 __half2 hh;
                                 memcpy(&hh, &p0[k], 4);
-                                const float2 y = __half22float2(hh);
-                                p1[k] = pack(p[0] - y.x, p[1] - y.y);
+                                const float2 z = __half22float2(hh);
+                                p1[k] = pack(p.x - z.x, p.y - z.y);
                             }
                         }
                         st8(p_addr + c / 2, p0);
@@ -559,7 +567,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                 };
                 if (own) probabilities(kvc_int<1>{});
                 else probabilities(kvc_int<0>{});
-                l += sum;
+                l += sum + (sums.x + sums.y);
                 tmem_wait_st();
                 fence_before_sync();
                 __syncwarp();
