@@ -53,6 +53,7 @@ struct kvc_attn_seq {
     int q0, nq;             // rows of q
     int ln;                 // keys
     int k0;                 // packed: first key row
+    int slot;               // paged: its slot, or -1
     const int * table;      // paged: its table row
 };
 
@@ -62,6 +63,7 @@ __device__ __forceinline__ kvc_attn_seq attn_seq(const kvc_attn_args & a, int s)
     r.nq = min(min(max(a.cu_q[s + 1], r.q0), a.n_total) - r.q0, a.max_q);
     r.k0 = 0;
     r.ln = 0;
+    r.slot = -1;
     r.table = nullptr;
     if (a.cu_k) {
         r.k0 = min(max(a.cu_k[s], 0), a.n_keys);
@@ -69,6 +71,7 @@ __device__ __forceinline__ kvc_attn_seq attn_seq(const kvc_attn_args & a, int s)
     } else {
         const int slot = a.seqs[s];
         if (slot >= 0 && slot < a.n_slots) {
+            r.slot = slot;
             r.table = a.table + (size_t)slot * a.max_pages;
             r.ln = min(max(a.seq_len[slot], 0), a.max_pages * a.page);
         }
@@ -106,9 +109,13 @@ __device__ __forceinline__ bool attn_sees(const kvc_attn_args & a, const kvc_att
 // their partial results go to those slots and are joined afterwards, in the
 // workers' order.
 
+// x / d of numbers >= 0, most of them below 2^31 (a 64-bit division takes several times as long).
+__device__ __forceinline__ long long attn_quotient(long long x, long long d) {
+    return ((x | d) >> 31) == 0 ? (long long)((uint32_t)x / (uint32_t)d) : x / d;
+}
 // Worker that holds tile x of T.
 __device__ __forceinline__ int attn_worker(long long x, long long T, int W) {
-    return (int)(((x + 1) * W - 1) / T);
+    return (int)attn_quotient((x + 1) * W - 1, T);
 }
 
 // fn(qb, q, lo, hi, slot) for every piece of worker w's stretch: tiles lo..hi-1
@@ -140,7 +147,7 @@ __device__ __forceinline__ void attn_walk(const kvc_attn_args & a, int qb0, int 
     for (int o = 16; o; o >>= 1) T += __shfl_xor_sync(~0u, T, o);
     const int W = (int)min((long long)a.W, T);           // every worker has a tile
     if (w >= W) return;
-    const long long from = w * T / W, to = (w + 1) * T / W;
+    const long long from = attn_quotient(w * T, W), to = attn_quotient((w + 1) * T, W);
     long long at = 0;
     for (int qb = qb0; qb < qb1 && at < to; qb++)
         for (int s0 = 0; s0 < a.n_seqs && at < to; s0 += 32) {
@@ -176,7 +183,8 @@ __device__ __forceinline__ void attn_walk(const kvc_attn_args & a, int qb0, int 
                 q.nq = __shfl_sync(~0u, mine.nq, l);
                 q.ln = __shfl_sync(~0u, mine.ln, l);
                 q.k0 = __shfl_sync(~0u, mine.k0, l);
-                q.table = reinterpret_cast<const int *>(__shfl_sync(~0u, (unsigned long long)mine.table, l));
+                q.slot = __shfl_sync(~0u, mine.slot, l);
+                q.table = q.slot < 0 ? nullptr : a.table + (size_t)q.slot * a.max_pages;
                 fn(qb, q, lo, hi, lo == 0 && hi == ts ? -1 : (from > ps ? 0 : 1));
             }
             at += end;

@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
             int n = 0;
             attn_walk(a, qb, qb + 1, w, hg == 0, [&](int, const kvc_attn_seq & q, int lo, int hi, int slot) {
                 if (n >= batch && n < batch + MAX_SEGS && lane == 0) {
-                    segs[n - batch] = segment{lo, hi, slot, q.q0, q.nq, q.ln, (int)((q.table - a.table) / a.max_pages)};
+                    segs[n - batch] = segment{lo, hi, slot, q.q0, q.nq, q.ln, q.slot};
                 }
                 n++;
             });

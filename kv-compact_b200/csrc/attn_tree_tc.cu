@@ -24,11 +24,14 @@
 //   warp 12          MMA issue (one thread); 13-15 idle (register shares go by
 //                    warp group)
 //
-// Bound by latency inside a CTA: two softmax warps per scheduler, whose chain per
-// tile (scores, maximum, exponentials, P, sums) the other stream half hides, and
-// for block codes the conversion. Trees of 16 to 60 nodes on 26,122 F16 keys (8
-// heads of 4 query heads, 128 values) 122 us, 0.9 TB/s of rows; 25 nodes on
-// 30,000 Q4_0 / Q4_1 keys (4 heads of 8, 64 values, F32 queries) 90 us.
+// Bound by latency inside a CTA: a stream's chain per tile (scores, maximum,
+// exponentials, P, product, sums) takes about 6,000 cycles at 128 values with two
+// softmax warps per scheduler, which the other stream half hides; and about 15 us
+// per call go to the segments, the queries, the first tile and the join. Trees of
+// 16 to 60 nodes on 26,122 F16 keys (8 heads of 4 query heads, 128 values) 104 us,
+// 1.0 TB/s of rows; 25 nodes on 30,000 Q4_0 / Q4_1 keys (4 heads of 8, 64 values,
+// F32 queries) 83 us. Queries read pair by pair before the first tile was asked
+// for: 122 and 90 us.
 #include "attn.h"
 #include "attn_tc.h"
 #include "attn_tree.h"
@@ -246,7 +249,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                 int n = 0;
                 attn_walk(a, 0, n_blocks, w, h == 0, [&](int qb, const kvc_attn_seq & q, int lo, int hi, int slot) {
                     if (n >= batch && n < batch + MAX_SEGS && lane == 0)
-                        X.segs[n - batch] = segment{lo, hi, slot, qb, q.q0, q.nq, q.ln, (int)((q.table - a.table) / a.max_pages)};
+                        X.segs[n - batch] = segment{lo, hi, slot, qb, q.q0, q.nq, q.ln, q.slot};
                     n++;
                 });
                 if (lane == 0) {
