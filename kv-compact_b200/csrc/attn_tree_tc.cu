@@ -932,11 +932,13 @@ bool kvc_attn_tree_tc_plan(kvc_attn_args * a, int sms, long long * blocks) {
     // kernel's hardly does up to 128 rows, but putting two fp16 pieces of 128
     // values into the tiles costs it most. 43,000 keys x 8 heads, us here / there:
     //   rows                 32         36         64         80
-    //   F16, d 64         73 / 72    73 / 99   77 / 105   78 / 171
-    //   Q8_0, d 64       106 / 71  107 / 108  112 / 113  111 / 206
-    //   F16, d 128      103 / 104  103 / 144  108 / 156  109 / 229
-    //   Q8_0, d 128     222 / 117  222 / 164  227 / 175  226 / 297
-    //   Q4_0, d 128     178 / 97   180 / 148  189 / 156  190 / 286
+    //   F16, d 64         65 / 71    65 / 99   68 / 105   69 / 172
+    //   Q8_0, d 64       103 / 71  103 / 109  107 / 113  105 / 207
+    //   F16, d 128       94 / 104   93 / 143   98 / 156  100 / 229
+    //   Q8_0, d 128     208 / 117  208 / 165  211 / 175  211 / 296
+    //   Q4_0, d 128     167 / 97   167 / 148  171 / 157  170 / 286
+    // (F16 with 32 rows stays there: on short caches this kernel takes 25 us at
+    // least, that one 19.)
     const long long few = a->k_type != KV_TYPE_F16 && top > 64 ? 64 : 32;
     if (rows <= few || top > 128 || a->dk % 32 || a->dv % 32) return false;
     if (a->k_type == KV_TYPE_F16 && a->v_type == KV_TYPE_F16) {
