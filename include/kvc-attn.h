@@ -68,8 +68,9 @@ int kvc_attn_prompt(const kvc_prompt_desc * desc, void * stream);
  * sequence is a tree of one node. Row r of the cache adds beta (when the cache
  * has it) to its scaled score; beta = -inf hides the row from the head's
  * queries. An entry whose sequence id lies outside the cache sees no key. max_nodes
- * is the most nodes of any entry; entries with more are cut to it (the rows
- * of the nodes behind are left as they were). */
+ * is the most nodes of any entry; of entries with more the first max_nodes are
+ * computed, as they would be beside the others, whose own rows count as theirs
+ * (the output rows of the nodes behind are left as they were). */
 typedef struct kvc_tree_desc {
     const void *     q;          /* [total x n_head x d_k], rows q_stride elements apart */
     void *           out;        /* [total x n_head x d_v] dense, of q's type */

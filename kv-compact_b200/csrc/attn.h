@@ -51,6 +51,7 @@ struct kvc_attn_args {
 // One sequence of a batch.
 struct kvc_attn_seq {
     int q0, nq;             // rows of q
+    int nodes;              // paged: nodes of the entry, of which nq are computed (fewer where max_q cuts them)
     int ln;                 // keys
     int k0;                 // packed: first key row
     int slot;               // paged: its slot, or -1
@@ -60,7 +61,8 @@ struct kvc_attn_seq {
 __device__ __forceinline__ kvc_attn_seq attn_seq(const kvc_attn_args & a, int s) {
     kvc_attn_seq r;
     r.q0 = min(max(a.cu_q[s], 0), a.n_total);
-    r.nq = min(min(max(a.cu_q[s + 1], r.q0), a.n_total) - r.q0, a.max_q);
+    r.nodes = max(a.cu_q[s + 1], r.q0) - r.q0;
+    r.nq = min(min(r.nodes, a.n_total - r.q0), a.max_q);
     r.k0 = 0;
     r.ln = 0;
     r.slot = -1;
@@ -91,10 +93,11 @@ __device__ __forceinline__ long long attn_row(const kvc_attn_args & a, const kvc
     return (long long)p * a.page + *off;
 }
 
-// Whether node / query i of a sequence sees key j (j < ln).
+// Whether node / query i of a sequence sees key j (j < ln). The last rows of a paged sequence are its entry's nodes' own,
+// those of nodes that are not computed among them.
 __device__ __forceinline__ bool attn_sees(const kvc_attn_args & a, const kvc_attn_seq & q, int i, int j) {
     if (a.cu_k) return !a.causal || j <= i + (q.ln - q.nq);
-    const int b = j - (q.ln - q.nq);
+    const int b = j - (q.ln - q.nodes);
     if (b < 0 || !a.mask) return true;
     return (b >> 5) < a.mask_words && ((a.mask[(size_t)(q.q0 + i) * a.mask_words + (b >> 5)] >> (b & 31)) & 1u);
 }
@@ -181,6 +184,7 @@ __device__ __forceinline__ void attn_walk(const kvc_attn_args & a, int qb0, int 
                 kvc_attn_seq q;
                 q.q0 = __shfl_sync(~0u, mine.q0, l);
                 q.nq = __shfl_sync(~0u, mine.nq, l);
+                q.nodes = __shfl_sync(~0u, mine.nodes, l);
                 q.ln = __shfl_sync(~0u, mine.ln, l);
                 q.k0 = __shfl_sync(~0u, mine.k0, l);
                 q.slot = __shfl_sync(~0u, mine.slot, l);

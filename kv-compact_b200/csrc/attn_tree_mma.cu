@@ -69,7 +69,7 @@ struct mma_geom {
 // A piece of the CTA's stretch: key tiles lo .. hi-1 of one sequence.
 struct segment {
     int lo, hi, slot;
-    int q0, nq, ln;
+    int q0, nq, nodes, ln;
     int table;                  // table row
 };
 
@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
             int n = 0;
             attn_walk(a, qb, qb + 1, w, hg == 0, [&](int, const kvc_attn_seq & q, int lo, int hi, int slot) {
                 if (n >= batch && n < batch + MAX_SEGS && lane == 0) {
-                    segs[n - batch] = segment{lo, hi, slot, q.q0, q.nq, q.ln, q.slot};
+                    segs[n - batch] = segment{lo, hi, slot, q.q0, q.nq, q.nodes, q.ln, q.slot};
                 }
                 n++;
             });
@@ -423,6 +423,7 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
         kvc_attn_seq q;
         q.q0 = segs[seg].q0;
         q.nq = segs[seg].nq;
+        q.nodes = segs[seg].nodes;
         q.ln = segs[seg].ln;
         // this warp's KV head, block of query rows and share of the keys
         const int rows_here = (int)min((long long)a.rb, (long long)q.nq * a.g - (long long)qb * a.rb);
@@ -436,8 +437,8 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
         const int r0 = qb * a.rb + unit / nh * RW;
         const int nr = min(RW, rows_here - unit / nh * RW);
         // rows from here on are the nodes' own, and the mask decides on them (one node that sees itself needs none)
-        const bool masked = a.mask && a.mask_words > 0 && !(q.nq == 1 && (a.mask[(size_t)q.q0 * a.mask_words] & 1u));
-        const int first_own = masked || (a.mask && !a.mask_words) ? q.ln - q.nq : INT_MAX;
+        const bool masked = a.mask && a.mask_words > 0 && !(q.nodes == 1 && (a.mask[(size_t)q.q0 * a.mask_words] & 1u));
+        const int first_own = masked || (a.mask && !a.mask_words) ? q.ln - q.nodes : INT_MAX;
 
         // query fragments: lane (g, t) holds, of row g of each block of 8, the
         // elements that the k-steps of its K type ask of it; two pieces lie in

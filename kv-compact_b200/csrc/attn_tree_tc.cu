@@ -72,7 +72,7 @@ struct cfg {
 };
 
 struct segment {
-    int lo, hi, slot, qb, q0, nq, ln, table;
+    int lo, hi, slot, qb, q0, nq, nodes, ln, table;
 };
 
 // Per key of a tile. Eight tiles deep: when tile i is filled, tile i - 5 and those before it have been read.
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                 int n = 0;
                 attn_walk(a, 0, n_blocks, w, h == 0, [&](int qb, const kvc_attn_seq & q, int lo, int hi, int slot) {
                     if (n >= batch && n < batch + MAX_SEGS && lane == 0)
-                        X.segs[n - batch] = segment{lo, hi, slot, qb, q.q0, q.nq, q.ln, q.slot};
+                        X.segs[n - batch] = segment{lo, hi, slot, qb, q.q0, q.nq, q.nodes, q.ln, q.slot};
                     n++;
                 });
                 if (lane == 0) {
@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
             const float mul = QP == 2 ? X.mul[r] : 1.0f;
             const bool real = r < rows_here;
             const int node = (int)a.by_group.div(r0 + r);
-            const int first_own = a.mask ? S.ln - S.nq : INT_MAX;
+            const int first_own = a.mask ? S.ln - S.nodes : INT_MAX;
             const int steps = (n + 1 - t) / 2;
             float m = -INFINITY, l = 0.0f, back = 0.0f;  // back: 2^(R - 10) of the tile whose product is still in TMEM
             float2 O[D / 2];

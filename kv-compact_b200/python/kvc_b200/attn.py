@@ -89,10 +89,11 @@ class Tree:
 
     q [total, heads, d_k] float16 or float32; cu int32 [n + 1]: entry s has the rows cu[s] .. cu[s+1]-1 of q; seqs int32
     [n]: its sequence, whose last rows are the nodes' own; mask int32 [total, words]: bit j of a node's words shows it the
-    row of its entry's node j (None: all); max_nodes: most nodes of an entry. out [total, heads, d_v] (of q's type) and lse
+    row of its entry's node j (None: all); max_nodes: most nodes of an entry (left out: 1 for a row of q per entry and no
+    mask, else all rows of q, which always suffices but costs time). out [total, heads, d_v] (of q's type) and lse
     [total, heads] are made here unless given (lse=False: none)."""
 
-    def __init__(self, fns, cache, q, cu, seqs, mask=None, max_nodes=1, scale=None, layer=0, out=None, lse=None):
+    def __init__(self, fns, cache, q, cu, seqs, mask=None, max_nodes=None, scale=None, layer=0, out=None, lse=None):
         import torch
         dev, c = cache.device, cache.desc
         _kind(q.dtype)
@@ -104,6 +105,8 @@ class Tree:
         if mask is not None:
             need(mask, "mask", (torch.int32,), dev, (q.shape[0], None))
         total, h = q.shape[0], q.shape[1]
+        if max_nodes is None:
+            max_nodes = 1 if mask is None and total <= n else total
         self.out = torch.empty(total, h, c.d_v, dtype=q.dtype, device=dev) if out is None else need(
             out, "out", (q.dtype,), dev, (total, h, c.d_v))
         self.lse = None if lse is False else torch.empty(total, h, device=dev) if lse is None else need(

@@ -537,6 +537,40 @@ def test_tree_far_rows(kvc, kind, page, nodes):
     assert float((u.out.double() - out).abs().max()) < 1e-4
 
 
+@pytest.mark.parametrize("kind,nodes,cut", [(R.F32, [1, 3], 1), (R.F32, [1, 20], 9), (R.Q8_0, [1, 3], 1), (R.F16, [2, 9], 5),
+                                            (R.F16, [1, 60], 40), (R.Q8_0, [3, 80], 36)])
+@pytest.mark.parametrize("qt", [torch.float16, torch.float32])
+def test_tree_cut_entries(kvc, kind, nodes, cut, qt):
+    """An entry with more nodes than max_nodes: the nodes that are left see what they would see beside the others (whose
+    own rows are in the cache all the same), and the rows of the others are left as they were."""
+    c, q, t, (out, lse) = tree_case(kvc, lens=[90, 70], nodes=nodes, kt=kind, vt=kind, qt=qt, beta=True, seed=cut)
+    u = attn.Tree(kvc, c.handle(kvc), q, t._keep[1], t._keep[2], mask=t._keep[3], max_nodes=cut, scale=64 ** -0.5)
+    u.out.fill_(5.0)
+    u.lse.fill_(5.0)
+    u.run()
+    torch.cuda.synchronize()
+    used = torch.cat([c.rows(0), c.rows(1)])
+    K, V = (R.decode(x[0][used], kind) for x in (c.K, c.V))
+    o_tol, l_tol = bounds(q, K.view(-1, c.hkv, c.dk), V, float(c.beta.abs().max()), kind, qt == torch.float16, c.dk ** -0.5)
+    for first, n in ((0, min(nodes[0], cut)), (nodes[0], min(nodes[1], cut))):
+        check(u.out[first:first + n], out[first:first + n], o_tol, "out")
+        check(u.lse[first:first + n], lse[first:first + n], l_tol, "lse")
+    behind = slice(nodes[0] + cut, None)
+    assert bool((u.out[behind] == 5.0).all()) and bool((u.lse[behind] == 5.0).all())
+
+
+def test_tree_max_nodes_left_out(kvc):
+    """Where max_nodes is not given, a mask or more rows than entries make it the number of rows; else it is 1."""
+    c, q, t, (out, _) = tree_case(kvc, lens=[40, 9], nodes=[1, 5], qt=torch.float32)
+    u = attn.Tree(kvc, c.handle(kvc), q, t._keep[1], t._keep[2], mask=t._keep[3], scale=64 ** -0.5)
+    u.run()
+    torch.cuda.synchronize()
+    assert u.desc.max_nodes == 6 and float((u.out.double() - out).abs().max()) < 1e-4
+    assert attn.Tree(kvc, c.handle(kvc), q, t._keep[1], t._keep[2]).desc.max_nodes == 6
+    assert attn.Tree(kvc, c.handle(kvc), q[:2], t._keep[1], t._keep[2], mask=t._keep[3][:2]).desc.max_nodes == 2
+    assert attn.Tree(kvc, c.handle(kvc), q[:2], t._keep[1], t._keep[2]).desc.max_nodes == 1
+
+
 # ---- prompts ------------------------------------------------------------------------------
 
 def prompt_case(new, past, hkv=2, g=4, dk=64, dv=64, dtype=torch.float16, causal=True, seed=0, wide=False, scale=None, edit=None):
