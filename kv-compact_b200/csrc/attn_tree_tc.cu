@@ -38,6 +38,7 @@
 
 #include <limits.h>
 #include <math.h>
+#include <stddef.h>
 
 namespace {
 
@@ -76,23 +77,26 @@ struct segment {
 };
 
 // Per key of a tile. Eight tiles deep: when tile i is filled, tile i - 5 and those before it have been read.
-struct tile_info {
+struct alignas(16) tile_info {      // read four at a time
     float f[TN];                // factor of S: scale 2^e
     float b[TN];                // beta, or -inf
     int e[TN];                  // exponent of the V row << 23, or HIDDEN
 };
 
 struct shared {
-    uint64_t full[8], empty[8], s_full[2], p_full[2], o_full[2];
-    uint32_t tmem;
+    uint64_t full[8], empty[8], s_full[2], p_full[2], o_full[2], done;
+    uint32_t tmem, lost;        // lost: a wait ran out
     int n_segs[2];
-    unsigned long long bad[2];  // per stream: rows of the tile that are taken value by value
+    unsigned long long bad[2][2];   // per stream, of even and odd steps (a slow warp may still read the step before's): rows
+                                    // of the tile that are taken value by value
     segment segs[MAX_SEGS];
     int rows[2][TN];            // pool rows of a tile
     float mul[TM];              // power of two that a query row was divided by
     float jm[TM], jl[TM];
     tile_info info[8];
 };
+
+static_assert(offsetof(shared, info) % 16 == 0, "tile_info on a 16-byte boundary");
 
 template <int N>
 __device__ __forceinline__ void reg_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(N)); }
@@ -225,18 +229,28 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
             mbar_init(X.p_full + t, 4);
             mbar_init(X.o_full + t, 1);
         }
+        mbar_init(&X.done, 1);
+        X.lost = 0;
         mbar_init_fence();
     }
     cudaTriggerProgrammaticLaunchCompletion();
     __syncthreads();
     fence_after_sync();
     const uint32_t tmem = X.tmem;
-    bool ok = true;                                      // false: a wait ran out; the status says so
+    // False: a wait ran out; the status says so. The thread goes on without waiting, whatever it then reads, and takes
+    // every barrier of its group: these have no bound, and other warps may be behind them already.
+    bool ok = true;
     auto await = [&](uint64_t * bar, uint32_t parity) {
         if (ok && !mbar_wait(bar, parity, POLLS)) {
             ok = false;
+            X.lost = 1;
             if (a.status) *a.status = KVC_ERR_CUDA;
         }
+    };
+    // The same where the warp goes on to instructions of all its lanes: they agree.
+    auto await_warp = [&](uint64_t * bar, uint32_t parity) {
+        await(bar, parity);
+        ok = __all_sync(~0u, ok);
     };
     int items = 0;                                       // K and V tiles through the ring before this segment
     int turns[2] = {0, 0};                               // tiles of each stream before it
@@ -396,8 +410,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
             };
             for (int j = 0; j < steps; j++) {
                 const int i = 2 * j + t;                 // tile of the segment
-                await(X.s_full + t, (turns[t] + j) & 1);
-                if (!__all_sync(~0u, ok)) break;
+                await_warp(X.s_full + t, (turns[t] + j) & 1);
                 fence_after_sync();
                 const tile_info & I = X.info[i & 7];
                 const int j0 = (S.lo + i) * TN;
@@ -458,8 +471,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                 m = mn;
                 l *= f;
                 if (j > 0) {
-                    await(X.o_full + t, (turns[t] + j - 1) & 1);       // the product of the tile before
-                    if (!__all_sync(~0u, ok)) break;
+                    await_warp(X.o_full + t, (turns[t] + j - 1) & 1);  // the product of the tile before
                     fence_after_sync();
                     collect(f);
                 }
@@ -470,12 +482,12 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                 float2 sums = make_float2(0.0f, 0.0f);
                 if (KP == 2 || own) {
                     const int it = items + 2 * i + 1;    // the exponents are written with V
-                    await(X.full + it % C::SLOTS, (it / C::SLOTS) & 1);
+                    await_warp(X.full + it % C::SLOTS, (it / C::SLOTS) & 1);
                     const int2 e2 = *reinterpret_cast<const int2 *>(&I.e[2 * lane]);
                     R = __reduce_max_sync(~0u, max(e2.x, e2.y));
                     if (own) {
                         uint8_t * vt = ring + (it % C::SLOTS) * C::SLOT;
-                        if (r == 0) X.bad[t] = 0;
+                        if (r == 0) X.bad[t][j & 1] = 0;
                         const int least = __reduce_min_sync(~0u, min(e2.x > HIDDEN ? e2.x : INT_MAX, e2.y > HIDDEN ? e2.y : INT_MAX));
                         group_sync(1 + t, 128);
                         if (r < TN && I.e[r] > HIDDEN) {
@@ -485,10 +497,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                                 for (uint32_t y : {v.x, v.y, v.z, v.w})
                                     bad |= (y & 0x7C00u) == 0x7C00u || (y & 0x7C000000u) == 0x7C000000u;
                             }
-                            if (bad) atomicOr(&X.bad[t], 1ull << r);
+                            if (bad) atomicOr(&X.bad[t][j & 1], 1ull << r);
                         }
                         group_sync(1 + t, 128);
-                        const unsigned long long bad = X.bad[t];
+                        const unsigned long long bad = X.bad[t][j & 1];
                         if (bad) {
                             R = max((bad >> (2 * lane)) & 1 ? HIDDEN : e2.x, (bad >> (2 * lane + 1)) & 1 ? HIDDEN : e2.y);
                             R = __reduce_max_sync(~0u, R);
@@ -577,11 +589,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                 if (lane == 0) mbar_arrive(X.p_full + t);
             }
             if (steps > 0) {
-                await(X.o_full + t, (turns[t] + steps - 1) & 1);
-                if (__all_sync(~0u, ok)) {
-                    fence_after_sync();
-                    collect(1.0f);
-                }
+                await_warp(X.o_full + t, (turns[t] + steps - 1) & 1);
+                fence_after_sync();
+                collect(1.0f);
             }
             // ---- join the streams (over the ring: every product has been taken)
             group_sync(3, 256);
@@ -833,7 +843,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                 const uint32_t qa = smem_u32(sq), ra = smem_u32(ring);
                 auto qk = [&](int i) {
                     const int it = items + 2 * i;
-                    await(X.full + it % C::SLOTS, (it / C::SLOTS) & 1);
+                    await_warp(X.full + it % C::SLOTS, (it / C::SLOTS) & 1);
                     if (!ok) return;
                     fence_after_sync();
                     const uint32_t ka = ra + (it % C::SLOTS) * C::SLOT;
@@ -854,7 +864,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                 };
                 auto pv = [&](int i) {
                     const int it = items + 2 * i + 1;
-                    await(X.full + it % C::SLOTS, (it / C::SLOTS) & 1);
+                    await_warp(X.full + it % C::SLOTS, (it / C::SLOTS) & 1);
                     if (!ok) return;
                     fence_after_sync();
                     const uint32_t va = ra + (it % C::SLOTS) * C::SLOT, p = tmem + C::P_COL + (i & 1) * 64;
@@ -875,7 +885,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                 if (n > 0) qk(0);
                 if (n > 1) qk(1);
                 for (int i = 0; i < n && ok; i++) {
-                    await(X.p_full + (i & 1), (turns[i & 1] + (i >> 1)) & 1);
+                    await_warp(X.p_full + (i & 1), (turns[i & 1] + (i >> 1)) & 1);
                     if (!ok) break;
                     fence_after_sync();
                     if (i + 2 < n) qk(i + 2);            // first: the stream's next softmax can begin
@@ -889,6 +899,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
     __syncthreads();
     if (warp == 12) {
         fence_after_sync();
+        if (X.lost) {                                    // products may be under way that nobody waited for
+            commit_mma(&X.done);
+            mbar_wait(&X.done, 0, POLLS);
+            __syncwarp();
+        }
         tmem_free(tmem, C::COLS);
     }
 }
