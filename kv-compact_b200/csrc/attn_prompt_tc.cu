@@ -87,7 +87,9 @@ __global__ void __launch_bounds__(cfg<D, NT>::THREADS, 3 - NT) k_prompt_tc(const
     uint64_t * p_full = s_full + 2;                      // [2] P is, and O may be added to
     uint64_t * o_full = p_full + 2;                      // [2] the product has been added
     uint64_t * v_fixed = o_full + 2;                     // the last V tile's rows past the end are zero
-    uint32_t * slot = reinterpret_cast<uint32_t *>(v_fixed + 1);
+    uint64_t * done = v_fixed + 1;                       // products that nobody waited for
+    uint32_t * slot = reinterpret_cast<uint32_t *>(done + 1);
+    uint32_t * lost = slot + 1;                          // a wait ran out
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int h = blockIdx.x % a.Hkv;
 
@@ -144,6 +146,8 @@ __global__ void __launch_bounds__(cfg<D, NT>::THREADS, 3 - NT) k_prompt_tc(const
             mbar_init(o_full + t, 1);
         }
         mbar_init(v_fixed, 1);
+        mbar_init(done, 1);
+        *lost = 0;
         mbar_init_fence();
     }
     __syncthreads();
@@ -207,8 +211,13 @@ __global__ void __launch_bounds__(cfg<D, NT>::THREADS, 3 - NT) k_prompt_tc(const
                                id_o, j > 0 || k > 0);
                 commit_mma(o_full + t);
             };
-            auto wait_full = [&](int i) { ok = ok && mbar_wait(full + i % C::SLOTS, (i / C::SLOTS) & 1, POLLS); };
-            ok = mbar_wait(q_full, 0, POLLS);
+            // the products are issued by whole warps: the lanes agree on what a wait gave
+            auto wait_warp = [&](uint64_t * bar, uint32_t parity) {
+                ok = ok && mbar_wait(bar, parity, POLLS);
+                ok = __all_sync(~0u, ok);
+            };
+            auto wait_full = [&](int i) { wait_warp(full + i % C::SLOTS, (i / C::SLOTS) & 1); };
+            wait_warp(q_full, 0);
             wait_full(0);
             fence_after_sync();
             if (ok) {
@@ -219,12 +228,12 @@ __global__ void __launch_bounds__(cfg<D, NT>::THREADS, 3 - NT) k_prompt_tc(const
             }
             for (int j = 0; j < n && ok; j++) {
                 wait_full(2 * j + 1);
-                if (j == n - 1 && fixed) ok = ok && mbar_wait(v_fixed, 0, POLLS);
+                if (j == n - 1 && fixed) wait_warp(v_fixed, 0);
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
                     if (!ok) break;
                     if (j < steps[t]) {
-                        ok = mbar_wait(p_full + t, j & 1, POLLS);
+                        wait_warp(p_full + t, j & 1);
                         if (!ok) break;
                         fence_after_sync();
                         pv(t, j);
@@ -348,14 +357,20 @@ __global__ void __launch_bounds__(cfg<D, NT>::THREADS, 3 - NT) k_prompt_tc(const
         if (real && a.lse) a.lse[row] = !ok ? NAN : l == 0.0f ? -INFINITY : m * a.scale + logf(l);
         fence_before_sync();
     }
+    if (!ok) *lost = 1;
     __syncthreads();
-    // copies in flight land before the CTA ends (only where a wait ran out can there be any)
-    if (warp == 4 * NT && lane < C::SLOTS && !ok) {
+    // copies in flight land, and products end, before the CTA does (only where a wait ran out can there be any)
+    if (warp == 4 * NT && lane < C::SLOTS && *lost) {
         mbar_wait(full + lane, 0, POLLS);
         mbar_wait(full + lane, 1, POLLS);
     }
     if (warp == 4 * NT + 1) {
         fence_after_sync();
+        if (*lost) {
+            commit_mma(done);
+            mbar_wait(done, 0, POLLS);
+            __syncwarp();
+        }
         tmem_free(tmem, C::COLS);
     }
 }
