@@ -387,8 +387,16 @@ size_t simt_smem(int dk, int dv) {
 
 template <int C>
 int launch_simt(const kvc_attn_args & a, dim3 grid, cudaStream_t st) {
+    // the limit is the function's, whoever calls it: one value for all sizes
+    static std::atomic<bool> set[64];
+    int dev = 0;
+    KVC_CUDA(cudaGetDevice(&dev));
+    if (!set[dev & 63].load(std::memory_order_relaxed)) {
+        KVC_CUDA(cudaFuncSetAttribute(k_attn_simt<C>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      (int)simt_smem(KVC_MAX_D, KVC_MAX_D)));
+        set[dev & 63].store(true, std::memory_order_relaxed);
+    }
     const size_t sm = simt_smem(a.dk, a.dv);
-    KVC_CUDA(cudaFuncSetAttribute(k_attn_simt<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm));
     k_attn_simt<C><<<grid, THREADS, sm, st>>>(a);
     g_serve_launches++;
     KVC_CUDA(cudaGetLastError());

@@ -7,6 +7,7 @@ queries P times the row scale is rounded to fp16 once, 2^-11 (half an eps), the 
 products and the sum of minimum and centre.
 """
 import math
+import threading
 
 import pytest
 import torch
@@ -514,6 +515,35 @@ def test_tree_calls_side_by_side(kvc):
     torch.cuda.synchronize()
     for u in calls:
         assert torch.equal(u.out, want)
+
+
+def test_calls_from_host_threads(kvc):
+    """Calls of the general kernel with different head sizes from several host threads, each on a stream of its own. (The
+    C calls are made directly, so that they meet; a call that is refused gives its code.)"""
+    sizes = [(256, 100), (32, 100), (200, 100), (32, 66)]
+    gate, failed = threading.Barrier(len(sizes)), []
+
+    def worker(dk, dv):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                c, q, t, _ = tree_case(kvc, lens=[4], nodes=[1], hkv=1, g=1, dk=dk, dv=dv, kt=R.F32, vt=R.F32, qt=torch.float32)
+                t.run()
+                torch.cuda.current_stream().synchronize()
+                want, st = t.out.clone(), torch.cuda.current_stream().cuda_stream
+                gate.wait(60)
+                codes = {t.fn(*t._args, st) for _ in range(20000)}
+                torch.cuda.current_stream().synchronize()
+                assert codes == {0} and torch.equal(t.out, want)
+        except Exception as e:  # noqa: BLE001
+            gate.abort()
+            failed.append(f"{dk}, {dv}: {e}")
+
+    threads = [threading.Thread(target=worker, args=a) for a in sizes]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
 
 
 @pytest.mark.parametrize("kind,page,nodes", [(R.F16, 16, [1, 2]), (R.F16, 16, [40, 2]), (R.F16, 5, [1, 2]), (R.F32, 16, [1, 2])])
