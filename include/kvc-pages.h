@@ -23,6 +23,7 @@
  * Sequence lists are HOST arrays, read before the call returns: ids in
  * [0, n_slots), at most KVC_PAGES_MAX_SEQS of them; each destination appears
  * once and is no other entry's source. Everything else is device memory.
+ * n_pages and max_pages times page_size are at most 2^31 - 1 - 65536.
  * Calls with n = 0 do nothing. Return codes: 0; -1 a null argument; -2 bad
  * counts, ids or a repeated destination; -4 a row size that does not match;
  * -10 no sm_100 device; -12 CUDA error; -13 a shape outside the limits or a

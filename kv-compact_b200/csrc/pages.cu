@@ -59,8 +59,9 @@ int kvc_check_cache(const kvc_page_cache * c) {
     if (kvc_row_elements(c->k_type, c->k_row_bytes) != ek || kvc_row_bytes(c->k_type, (int)ek) != c->k_row_bytes ||
         kvc_row_elements(c->v_type, c->v_row_bytes) != ev || kvc_row_bytes(c->v_type, (int)ev) != c->v_row_bytes)
         return KVC_ERR_ROWSIZE;
-    // row numbers of the pool and of a sequence are 32-bit
-    if ((long long)c->n_pages * c->page_size > INT_MAX || (long long)c->max_pages * c->page_size > INT_MAX)
+    // row numbers of the pool and of a sequence are 32-bit, with room for the step past the end that scans and grids take
+    constexpr int MOST_ROWS = INT_MAX - 65536;
+    if ((long long)c->n_pages * c->page_size > MOST_ROWS || (long long)c->max_pages * c->page_size > MOST_ROWS)
         return KVC_ERR_SHAPE;
     // the widest element of the type decides how rows may be addressed
     const uintptr_t ka = c->k_type == KV_TYPE_F32 ? 4 : 2, va = c->v_type == KV_TYPE_F32 ? 4 : 2;
@@ -110,6 +111,9 @@ cache_dev on_device(const kvc_page_cache * c) {
             c->max_pages, c->n_head_kv, kvc_make_divisor((uint32_t)c->page_size)};
 }
 
+// Pages of `rows` rows (rows + page may pass 2^31).
+__device__ __forceinline__ int pages_of(int rows, int page) { return rows / page + (rows % page != 0); }
+
 constexpr int PLAN_THREADS = 1024;
 constexpr int PLAN_PER = 16;          // counts per thread and scan step
 
@@ -144,15 +148,20 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_plan(cache_dev c, const __grid
                                                        int * __restrict__ ws) {
     __shared__ int sums[32];
     __shared__ int bad;
+    __shared__ unsigned long long asked;                 // new pages of all entries: up to 256 times 2^31
     const int t = threadIdx.x;
-    if (t == 0) bad = 0;
+    if (t == 0) {
+        bad = 0;
+        asked = 0;
+    }
+    __syncthreads();
     plan_item it{};
     if (t < ids.n) {
         const int cap = c.max_pages * c.page;
         const int len = min(max(c.seq_len[ids.src[t]], 0), cap);
         long long length = len;
         if (op == OP_RESERVE) {
-            it.whole = (len + c.page - 1) / c.page;
+            it.whole = pages_of(len, c.page);
             length = (long long)len + counts.src[t];
         } else if (op == OP_FORK) {
             it.whole = len / c.page;
@@ -168,7 +177,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_plan(cache_dev c, const __grid
             atomicOr(&bad, 1);
         } else {
             it.length = (int)length;
-            it.need = max((it.length + c.page - 1) / c.page - it.whole, 0);
+            it.need = max(pages_of(it.length, c.page) - it.whole, 0);
+            atomicAdd(&asked, (unsigned long long)it.need);
         }
     }
     int total;
@@ -178,8 +188,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_plan(cache_dev c, const __grid
     int * fresh = reinterpret_cast<int *>(reinterpret_cast<char *>(ws) + WS_ITEMS);
     int found = 0;
     __syncthreads();
-    const bool too_long = bad != 0;
-    if (!too_long) {
+    const bool too_long = bad != 0, too_many = asked > (unsigned long long)c.n_pages;      // beyond that the sums may have wrapped
+    if (!too_long && !too_many) {
         const bool wide = ((uintptr_t)c.ref & 15) == 0;
         for (int at = 0; found < total && at < c.n_pages; at += PLAN_THREADS * PLAN_PER) {
             const int p0 = at + t * PLAN_PER;
@@ -210,7 +220,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_plan(cache_dev c, const __grid
         }
     }
     if (t == 0) {
-        const bool ok = !too_long && found >= total;
+        const bool ok = !too_long && !too_many && found >= total;
         ws[0] = ok;
         if (!ok) *c.status = too_long ? KVC_ERR_SHAPE : KVC_ERR_OOM;
     }

@@ -221,6 +221,20 @@ def test_a_call_that_cannot_be_done_changes_nothing(kvc):
     m.same(c)
 
 
+@pytest.mark.parametrize("add", [[2 ** 30, 2 ** 30], [2 ** 30, 1], [5, 0]])
+def test_more_pages_asked_for_than_32_bits_count(kvc, add):
+    """Table rows so long that the entries of a call together ask for 2^31 pages (the table is not written)."""
+    z = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")  # noqa: E731
+    rows = torch.zeros(1, 4, 4, dtype=torch.uint8, device="cuda")
+    table = torch.empty(2, 2 ** 30, dtype=torch.int32, device="cuda")
+    table[:, :8] = -1
+    c = pages.PageCache(kvc, rows, rows.clone(), table, z(2), z(4), z(1), 1, 1, 1, 1, 0, 0)
+    c.reserve([0, 1], add)
+    torch.cuda.synchronize()
+    assert int(c.status) == -11 and c.seq_len.tolist() == [0, 0] and int(c.ref_count.abs().sum()) == 0
+    assert bool((table[:, :8] == -1).all())
+
+
 @pytest.mark.parametrize("n_pages", [1, 15, 16, 17, 5000, 40001])
 def test_lowest_free_pages(kvc, n_pages):
     """Pools around and beyond one step of the scan, with few free pages and far ones."""

@@ -65,6 +65,16 @@ def test_cache_refusals(kvc, kw, code):
     assert L.kvc_attn_tree(ref, ctypes.addressof(t), None, 0, None) == code
 
 
+@pytest.mark.parametrize("kw", [dict(n_pages=2 ** 31 - 1, page_size=1), dict(max_pages=2 ** 31 - 1, page_size=1),
+                                dict(n_pages=1, page_size=2 ** 31 - 1, max_pages=1)])
+def test_cache_sizes_leave_room_for_a_step(kvc, kw):
+    """Scans and grids step past the last page and row; their numbers are 32-bit."""
+    c, L = cache_desc(**kw), kvc["_lib"]
+    assert L.kvc_pages_free(ctypes.addressof(c), pages.ids([0]), 1, None, 0, None) == -13
+    small = {k: v - 65536 if v > 1 else v for k, v in kw.items()}
+    assert L.kvc_pages_free(ctypes.addressof(cache_desc(**small)), pages.ids([0]), 1, None, 0, None) == -1    # no workspace
+
+
 def test_page_call_refusals(kvc):
     L, c = kvc["_lib"], cache_desc()
     ref = ctypes.addressof(c)
