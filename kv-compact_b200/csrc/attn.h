@@ -40,8 +40,9 @@ struct kvc_attn_args {
     int n_slots, n_pages, max_pages, page;
     kvc_divisor by_page, by_group;
     // the split: blocks of rb query rows, tiles of `tile` keys, W workers per
-    // (KV head, row block)
-    int rb, tile, W;
+    // KV head and stretch; n_parts stretches, each with partial results of its own:
+    // one per row block, or 1 where the row blocks are laid end to end
+    int rb, tile, W, n_parts;
     kvc_divisor by_tile;
     float * part;           // partial results
     int * meta;             // [row blocks][n_seqs][2]: first and last worker of a sequence (W > 1)
@@ -197,11 +198,12 @@ __device__ __forceinline__ void attn_walk(const kvc_attn_args & a, int qb0, int 
 
 // Partial results of worker w, slot s: rb sums of d_v, then rb maxima, rb sums.
 __device__ __forceinline__ float * attn_part(const kvc_attn_args & a, int qb, int h, int w, int slot) {
-    return a.part + ((((size_t)qb * a.Hkv + h) * a.W + w) * 2 + slot) * ((size_t)a.rb * (a.dv + 2));
+    const size_t p = a.n_parts > 1 ? qb : 0;
+    return a.part + (((p * a.Hkv + h) * a.W + w) * 2 + slot) * ((size_t)a.rb * (a.dv + 2));
 }
-// Workspace bytes: the partial results, then meta.
+// Workspace bytes for `blocks` row blocks: the partial results, then meta.
 inline size_t kvc_attn_part_bytes(const kvc_attn_args & a, long long blocks, size_t * meta_at) {
-    *meta_at = (size_t)blocks * a.Hkv * a.W * 2 * a.rb * (a.dv + 2) * sizeof(float);
+    *meta_at = (size_t)a.n_parts * a.Hkv * a.W * 2 * a.rb * (a.dv + 2) * sizeof(float);
     return a.W > 1 ? *meta_at + (size_t)blocks * a.n_seqs * 2 * sizeof(int) : 0;
 }
 

@@ -413,6 +413,7 @@ void kvc_attn_simt_split(kvc_attn_args * a, int sms, bool whole) {
     const long long blocks = ((long long)a->max_q * a->g + RB - 1) / RB * a->Hkv;
     const long long w = whole || blocks <= 0 ? 1 : (8LL * sms + blocks - 1) / blocks;
     a->W = (int)(w < 1 ? 1 : w);
+    a->n_parts = (int)(blocks / a->Hkv);
 }
 
 int kvc_launch_attn_simt(const kvc_attn_args & a, cudaStream_t st) {

@@ -89,7 +89,7 @@ int make_plan(const kvc_page_cache * c, const kvc_tree_desc * t, int sms, tree_p
     } else {
         p->kernel = tree_plan::SIMT;
         kvc_attn_simt_split(&a, sms, false);
-        blocks = ((long long)a.max_q * a.g + a.rb - 1) / a.rb;
+        blocks = a.n_parts;
     }
     p->bytes = kvc_attn_part_bytes(a, blocks, &p->meta_at);
     return KVC_OK;

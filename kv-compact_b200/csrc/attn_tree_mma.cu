@@ -1193,6 +1193,7 @@ bool kvc_attn_tree_mma_plan(kvc_attn_args * a, int sms, long long * blocks) {
     a->by_tile = kvc_make_divisor((uint32_t)tile);
     const int w = sms / (G.ngh * ngr);                   // one CTA per SM, equal stretches
     a->W = w < 1 ? 1 : w;
+    a->n_parts = ngr;
     *blocks = ngr;
     return true;
 }

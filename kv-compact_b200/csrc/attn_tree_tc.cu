@@ -972,6 +972,7 @@ bool kvc_attn_tree_tc_plan(kvc_attn_args * a, int sms, long long * blocks) {
     a->by_tile = kvc_make_divisor(TN);
     const long long w = sms / a->Hkv;                    // one CTA per SM; the row blocks are laid end to end
     a->W = (int)(w < 1 ? 1 : w);
+    a->n_parts = 1;
     *blocks = n;
     return true;
 }

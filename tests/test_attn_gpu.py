@@ -6,6 +6,7 @@ A 2^-21 with A = max sum |q||k| scale, and x = score + beta and its scaling to b
 queries P times the row scale is rounded to fp16 once, 2^-11 (half an eps), the output once more; Q4_1 rounds two such
 products and the sum of minimum and centre.
 """
+import ctypes
 import math
 import threading
 
@@ -336,6 +337,25 @@ def test_tree_refuses_a_small_workspace(kvc):
     assert t.fn(cache, desc, ws, size - 1, None) == -13
     assert t.fn(cache, desc, None, size, None) == -1
     assert t.fn(cache, desc, ws + 4, size, None) == -13
+
+
+def test_tree_workspace_of_many_nodes(kvc):
+    """The partial results go by the workers, not by the rows of an entry: a worker shares two pieces at most."""
+    c, q, t, _ = tree_case(kvc, lens=[100], nodes=[40], hkv=8, g=4, dk=128, dv=128, kt=R.F16, vt=R.F16)
+    size = {}
+    for n in (40, 1000, 16000):
+        t.desc.total, t.desc.max_nodes = n, n
+        rc = ctypes.c_int(0)
+        size[n] = kvc["_lib"].kvc_attn_tree_workspace(t.cache.ref, t.ref, ctypes.addressof(rc))
+        assert rc.value == 0
+    assert size[40] < size[1000] < size[16000] < size[40] + 16000 * 4      # meta: two numbers per 128 rows and entry
+
+
+@pytest.mark.parametrize("kind,qt", [(R.F16, torch.float16), (R.Q8_0, torch.float32)])
+def test_tree_several_row_blocks_in_a_stretch(kvc, kind, qt):
+    """Row blocks laid end to end over the workers, with entries that start and end anywhere in a worker's stretch."""
+    tree_check(kvc, lens=[700, 0, 90, 3000], nodes=[100, 70, 3, 150], hkv=3, g=4, kt=kind, vt=kind, qt=qt, page=16, beta=True)
+    tree_check(kvc, lens=[20, 5000], nodes=[300, 65], hkv=1, g=2, kt=kind, vt=kind, qt=qt, page=64)
 
 
 def many_rows(**kw):
