@@ -22,7 +22,8 @@
  *
  * Sequence lists are HOST arrays, read before the call returns: ids in
  * [0, n_slots), at most KVC_PAGES_MAX_SEQS of them; each destination appears
- * once and is no other entry's source. Everything else is device memory.
+ * once and is no other entry's source. A captured call keeps them, and host
+ * counts and first rows, as they were. Everything else is device memory.
  * n_pages and max_pages times page_size are at most 2^31 - 1 - 65536.
  * Calls with n = 0 do nothing. Return codes: 0; -1 a null argument; -2 bad
  * counts, ids or a repeated destination; -4 a row size that does not match;
@@ -77,7 +78,12 @@ int kvc_pages_reserve(const kvc_page_cache * cache, const int * seqs, const int 
  * write then sets no beta; beta_rows needs a cache with beta). Rows past the
  * sequence's length are skipped; a write also skips rows of pages that more
  * than one sequence holds, and then sets *status to -2. seqs may repeat in a
- * read. */
+ * read.
+ * One layer's rows (a decoder has layer l's K and V only after layer l - 1's
+ * attention): these two calls, and kvc_attn_tree with layer 0, also take a
+ * description of that layer alone, the same but for n_layers = 1 and K, V and
+ * beta at the layer's own part (K + l * n_pages * page_size * k_row_bytes, and
+ * so on). Calls that change tables want all layers. */
 int kvc_pages_write(const kvc_page_cache * cache, const int * seqs, const int * first, const int * count, int n,
                     const uint8_t * k_rows, const uint8_t * v_rows, const float * beta_rows, void * stream);
 int kvc_pages_read(const kvc_page_cache * cache, const int * seqs, const int * first, const int * count, int n,

@@ -91,7 +91,7 @@ class PageCache:
                                   d_v, k_type, v_type, K.shape[2], V.shape[2], K.data_ptr(), V.data_ptr(),
                                   beta.data_ptr() if beta is not None else None, page_table.data_ptr(),
                                   seq_len.data_ptr(), ref_count.data_ptr(), status.data_ptr())
-        self.ref = ctypes.addressof(self.desc)
+        self.ref, self._layers = ctypes.addressof(self.desc), {}
         size = self.lib.kvc_pages_workspace(self.ref)
         if size == 0:
             raise ValueError("kvc_pages_workspace: the cache's sizes are outside the limits")
@@ -114,8 +114,19 @@ class PageCache:
         return cls(fns, K, V, z(n_slots, max_pages) - 1, z(n_slots), z(n_pages), z(1), page_size, n_head_kv, d_k, d_v,
                    k_type, v_type, beta=b)
 
-    def _call(self, name, *args):
-        rc = on_device(self.index, getattr(self.lib, name), self.ref, *args)
+    def _layer(self, layer):
+        """The description of one layer alone (write and read take it, calls that change tables do not)."""
+        if not 0 <= layer < self.desc.n_layers:
+            raise ValueError(f"layer {layer} of {self.desc.n_layers}")
+        if layer not in self._layers:
+            d = PageCacheDesc.from_buffer_copy(self.desc)
+            d.n_layers, d.K, d.V = 1, self.K[layer].data_ptr(), self.V[layer].data_ptr()
+            d.beta = self.beta[layer].data_ptr() if self.beta is not None else None
+            self._layers[layer] = d
+        return self._layers[layer]
+
+    def _call(self, name, *args, desc=None):
+        rc = on_device(self.index, getattr(self.lib, name), ctypes.addressof(desc or self.desc), *args)
         if rc != 0:
             raise RuntimeError(f"{name} failed: {rc}")
 
@@ -134,33 +145,36 @@ class PageCache:
             raise ValueError("seqs and add differ in length")
         self._call("kvc_pages_reserve", seqs, add, len(seqs), *self._ws)
 
-    def _rows(self, name, seqs, first, count, k_rows, v_rows, beta_rows):
+    def _rows(self, name, seqs, first, count, k_rows, v_rows, beta_rows, layer):
         import torch
         seqs, first, count = ids(seqs), ids(first), ids(count)
         if not len(seqs) == len(first) == len(count):
             raise ValueError("seqs, first and count differ in length")
-        n, d = sum(count), self.desc
+        n, d = sum(count), self.desc if layer is None else self._layer(layer)
         for t, what, kind, shape in ((k_rows, "k_rows", torch.uint8, (d.n_layers, n, d.k_row_bytes)),
                                      (v_rows, "v_rows", torch.uint8, (d.n_layers, n, d.v_row_bytes)),
                                      (beta_rows, "beta_rows", torch.float32, (d.n_layers, d.n_head_kv, n))):
             if t is not None:
                 need(t, what, (kind,), self.device, shape)
         at = [t.data_ptr() if t is not None else None for t in (k_rows, v_rows, beta_rows)]
-        self._call(name, seqs, first, count, len(seqs), *at)
+        self._call(name, seqs, first, count, len(seqs), *at, desc=d)
 
-    def write(self, seqs, first, count, k_rows=None, v_rows=None, beta_rows=None):
-        """Rows first[i] .. first[i]+count[i]-1 of sequence seqs[i] from packed rows."""
-        self._rows("kvc_pages_write", seqs, first, count, k_rows, v_rows, beta_rows)
+    def write(self, seqs, first, count, k_rows=None, v_rows=None, beta_rows=None, layer=None):
+        """Rows first[i] .. first[i]+count[i]-1 of sequence seqs[i] from packed rows: k_rows, v_rows uint8 [n_layers, sum of
+        count, row bytes], beta_rows float32 [n_layers, n_head_kv, sum of count]. With a layer given (a decoder has its rows
+        only after the layer before), that one's alone: [1, ...]."""
+        self._rows("kvc_pages_write", seqs, first, count, k_rows, v_rows, beta_rows, layer)
 
-    def read(self, seqs, first, count):
-        """The packed rows (K, V, beta or None) of the given stretches; rows past a sequence's end are zero."""
+    def read(self, seqs, first, count, layer=None):
+        """The packed rows (K, V, beta or None) of the given stretches, of all layers or of one ([1, ...]); rows past a
+        sequence's end are zero."""
         import torch
         seqs, first, count = ids(seqs), ids(first), ids(count)
-        n, d = sum(count), self.desc
+        n, d = sum(count), self.desc if layer is None else self._layer(layer)
         k = torch.zeros(d.n_layers, n, d.k_row_bytes, dtype=torch.uint8, device=self.device)
         v = torch.zeros(d.n_layers, n, d.v_row_bytes, dtype=torch.uint8, device=self.device)
         b = torch.zeros(d.n_layers, d.n_head_kv, n, device=self.device) if self.beta is not None else None
-        self._rows("kvc_pages_read", seqs, first, count, k, v, b)
+        self._rows("kvc_pages_read", seqs, first, count, k, v, b, layer)
         return k, v, b
 
     def copy(self, src_pages, dst_pages):

@@ -113,6 +113,73 @@ def test_a_whole_step_in_a_graph(kvc):
     assert c.seq_len.tolist()[:3] == [70, 140, 56]
 
 
+@pytest.mark.parametrize("nodes", [1, 3])
+def test_a_decoder_writes_layer_by_layer(kvc, nodes):
+    """A row per token, layer by layer: a layer's K and V come from the output of the layer before. In one graph."""
+    gen = torch.Generator().manual_seed(6)
+    dev = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    layers, lens = 3, [30, 100, 15]
+    c = R.Cache(lens, H, D, D, R.F16, R.F16, PAGE, layers=layers, spare=40, beta=True, max_pages=16)
+    h, n = c.handle(kvc), 3 * nodes
+    x = torch.randn(n, H * G * D, generator=gen).cuda()
+    proj = [[(torch.randn(H * G * D, w, generator=gen) * 0.1).cuda() for w in (H * G * D, H * D, H * D)] for _ in range(layers)]
+    mask = attn.tree_mask([list(range(-1, nodes - 1))] * 3).cuda()            # a chain: each node sees those before it
+    seqs, first, one = pages.ids([0, 1, 2]), pages.ids(lens), pages.ids([nodes] * 3)
+    cu = dev([0, nodes, 2 * nodes, 3 * nodes])
+    q = torch.zeros(n, H * G, D, device="cuda")
+    trees = [attn.Tree(kvc, h, q, cu, dev([0, 1, 2]), mask=mask, max_nodes=nodes, layer=l) for l in range(layers)]
+    zero = torch.zeros(1, H, n, device="cuda")
+    kept = []
+
+    def step():
+        y = x
+        h.reserve(seqs, one)
+        for l in range(layers):
+            q.copy_((y @ proj[l][0]).view(n, H * G, D))
+            rows = [(y @ p).half().view(1, n, H * D) for p in proj[l][1:]]
+            kept.append(rows)
+            h.write(seqs, first, one, *(r.view(torch.uint8) for r in rows), zero, layer=l)
+            y = trees[l].run().flatten(1)
+        return y
+
+    for p in proj[0]:
+        x @ p                                              # cuBLAS sets itself up outside the capture
+    before = [t.clone() for t in (c.K, c.V, c.beta)]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step()
+    g.replay()
+    h.check()
+    assert c.seq_len.tolist()[:3] == [m + nodes for m in lens]
+    y = x
+    for l in range(layers):
+        ql = (y @ proj[l][0]).view(n, H * G, D)
+        k, v, b = h.read(seqs, first, one, layer=l)
+        torch.cuda.synchronize()
+        assert torch.equal(k, kept[l][0].view(torch.uint8)) and torch.equal(v, kept[l][1].view(torch.uint8)) and torch.equal(b, zero)
+
+        def see(i, m, rows):
+            s = torch.ones(m, rows, dtype=torch.bool)
+            s[:, rows - m:] = torch.tril(torch.ones(m, m, dtype=torch.bool))
+            return s
+        out, _ = c.attend(ql, cu.tolist(), [0, 1, 2], see, D ** -0.5, l)
+        # scores within +-60 and |V| < 16, as above: 2 (60 2^-20 + 2^-21) 16
+        assert float((trees[l].out.double() - out).abs().max()) < 2e-3
+        y = trees[l].out.flatten(1)
+    # nothing else was written: rows of the other tokens and layers are as before
+    new = torch.cat([c.rows(s)[m:] for s, m in enumerate(lens)])
+    old = torch.ones(c.K.shape[1], dtype=torch.bool, device="cuda")
+    old[new] = False
+    assert torch.equal(c.K[:, old], before[0][:, old]) and torch.equal(c.V[:, old], before[1][:, old])
+    for bad in (-1, layers):
+        with pytest.raises(ValueError):
+            h.write(seqs, first, one, layer=bad)
+        with pytest.raises(ValueError):
+            h.read(seqs, first, one, layer=bad)
+    with pytest.raises(ValueError):
+        h.write(seqs, first, one, torch.zeros(layers, n, c.K.shape[2], dtype=torch.uint8, device="cuda"), layer=0)
+
+
 def test_launches_are_counted(kvc):
     c = R.Cache([30], H, D, D, R.Q8_0, R.Q8_0, PAGE)
     h = c.handle(kvc)
