@@ -500,7 +500,7 @@ __global__ void __launch_bounds__(32 * MAXW, 1) k_tree_mma(const __grid_constant
                 top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
                 // largest value of the row in [2^13, 2^14): both pieces normal numbers
                 if (top > 0.0f && top < INFINITY) {
-                    const int e = min(max(13 - ilogbf(top), -100), 100);
+                    const int e = min(13 - ilogbf(top), 100);
                     up = scalbnf(1.0f, e);
                     m = a.scale * scalbnf(1.0f, -e);
                 }

@@ -51,6 +51,10 @@ constexpr int MAX_SEGS = 64;
 constexpr uint32_t POLLS = 1u << 22;            // bound of every wait
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int P_SHIFT = 10;
+// S is the product of the row's q / 2^u and the key's k / 2^e, e >= -15: with F32 queries 2^u S could pass fp32's range
+// where q.k does not, so 2^u comes over this power of two and f times it.
+template <int QP>
+constexpr int HEADROOM = QP == 2 ? 16 : 0;
 constexpr int HIDDEN = -200 * (1 << 23);        // exponent bits of a row that counts for nothing
 // registers per thread of the warp groups; their sum x 128 is what the block is launched with
 constexpr int REG_SOFTMAX = 192, REG_PRODUCE = 88, REG_MMA = 40, REG_LAUNCH = 128;
@@ -78,7 +82,7 @@ struct segment {
 
 // Per key of a tile. Eight tiles deep: when tile i is filled, tile i - 5 and those before it have been read.
 struct alignas(16) tile_info {      // read four at a time
-    float f[TN];                // factor of S: scale 2^e
+    float f[TN];                // factor of S: scale 2^(e + HEADROOM)
     float b[TN];                // beta, or -inf
     int e[TN];                  // exponent of the V row << 23, or HIDDEN
 };
@@ -91,7 +95,7 @@ struct shared {
                                     // of the tile that are taken value by value
     segment segs[MAX_SEGS];
     int rows[2][TN];            // pool rows of a tile
-    float mul[TM];              // power of two that a query row was divided by
+    float mul[TM];              // power of two that a query row was divided by, over 2^HEADROOM
     float jm[TM], jl[TM];
     tile_info info[8];
 };
@@ -351,10 +355,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                     float down = 1.0f;
                     // largest value of the row in [2^13, 2^14): both pieces normal numbers
                     if (top > 0.0f && top < INFINITY) {
-                        const int e = min(max(13 - ilogbf(top), -100), 100);
+                        const int e = min(13 - ilogbf(top), 100);
                         up = scalbnf(1.0f, e);
                         down = scalbnf(1.0f, -e);
                     }
+                    down *= 1.0f / (1 << HEADROOM<QP>);
                     if (part == 0) X.mul[row] = down;
                 }
 #pragma unroll
@@ -694,7 +699,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                         tile_info & I = X.info[i & 7];
                         const bool live = bias != -INFINITY;
                         X.rows[i & 1][key] = live ? row : -1;
-                        I.f[key] = a.scale;
+                        I.f[key] = a.scale * (1 << HEADROOM<QP>);
                         I.b[key] = bias;
                         I.e[key] = live ? 0 : HIDDEN;
                     }
@@ -818,7 +823,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_tree_tc(const __grid_constant__ 
                         if (part == 0) {
                             tile_info & I = X.info[i & 7];
                             if (side == 0) {
-                                I.f[key] = a.scale * scalbnf(1.0f, e);
+                                I.f[key] = a.scale * scalbnf(1.0f, e + HEADROOM<QP>);
                                 I.b[key] = live ? bias_now : -INFINITY;
                             } else {
                                 I.e[key] = live ? e * (1 << 23) : HIDDEN;

@@ -240,6 +240,23 @@ def test_tree_large_and_small_scales(kvc):
             tree_check(kvc, lens=[100], nodes=[1], kt=kind, vt=kind, qt=torch.float32, edit=edit, seed=11)
 
 
+@pytest.mark.parametrize("kind", [R.F32, R.F16, R.Q8_0])
+@pytest.mark.parametrize("nodes", [[1, 2], [40, 2]])
+def test_tree_huge_queries(kvc, kind, nodes):
+    """F32 queries up to 2^120: scores of up to 2^122, of which the largest takes everything."""
+    def edit(c, q):
+        q[0] *= 2.0 ** 118
+    c, q, t, (out, lse) = tree_case(kvc, lens=[90, 33], nodes=nodes, kt=kind, vt=kind, qt=torch.float32, edit=edit)
+    t.run()
+    torch.cuda.synchronize()
+    # one key's values alone: no rounding but the pieces' (2^-21); the score itself is off by 2^-21 of sum |q||k|, which is
+    # some 8 times its largest value here, and its product with the scale by 2^-23
+    v = float(R.decode(c.V[0], kind).abs().max())
+    assert float((t.out[0].double() - out[0]).abs().max()) <= 2.0 ** -20 * v
+    assert float((t.lse[0].double() / lse[0] - 1).abs().max()) < 2.0 ** -17
+    assert float((t.out[1:].double() - out[1:]).abs().max()) < 1e-4
+
+
 def test_tree_bad_pages_and_slots(kvc):
     """Entries outside the pool count as no rows; an id outside the cache as an empty sequence."""
     for hkv, page, kt in ((2, 16, R.Q8_0), (3, 16, R.Q8_0), (2, 16, R.F32), (2, 5, R.F16)):
