@@ -20,7 +20,7 @@ class PageCacheDesc(Structure):
 
 def ids(values):
     """A host list of sequence ids or counts, as the calls take it (built once, passed often)."""
-    if isinstance(values, ctypes.Array):
+    if isinstance(values, ctypes.Array) and values._type_ is c_int:
         return values
     values = [int(v) for v in values]
     return (c_int * len(values))(*values)

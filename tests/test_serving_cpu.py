@@ -114,6 +114,15 @@ def test_page_call_refusals(kvc):
     assert L.kvc_pages_copy(ref, None, None, 0, None) == ok_code()
 
 
+def test_ids_are_ints():
+    """Host lists of any integer type become C ints; only an array of these is passed on as it is."""
+    given = (ctypes.c_int * 3)(1, 2, 3)
+    assert pages.ids(given) is given
+    for values in ([1, 2, 3], (ctypes.c_int64 * 3)(1, 2, 3), np.array([1, 2, 3]), torch.tensor([1, 2, 3]), (1, 2, 3)):
+        got = pages.ids(values)
+        assert isinstance(got, ctypes.Array) and got._type_ is ctypes.c_int and list(got) == [1, 2, 3]
+
+
 def tree_desc(c, **kw):
     d = dict(q=c.K, out=c.K, lse=None, cu=c.K, seqs=c.K, mask=None, q_type=1, mask_words=0, n_seqs=1, total=1, max_nodes=1,
              n_head=4, layer=0, scale=0.1, q_stride=4 * 64)
