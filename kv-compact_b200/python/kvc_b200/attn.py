@@ -111,11 +111,13 @@ class Tree:
             out, "out", (q.dtype,), dev, (total, h, c.d_v))
         self.lse = None if lse is False else torch.empty(total, h, device=dev) if lse is None else need(
             lse, "lse", (torch.float32,), dev, (total, h))
+        # a mask without words shows no node's own row; an empty tensor's null pointer would be no mask at all
+        at = None if mask is None else mask.data_ptr() or cu.data_ptr()
         lib = fns["_lib"]
         self.fn, self.index, self.cache = lib.kvc_attn_tree, dev.index, cache
         self._keep = (q, cu, seqs, mask)
         self.desc = TreeDesc(q.data_ptr(), self.out.data_ptr(), self.lse.data_ptr() if self.lse is not None else None,
-                             cu.data_ptr(), seqs.data_ptr(), mask.data_ptr() if mask is not None else None,
+                             cu.data_ptr(), seqs.data_ptr(), at,
                              _kind(q.dtype), mask.shape[1] if mask is not None else 0, n, total, max_nodes, h, layer,
                              c.d_k ** -0.5 if scale is None else scale, q.stride(0) if total > 1 else h * c.d_k)
         self.ref = ctypes.addressof(self.desc)

@@ -172,6 +172,20 @@ def test_tree_without_mask_sees_all(kvc):
 
 
 @pytest.mark.parametrize("kind", [R.F32, R.F16, R.Q8_0])
+@pytest.mark.parametrize("nodes", [[1, 3], [40, 1]])
+def test_tree_mask_without_words(kvc, kind, nodes):
+    """Shows no node's own row, as a mask of zeros does."""
+    c, q, t, (out, lse) = tree_case(kvc, lens=[40, 3], nodes=nodes, kt=kind, vt=kind, qt=torch.float32, mask="none")
+    none = torch.zeros(sum(nodes), 0, dtype=torch.int32, device="cuda")
+    u = attn.Tree(kvc, c.handle(kvc), q, t._keep[1], t._keep[2], mask=none, max_nodes=max(nodes), scale=64 ** -0.5)
+    u.run()
+    t.run()
+    torch.cuda.synchronize()
+    assert torch.equal(u.out, t.out) and torch.equal(u.lse, t.lse)
+    assert float((u.out.double() - out).abs().max()) < 1e-4
+
+
+@pytest.mark.parametrize("kind", [R.F32, R.F16, R.Q8_0])
 def test_tree_rows_that_see_nothing(kvc, kind):
     """No cached rows and an empty mask, or beta of -inf on every row: output 0, log-sum-exp -inf."""
     t = tree_check(kvc, lens=[0, 20], nodes=[3, 2], kt=kind, vt=kind, mask="none")
