@@ -27,7 +27,8 @@
  * n_pages and max_pages times page_size are at most 2^31 - 1 - 65536.
  * Calls with n = 0 do nothing. Return codes: 0; -1 a null argument; -2 bad
  * counts, ids or a repeated destination; -4 a row size that does not match;
- * -10 no sm_100 device; -12 CUDA error; -13 a shape outside the limits or a
+ * -10 no sm_100 device; -12 CUDA error; -13 a shape outside the limits, an
+ * array that is not aligned to its elements (workspaces: to 16 bytes) or a
  * workspace that is too small. The current device must be the cache's.
  */
 #ifndef KVC_PAGES_H

@@ -21,6 +21,7 @@ KVC_EXPORT int kvc_attn_prompt(const kvc_prompt_desc * t, void * stream) {
     const int size = t->type == KV_TYPE_F32 ? 4 : 2;
     for (const void * p : {t->q, t->k, t->v, (const void *)t->out})
         if ((uintptr_t)p % size) return KVC_ERR_SHAPE;
+    if (!kvc_words_aligned({t->lse, t->cu_q, t->cu_k})) return KVC_ERR_SHAPE;
     if ((long long)t->total_q * t->n_head > INT_MAX) return KVC_ERR_SHAPE;
     const int sms = kvc_serve_device();
     if (sms < 0) return sms;

@@ -35,6 +35,7 @@ int make_plan(const kvc_page_cache * c, const kvc_tree_desc * t, int sms, tree_p
     }
     const uintptr_t qa = t->q_type == KV_TYPE_F32 ? 3 : 1;
     if (((uintptr_t)t->q & qa) || ((uintptr_t)t->out & qa)) return KVC_ERR_SHAPE;
+    if (!kvc_words_aligned({t->lse, t->cu, t->seqs, t->mask})) return KVC_ERR_SHAPE;
     if ((long long)t->total * t->n_head > INT_MAX || (long long)t->max_nodes * t->n_head > INT_MAX) return KVC_ERR_SHAPE;
     if (sms < 0) return sms;                             // no device: after the argument checks
     kvc_attn_args & a = p->a;

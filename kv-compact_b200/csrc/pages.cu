@@ -66,6 +66,7 @@ int kvc_check_cache(const kvc_page_cache * c) {
     // the widest element of the type decides how rows may be addressed
     const uintptr_t ka = c->k_type == KV_TYPE_F32 ? 4 : 2, va = c->v_type == KV_TYPE_F32 ? 4 : 2;
     if ((uintptr_t)c->K % ka || (uintptr_t)c->V % va) return KVC_ERR_SHAPE;
+    if (!kvc_words_aligned({c->beta, c->page_table, c->seq_len, c->ref_count, c->status})) return KVC_ERR_SHAPE;
     return KVC_OK;
 }
 
@@ -691,6 +692,7 @@ int packed_move(int mode, const kvc_page_cache * cache, const int * seqs, const 
     long long total;
     if ((rc = check_spans(cache, seqs, first, count, n, &ids, &span, &total))) return rc;
     if (b_rows && !cache->beta) return KVC_ERR_NULL;
+    if (!kvc_words_aligned({b_rows})) return KVC_ERR_SHAPE;
     if (mode == MV_WRITE)               // two entries that write one row would race
         for (int i = 0; i < n; i++)
             for (int j = 0; j < i; j++)
@@ -757,6 +759,7 @@ KVC_EXPORT int kvc_pages_copy(const kvc_page_cache * cache, const int * src, con
     if (rc) return rc;
     if (n < 0 || (long long)n * cache->page_size > INT_MAX - 65536) return KVC_ERR_DIMS;
     if (n > 0 && (!src || !dst)) return KVC_ERR_NULL;
+    if (!kvc_words_aligned({src, dst})) return KVC_ERR_SHAPE;
     const int sms = kvc_serve_device();
     if (sms < 0) return sms;
     move_args a{};
@@ -805,6 +808,7 @@ KVC_EXPORT int kvc_pages_compact(const kvc_page_cache * cache, const int * src, 
     if (keep_ld < 0) return KVC_ERR_DIMS;
     if (n > 0 && (!base || !keep_n || (!keep && keep_ld > 0))) return KVC_ERR_NULL;
     if (beta_rows && !cache->beta) return KVC_ERR_NULL;
+    if (!kvc_words_aligned({base, keep_n, keep, beta_rows})) return KVC_ERR_SHAPE;
     if ((rc = check_ws(cache, ws, ws_bytes))) return rc;
     const int sms = kvc_serve_device();
     if (sms < 0) return sms;

@@ -6,12 +6,20 @@
 #include "kvc_internal.h"
 
 #include <atomic>
+#include <initializer_list>
 
 // The current device, checked once per device: >= 0 SM count, or a negative
 // error code when it cannot run the library's kernels.
 int kvc_serve_device();
 // Kernels launched by the serving operators (part of kvc_launch_count).
 extern std::atomic<uint64_t> g_serve_launches;
+
+// Whether arrays of 32-bit numbers lie on 4-byte boundaries (a kernel that reads others faults).
+inline bool kvc_words_aligned(std::initializer_list<const void *> arrays) {
+    for (const void * p : arrays)
+        if ((uintptr_t)p & 3) return false;
+    return true;
+}
 
 // Argument checks of a page cache (null pointers, counts, row sizes).
 int kvc_check_cache(const kvc_page_cache * c);

@@ -53,6 +53,40 @@ BAD_CACHES = [
 ]
 
 
+@pytest.mark.parametrize("field", ["K", "V", "beta", "page_table", "seq_len", "ref_count", "status"])
+def test_cache_arrays_off_their_elements(kvc, field):
+    c = cache_desc(k_type=0, k_row_bytes=512, v_type=0, v_row_bytes=512)
+    at = c.K
+    setattr(c, field, at + 2)
+    one = pages.ids([0])
+    assert kvc["_lib"].kvc_pages_free(ctypes.addressof(c), one, 1, at, 1 << 20, None) == -13
+    assert kvc["_lib"].kvc_pages_workspace(ctypes.addressof(c)) == 0
+
+
+def test_call_arrays_off_their_elements(kvc):
+    L, c = kvc["_lib"], cache_desc(beta=None)
+    c.beta = c.K
+    ref, at, odd, one = ctypes.addressof(c), c.K, c.K + 2, pages.ids([0])
+    ws = (at, L.kvc_pages_workspace(ref))
+    assert ws[1] > 0
+    assert L.kvc_pages_copy(ref, odd, at, 1, None) == -13 and L.kvc_pages_copy(ref, at, odd, 1, None) == -13
+    for call in (L.kvc_pages_write, L.kvc_pages_read):
+        assert call(ref, one, one, pages.ids([1]), 1, None, None, odd, None) == -13
+    good = dict(base=at, keep_n=at, keep=at, beta=at)
+    for name in good:
+        a = dict(good, **{name: odd})
+        assert L.kvc_pages_compact(ref, one, one, 1, a["base"], a["keep_n"], a["keep"], 4, 0, None, a["beta"], *ws, None) == -13
+    for name in ("lse", "cu", "seqs", "mask"):
+        t = tree_desc(c, **{name: odd})
+        assert L.kvc_attn_tree(ref, ctypes.addressof(t), None, 0, None) == -13
+    for name in ("lse", "cu_q", "cu_k"):
+        d = dict(q=4096, k=4096, v=4096, out=4096, lse=4096, cu_q=4096, cu_k=4096, type=1, n_seqs=1, total_q=4, total_k=4,
+                 n_head=4, n_head_kv=2, d_k=64, d_v=64, causal=1, scale=0.1, q_stride=256, q_head_stride=64, k_stride=128,
+                 k_head_stride=64, v_stride=128, v_head_stride=64)
+        p = attn.PromptDesc(**dict(d, **{name: 4098}))
+        assert L.kvc_attn_prompt(ctypes.addressof(p), None) == -13
+
+
 @pytest.mark.parametrize("kw,code", BAD_CACHES)
 def test_cache_refusals(kvc, kw, code):
     c, L = cache_desc(**kw), kvc["_lib"]
