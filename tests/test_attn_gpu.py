@@ -166,6 +166,57 @@ def test_tree_many_sequences(kvc):
     tree_check(kvc, lens=lens, nodes=[1] * 150, hkv=4, g=2, kt=R.Q8_0, vt=R.Q8_0, page=32)
 
 
+def attend_entries(c, q, cu, bits, scale):
+    """The definition, an entry at a time over all heads."""
+    H, g = c.hkv, q.shape[1] // c.hkv
+    out, lse = [], []
+    for i in range(len(cu) - 1):
+        rows, m = c.rows(i), cu[i + 1] - cu[i]
+        K, V = (R.decode(x[0][rows], k).view(len(rows), H, -1) for x, k in ((c.K, c.kt), (c.V, c.vt)))
+        x = torch.einsum("mhgd,nhd->mhgn", q[cu[i]:cu[i + 1]].double().view(m, H, g, -1), K) * scale
+        if c.beta is not None:
+            x = x + c.beta[0, rows // c.page, :, rows % c.page].double().t()[None, :, None]
+        see = torch.ones(m, len(rows), dtype=torch.bool)
+        see[:, len(rows) - m:] = torch.tensor([[bool((int(bits[cu[i] + a, b // 32]) >> (b % 32)) & 1) for b in range(m)]
+                                               for a in range(m)])
+        x = x.masked_fill(~see.cuda()[:, None, None], -math.inf)
+        lse.append(torch.logsumexp(x, -1).flatten(1))
+        out.append(torch.einsum("mhgn,nhd->mhgd", torch.softmax(x, -1), V).flatten(1, 2))
+    return torch.cat(out), torch.cat(lse)
+
+
+@pytest.mark.parametrize("entries", [64, 65, 128, 129])
+@pytest.mark.parametrize("hkv,g,d,kind,page,most", [(296, 1, 256, R.F16, 8, 1), (148, 1, 256, R.F16, 8, 1), (296, 1, 256, R.F16, 5, 1),
+                                                    (160, 4, 64, R.F16, 16, 40), (160, 2, 64, R.Q8_0, 8, 70)])
+def test_tree_many_entries_per_worker(kvc, hkv, g, d, kind, page, most, entries):
+    """More entries in a CTA's stretch than its list of pieces holds: with so many heads one CTA (two of 148 heads) has all
+    entries of its heads. `most` > 32: the kernel for many query rows, whose entries of several tiles and row blocks are
+    among the others."""
+    lens = [(i * 37) % (8 if most == 1 else 100) for i in range(entries)]
+    nodes = [most if i in (3, entries - 1) else 1 + i % min(2, most) for i in range(entries)]
+    c = R.Cache([a + b for a, b in zip(lens, nodes)], hkv, d, d, kind, kind, page, beta=True, seed=entries)
+    gen = torch.Generator().manual_seed(entries)
+    q = torch.randn(sum(nodes), hkv * g, d, generator=gen).cuda().half()
+    cu = [sum(nodes[:i]) for i in range(entries + 1)]
+    bits = attn.tree_mask([[int(torch.randint(-1, i, (1,), generator=gen)) if i else -1 for i in range(n)] for n in nodes])
+    dev = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    t = attn.Tree(kvc, c.handle(kvc), q, dev(cu), dev(list(range(entries))), mask=bits.cuda(), max_nodes=most, scale=d ** -0.5)
+    t.out.fill_(7.0)
+    t.run()
+    out, lse = attend_entries(c, q, cu, bits, d ** -0.5)
+    used = torch.cat([c.rows(i) for i in range(entries)])
+    # |q||k| per head, row by row of q: A of bounds() without a product over all heads
+    A = float((q.double().norm(dim=-1).max() * R.decode(c.K[0][used], kind).view(-1, hkv, d).norm(dim=-1).max())) * d ** -0.5
+    v = float(R.decode(c.V[0][used], kind).abs().max())
+    e = A * 2.0 ** -21 + (A + float(c.beta.abs().max())) * 2.0 ** -22 + 2.0 ** -21
+    check(t.out, out, 2 * e * v + 2.0 ** -21 * v + 2 * 2.0 ** -11 * v, "out")
+    check(t.lse, lse, 2 * e + 2.0 ** -21, "lse")
+    first = t.out.clone()
+    t.run()
+    torch.cuda.synchronize()
+    assert torch.equal(first, t.out) and int(c.status) == 0
+
+
 def test_tree_without_mask_sees_all(kvc):
     tree_check(kvc, lens=[40, 3], nodes=[4, 2], mask=None)
     tree_check(kvc, lens=[40, 3], nodes=[4, 2], mask=None, kt=R.F32, vt=R.F32)

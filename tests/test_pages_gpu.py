@@ -322,6 +322,91 @@ def test_copy_pages(kvc):
     m.same(c)
 
 
+@pytest.mark.parametrize("page", [1, 3, 16, 70])
+@pytest.mark.parametrize("kt,vt,hkv,d", [(R.F16, R.F16, 2, 64), (R.Q8_0, R.F32, 8, 64), (R.F32, R.Q4_0, 32, 256)])
+def test_copy_pages_of_16_byte_pieces(kvc, page, kt, vt, hkv, d):
+    """Rows that go by bulk copies (the last ones one per CTA): pairs outside the pool and onto themselves among them."""
+    c = cache([40], page=page, hkv=hkv, d=d, kt=kt, vt=vt)
+    assert c.K.shape[2] % 16 == 0 and c.V.shape[2] % 16 == 0
+    m, h = Model(c), c.handle(kvc)
+    free = (c.ref == 0).nonzero()[:, 0].tolist()
+    used = [p for p in c.table[0].tolist() if p >= 0]
+    pairs = list(zip(used, free[:-3])) + [(-1, free[-1]), (c.n_pages, free[-2]), (used[0], -5), (used[0], c.n_pages), (free[-3],) * 2]
+    h.copy(dev([a for a, _ in pairs]), dev([b for _, b in pairs]))
+    for a, b in zip(used, free[:-3]):
+        for store in (m.K, m.V):
+            store[:, b * page:(b + 1) * page] = store[:, a * page:(a + 1) * page]
+        m.beta[:, b] = m.beta[:, a]
+    m.same(c)
+
+
+@pytest.mark.parametrize("page", [1, 5, 16])
+@pytest.mark.parametrize("parts", [(1, 1, 1), (1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 0, 1), (0, 1, 1)])
+def test_write_and_read_of_16_byte_pieces(kvc, page, parts):
+    """Some of the arrays alone, of all layers and of one, by bulk copies: what is left out stays as it was."""
+    c = R.Cache([90, 18, 4], 8, 64, 64, R.Q8_0, R.F32, page, layers=2, beta=True, spare=20)
+    m, h = Model(c), c.handle(kvc)
+    g = torch.Generator().manual_seed(2)
+    seqs, first, count = [1, 0, 1, 2], [0, 7, 15, 3], [5, 70, 10, 0]
+    n, at = sum(count), 0
+    rows = [torch.randint(0, 256, (2, n, c.K.shape[2]), generator=g).to(torch.uint8),
+            torch.randint(0, 256, (2, n, c.V.shape[2]), generator=g).to(torch.uint8), torch.randn(2, 8, n, generator=g)]
+    assert all(r.shape[2] % 16 == 0 for r in rows[:2])
+    for layer in (None, 1, 0):
+        part = slice(None) if layer is None else slice(layer, layer + 1)
+        given = [r[part].contiguous().cuda() if p else None for r, p in zip(rows, parts)]
+        h.write(seqs, first, count, *given, layer=layer)
+        at = 0
+        for s, f, cnt in zip(seqs, first, count):
+            for i in range(cnt):
+                if f + i < m.len[s]:
+                    r = m.at(s, f + i)
+                    if parts[0]:
+                        m.K[part, r] = rows[0][part, at]
+                    if parts[1]:
+                        m.V[part, r] = rows[1][part, at]
+                    if parts[2]:
+                        m.beta[part, r // page, :, r % page] = rows[2][part][:, :, at]
+                at += 1
+        m.same(c)
+        out = [torch.full_like(r[part], 7).cuda() if p else None for r, p in zip(rows, parts)]
+        want = [None if o is None else o.cpu() for o in out]
+        h._rows("kvc_pages_read", seqs, first, count, *out, layer)
+        at = 0
+        for s, f, cnt in zip(seqs, first, count):
+            for i in range(cnt):
+                if f + i < m.len[s]:
+                    r = m.at(s, f + i)
+                    for w, store in ((want[0], m.K), (want[1], m.V)):
+                        if w is not None:
+                            w[:, at] = store[part, r]
+                    if want[2] is not None:
+                        want[2][:, :, at] = m.beta[part, r // page, :, r % page]
+                at += 1
+        torch.cuda.synchronize()
+        for o, w in zip(out, want):
+            assert o is None or torch.equal(o.cpu(), w)
+        rows = [r.flip(1) if i < 2 else r + 1 for i, r in enumerate(rows)]
+
+
+@pytest.mark.parametrize("page", [1, 7, 64])
+def test_compact_of_16_byte_pieces(kvc, page):
+    """Refitted rows and beta with rows that go by bulk copies, more of them than a CTA takes at a time."""
+    c = R.Cache([300, 90], 8, 32, 32, R.F16, R.Q8_0, page, layers=2, beta=True, spare=800, slots=8)
+    m, h = Model(c), c.handle(kvc)
+    g = torch.Generator().manual_seed(page)
+    ld = 250
+    keep = torch.stack([torch.stack([torch.randperm(n, generator=g)[:ld].sort()[0] if n >= ld else
+                                     torch.arange(ld) % n for n in (300, 90)]) for _ in range(2)]).int()
+    v = torch.randint(0, 256, (2, 2, ld, c.V.shape[2]), generator=g).to(torch.uint8)
+    b = torch.randn(2, 2, 8, ld, generator=g)
+    assert c.K.shape[2] % 16 == 0 and c.V.shape[2] % 16 == 0
+    for src, dst, base, given in (([0, 1], [2, 3], [5, 0], (v, b)), ([2, 3], [2, 3], [0, 17], (None, None)), ([0, 1], [0, 1], [0, 3], (v, None))):
+        h.compact(src, dst, keep.cuda(), dev([ld, 60]), dev(base), *(None if x is None else x.cuda() for x in given))
+        m.compact(src, dst, keep, [ld, 60], base, *given)
+        m.same(c)
+
+
 def test_in_a_graph_and_on_a_stream(kvc):
     c = cache([21, 16], page=8)
     m, h = Model(c), c.handle(kvc)
