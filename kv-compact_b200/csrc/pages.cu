@@ -113,24 +113,26 @@ cache_dev on_device(const kvc_page_cache * c) {
 }
 
 // Pages of `rows` rows (rows + page may pass 2^31).
-__device__ __forceinline__ int pages_of(int rows, int page) { return rows / page + (rows % page != 0); }
+__device__ __forceinline__ int pages_of(int rows, kvc_divisor page) { return rows > 0 ? (int)page.div((uint32_t)rows - 1u) + 1 : 0; }
 
 constexpr int PLAN_THREADS = 1024;
 constexpr int PLAN_PER = 16;          // counts per thread and scan step
 
-__device__ __forceinline__ int warp_scan(int v, int lane) {          // inclusive
+template <typename T>
+__device__ __forceinline__ T warp_scan(T v, int lane) {              // inclusive
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(~0u, v, o);
+        const T u = __shfl_up_sync(~0u, v, o);
         if (lane >= o) v += u;
     }
     return v;
 }
 
 // Exclusive scan over the CTA; every thread gets its prefix and the total.
-__device__ int block_scan(int v, int * sums, int * total) {
+template <typename T>
+__device__ T block_scan(T v, T * sums, T * total) {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int inc = warp_scan(v, lane);
+    const T inc = warp_scan(v, lane);
     __syncthreads();
     if (lane == 31) sums[w] = inc;
     __syncthreads();
@@ -148,49 +150,42 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_plan(cache_dev c, const __grid
                                                        const __grid_constant__ plan_ids counts, int keep_ld,
                                                        int * __restrict__ ws) {
     __shared__ int sums[32];
-    __shared__ int bad;
-    __shared__ unsigned long long asked;                 // new pages of all entries: up to 256 times 2^31
+    __shared__ long long needs[32];
     const int t = threadIdx.x;
-    if (t == 0) {
-        bad = 0;
-        asked = 0;
-    }
-    __syncthreads();
+    bool bad = false;
     plan_item it{};
     if (t < ids.n) {
         const int cap = c.max_pages * c.page;
         const int len = min(max(c.seq_len[ids.src[t]], 0), cap);
         long long length = len;
         if (op == OP_RESERVE) {
-            it.whole = pages_of(len, c.page);
+            it.whole = pages_of(len, c.by_page);
             length = (long long)len + counts.src[t];
         } else if (op == OP_FORK) {
-            it.whole = len / c.page;
+            it.whole = (int)c.by_page.div((uint32_t)len);
             it.head = len - it.whole * c.page;
         } else {
             const int b = min(max(base[t], 0), len);
             it.kept = min(max(keep_n[t], 0), keep_ld);
-            it.whole = b / c.page;
+            it.whole = (int)c.by_page.div((uint32_t)b);
             it.head = b - it.whole * c.page;
             length = (long long)b + it.kept;
         }
         if (length > cap) {
-            atomicOr(&bad, 1);
+            bad = true;
         } else {
             it.length = (int)length;
-            it.need = max(pages_of(it.length, c.page) - it.whole, 0);
-            atomicAdd(&asked, (unsigned long long)it.need);
+            it.need = max(pages_of(it.length, c.by_page) - it.whole, 0);
         }
     }
-    int total;
-    it.first = block_scan(t < ids.n ? it.need : 0, sums, &total);
+    const bool too_long = __syncthreads_or(bad);
+    long long total;                                     // of all entries: up to 256 times 2^31
+    it.first = (int)block_scan<long long>(t < ids.n ? it.need : 0, needs, &total);
     plan_item * items = reinterpret_cast<plan_item *>(reinterpret_cast<char *>(ws) + WS_HEAD);
     if (t < ids.n) items[t] = it;
     int * fresh = reinterpret_cast<int *>(reinterpret_cast<char *>(ws) + WS_ITEMS);
     int found = 0;
-    __syncthreads();
-    const bool too_long = bad != 0, too_many = asked > (unsigned long long)c.n_pages;      // beyond that the sums may have wrapped
-    if (!too_long && !too_many) {
+    if (!too_long && total <= c.n_pages) {
         const bool wide = ((uintptr_t)c.ref & 15) == 0;
         for (int at = 0; found < total && at < c.n_pages; at += PLAN_THREADS * PLAN_PER) {
             const int p0 = at + t * PLAN_PER;
@@ -221,7 +216,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_plan(cache_dev c, const __grid
         }
     }
     if (t == 0) {
-        const bool ok = !too_long && !too_many && found >= total;
+        const bool ok = !too_long && found >= total;
         ws[0] = ok;
         if (!ok) *c.status = too_long ? KVC_ERR_SHAPE : KVC_ERR_OOM;
     }

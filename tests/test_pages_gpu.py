@@ -235,6 +235,25 @@ def test_more_pages_asked_for_than_32_bits_count(kvc, add):
     assert bool((table[:, :8] == -1).all())
 
 
+@pytest.mark.parametrize("at", [0, 31, 32, 100, 255])
+def test_one_entry_of_many_that_does_not_fit(kvc, at):
+    """A table row that is too short in any of 256 entries, or too few pages for all: nothing changes."""
+    c = cache([5] * 256, page=4, slots=256, spare=300, hkv=1, d=32)
+    m, h = Model(c), c.handle(kvc)
+    add = [4] * 256
+    add[at] = 48 * 4
+    for _ in range(20):
+        h.reserve(list(range(256)), add)
+        torch.cuda.synchronize()
+        assert int(c.status) == -13
+        c.status.zero_()
+    m.same(c)
+    h.reserve(list(range(256)), [9] * 256)             # 512 pages of 300
+    m.reserve(list(range(256)), [9] * 256)
+    assert m.status == -11
+    m.same(c)
+
+
 @pytest.mark.parametrize("n_pages", [1, 15, 16, 17, 5000, 40001])
 def test_lowest_free_pages(kvc, n_pages):
     """Pools around and beyond one step of the scan, with few free pages and far ones."""
