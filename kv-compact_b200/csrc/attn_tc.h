@@ -45,12 +45,14 @@ __device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, u
         "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n"
         :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc));
 }
-__device__ __forceinline__ void commit_mma(uint64_t * mbar) {
+// `go` false in that lane: nothing is committed (a warp whose lanes may differ in it takes no branch on it).
+__device__ __forceinline__ void commit_mma(uint64_t * mbar, bool go = true) {
     asm volatile(
         "{\n\t.reg .pred q;\n\t"
         "elect.sync _|q, 0xffffffff;\n\t"
+        "setp.ne.and.b32 q, %1, 0, q;\n\t"
         "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n"
-        :: "r"(smem_u32(mbar)) : "memory");
+        :: "r"(smem_u32(mbar)), "r"((uint32_t)go) : "memory");
 }
 
 #define KVC_R8(r, o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7])
