@@ -11,8 +11,8 @@
 // steps, and work is dealt in smaller pieces), or, for long sequences that fill
 // the machine several times, in one CTA, which then loads keys and values once
 // for both (NT = 2). 32 query heads on 8 KV heads, 128 values, us with one tile
-// in a CTA / two: ten packed prompts of 1 to 2,047 tokens 87 / 93, 812 tokens on
-// 10,333 keys 111 / 124, one prompt of 8,192 tokens 508 / 501.
+// in a CTA / two, in a loop: ten packed prompts of 1 to 2,047 tokens 95 / 96, 812
+// tokens on 10,333 keys 115 / 123, one prompt of 8,192 tokens 589 / 576.
 //
 //   warps 0-3 (, 4-7)  softmax of tile 0 (, 1): a thread owns a row. S comes
 //                      from TMEM, P goes back as fp16 over S's columns, from
@@ -23,12 +23,15 @@
 //   then one warp      TMA: Q once, then K and V through one ring of slots
 //   and one            MMA issue
 //
-// Rows, statistics and O are 32-bit; P is rounded to fp16 (2^-12 relative, as
-// the output is). Bound by the exponentials (16 per clock and SM against 4,096
+// Rows, statistics and O are 32-bit; P is rounded to fp16 once (2^-11 relative, as
+// the output is; l is the sum of the unrounded values): a second piece of P would be
+// half as many products again. Against 64 bits the outputs' error grows from 1.9e-4
+// (their own rounding) to 2.5e-4. Bound by the exponentials (16 per clock and SM against 4,096
 // multiply-adds) and the tensor cores about equally at d = 128: a tile's step is
 // a chain of softmax (about 2,350 cycles) and products (78 cycles for each of 16
 // instructions), and two tiles fill an SM's issue slots and tensor cores by turns.
-// The 8,192-token prompt runs at 1,100 TFLOP/s, 65 % of a dense product's rate.
+// The 8,192-token prompt takes 496 us in bursts, 1,100 TFLOP/s or 65 % of a dense
+// product's rate, and 574 in a loop of seconds, 960 TFLOP/s, 68 % of the sustained rate.
 // Steps of 64 keys (723 us), two threads per row (513) and exponentials that do
 // not wait for the step's maximum (544) were slower.
 #include "attn.h"
@@ -416,8 +419,12 @@ int kvc_launch_attn_prompt_tc(const kvc_attn_args & a, cudaStream_t st) {
         fprintf(stderr, "[kvc] cuTensorMapEncodeTiled failed for a prompt of %d rows\n", a.n_total);
         return KVC_ERR_CUDA;
     }
-    // two tiles in a CTA for sequences of 4,096 queries and more on average that make 4 CTAs per SM
-    const bool two = a.n_total / a.n_seqs >= 4096 && (long long)a.n_total / (2 * G.tokens) * a.Hkv >= 4LL * kvc_serve_device();
+    // Two tiles in a CTA for sequences of 6,000 queries and more on average that make 4 CTAs per SM (the host knows no
+    // more of the lengths). us with one tile / two, 32 heads on 8, 128 values: 4 x 2,000 queries 177 / 188, 3 x 4,100
+    // 429 / 446, 5,000 215 / 221, 2 x 6,000 565 / 571, 8,192 506 / 510 (589 / 576 in a loop of seconds), 16,000
+    // 1,843 / 1,791; 6,000 beside 16 of 100 301 / 313, 12,000 beside 8 of 300 1,071 / 1,050; 64 values: 4 x 2,000
+    // 147 / 150, 2 x 6,000 491 / 483, 16,000 1,554 / 1,497.
+    const bool two = a.n_total / a.n_seqs >= 6000 && (long long)a.n_total / (2 * G.tokens) * a.Hkv >= 4LL * kvc_serve_device();
     if (a.dk > 64 || a.dv > 64) return two ? launch<128, 2>(a, G, maps, st) : launch<128, 1>(a, G, maps, st);
     return two ? launch<64, 2>(a, G, maps, st) : launch<64, 1>(a, G, maps, st);
 }

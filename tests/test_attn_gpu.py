@@ -809,6 +809,33 @@ def test_prompt_long_sequence(kvc, d, causal):
     assert torch.equal(first, p.out) and bool(torch.isfinite(p.lse).all())
 
 
+@pytest.mark.parametrize("d,causal", [(64, True), (128, True), (64, False), (128, False)])
+@pytest.mark.parametrize("n", [5999, 6000, 6113])
+def test_prompt_either_side_of_two_tiles(kvc, d, causal, n):
+    """Sequences of just less and of as many tokens as make a CTA take two tiles; some rows of some heads."""
+    gen = torch.Generator().manual_seed(n + d)
+    past, hkv, g = 77, 8, 4
+    rnd = lambda *s: torch.randn(*s, generator=gen).to("cuda", torch.float16)  # noqa: E731
+    q, k, v = rnd(n, hkv * g, d), rnd(n + past, hkv, d), rnd(n + past, hkv, d)
+    cu = lambda x: torch.tensor([0, x], dtype=torch.int32, device="cuda")  # noqa: E731
+    p = attn.Prompt(kvc, q, k, v, cu(n), cu(n + past), scale=d ** -0.5, causal=causal)
+    p.out.fill_(7.0)
+    p.run()
+    torch.cuda.synchronize()
+    at = torch.tensor([0, 31, 32, 63, 64, 127, 128, 2047, 2048, n - 66, n - 65, n - 64, n - 33, n - 32, n - 2, n - 1], device="cuda")
+    j = torch.arange(n + past, device="cuda")[None]
+    see = (j <= at[:, None] + past) if causal else (j >= 0).expand(len(at), -1)
+    o_tol, l_tol = bounds(q, k.double(), v.double(), 0.0, R.F16, True, d ** -0.5)
+    for h in (0, 3, 13, 31):
+        o, w = R.attend(q[at, h], k[:, h // g].double(), v[:, h // g].double(), None, see, d ** -0.5)
+        check(p.out[at, h], o, o_tol, "out")
+        check(p.lse[at, h], w, l_tol, "lse")
+    first = p.out.clone()
+    p.run()
+    torch.cuda.synchronize()
+    assert torch.equal(first, p.out) and bool(torch.isfinite(p.lse).all())
+
+
 def test_prompt_fewer_keys_than_queries(kvc):
     """Queries that lie before the first key see nothing; a sequence without keys as well."""
     p = prompt_check(kvc, [100, 5], [-60, -5], dk=128, dv=128)
