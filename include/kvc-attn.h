@@ -4,13 +4,22 @@
  *
  * Query head h reads KV head h / (n_head / n_head_kv). Scores, the running
  * maximum and sum of each softmax and the output sums are held in 32 bits.
+ * On the tensor cores the probabilities (for block types times the scale of
+ * the row's block) meet V in fp16: with F16 queries rounded once, by up to
+ * 2^-11 of each, while the sum that divides them is not rounded, so that F16
+ * outputs carry this rounding beside their own; with F32 queries as two fp16
+ * pieces, 22 bits together, as the queries themselves. Prompts of F32, and
+ * shapes that the tensor-core kernels do not take, are 32-bit throughout.
  * A row that sees no key gets an output of 0 and a log-sum-exp of -inf.
  * The calls launch kernels on `stream` (a cudaStream_t; NULL = the legacy
  * default stream) and return; they read no device value on the host and
  * allocate nothing, so they can be captured into a graph. Pointers are device
  * memory of the current device. Return codes: 0; -1 a null argument; -2 bad
  * dimensions; -4 a row size that does not match; -10 no sm_100 device; -12
- * CUDA error; -13 a shape, alignment or workspace outside the limits.
+ * CUDA error; -13 a shape, alignment or workspace outside the limits. Waits
+ * inside the kernels have a limit, which no call is known to reach; beyond it
+ * kvc_attn_prompt gives rows of NaN, and kvc_attn_tree sets the cache's *status
+ * to -12 and leaves outputs that mean nothing.
  */
 #ifndef KVC_ATTN_H
 #define KVC_ATTN_H

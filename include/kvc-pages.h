@@ -16,8 +16,10 @@
  * Pages are handed out lowest index first, among those that were free when
  * the call started (pages that the call itself gives back serve later calls).
  * A call whose pages do not suffice, or whose table rows are too short,
- * changes nothing but *status, which it sets to -11 or -13; calls that
- * succeed leave *status as it is. The workspace (kvc_pages_workspace bytes)
+ * changes nothing but *status, which it sets to -11 or -13 (of both, -13);
+ * calls that succeed leave *status as it is. A copy that does not arrive
+ * within a kernel's limit sets *status to -12, and the call's rows mean
+ * nothing. The workspace (kvc_pages_workspace bytes)
  * may be shared by ordered calls, not by concurrent ones.
  *
  * Sequence lists are HOST arrays, read before the call returns: ids in

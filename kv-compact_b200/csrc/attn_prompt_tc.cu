@@ -26,7 +26,7 @@
 // Rows, statistics and O are 32-bit; P is rounded to fp16 once (2^-11 relative, as
 // the output is; l is the sum of the unrounded values): a second piece of P would be
 // half as many products again. Against 64 bits the outputs' error grows from 1.9e-4
-// (their own rounding) to 2.5e-4. Bound by the exponentials (16 per clock and SM against 4,096
+// (their own rounding) to 2.2e-4 - 2.9e-4. Bound by the exponentials (16 per clock and SM against 4,096
 // multiply-adds) and the tensor cores about equally at d = 128: a tile's step is
 // a chain of softmax (about 2,350 cycles) and products (78 cycles for each of 16
 // instructions), and two tiles fill an SM's issue slots and tensor cores by turns.

@@ -33,7 +33,7 @@
 // by side) are copied by all warps with cp.async instead.
 //
 // Bound by the work per key, not by memory: 160,000 Q8_0 keys of 8 heads, 4
-// query rows each, 128 values take 140 us with F32 queries (2.5 TB/s of rows,
+// query rows each, 128 values take 141 us with F32 queries (2.5 TB/s of rows,
 // 38 % of HBM's rate). 16 keys of a head cost about 1,000 instructions, 400 of
 // them on the half-rate ALU pipe (codes to fp16, comparisons), and four warps per
 // scheduler, all that 128 registers a thread allow, issue in 59 % of the cycles.

@@ -28,9 +28,9 @@
 // exponentials, P, product, sums) takes about 6,000 cycles at 128 values with two
 // softmax warps per scheduler, which the other stream half hides; and about 15 us
 // per call go to the segments, the queries, the first tile and the join. Trees of
-// 16 to 60 nodes on 26,122 F16 keys (8 heads of 4 query heads, 128 values) 104 us,
+// 16 to 60 nodes on 26,122 F16 keys (8 heads of 4 query heads, 128 values) 108 us,
 // 1.0 TB/s of rows; 25 nodes on 30,000 Q4_0 / Q4_1 keys (4 heads of 8, 64 values,
-// F32 queries) 83 us. Queries read pair by pair before the first tile was asked
+// F32 queries) 84 us. Queries read pair by pair before the first tile was asked
 // for: 122 and 90 us.
 #include "attn.h"
 #include "attn_tc.h"

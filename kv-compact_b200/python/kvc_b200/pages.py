@@ -132,7 +132,8 @@ class PageCache:
 
     def check(self):
         """Wait for the queued calls and raise if one of them could not be done (-11 no free pages, -13 too many rows for
-        the table, -2 a write into a shared page); clears the status."""
+        the table, -2 a write into a shared page, -12 a kernel's wait at its limit: rows or outputs since the last check mean
+        nothing); clears the status."""
         code = int(self.status.item())
         if code:
             self.status.zero_()
@@ -162,7 +163,8 @@ class PageCache:
     def write(self, seqs, first, count, k_rows=None, v_rows=None, beta_rows=None, layer=None):
         """Rows first[i] .. first[i]+count[i]-1 of sequence seqs[i] from packed rows: k_rows, v_rows uint8 [n_layers, sum of
         count, row bytes], beta_rows float32 [n_layers, n_head_kv, sum of count]. With a layer given (a decoder has its rows
-        only after the layer before), that one's alone: [1, ...]."""
+        only after the layer before), that one's alone: [1, ...]. An array left out is not written: a cache with beta wants it for
+        new rows, whose pages hold what was there before."""
         self._rows("kvc_pages_write", seqs, first, count, k_rows, v_rows, beta_rows, layer)
 
     def read(self, seqs, first, count, layer=None):
