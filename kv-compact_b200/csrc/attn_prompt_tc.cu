@@ -26,10 +26,11 @@
 // Rows, statistics and O are 32-bit; P is rounded to fp16 once (2^-11 relative, as
 // the output is; l is the sum of the unrounded values): a second piece of P would be
 // half as many products again. Against 64 bits the outputs' error grows from 1.9e-4
-// (their own rounding) to 2.2e-4 - 2.9e-4. Bound by the exponentials (16 per clock and SM against 4,096
-// multiply-adds) and the tensor cores about equally at d = 128: a tile's step is
-// a chain of softmax (about 2,350 cycles) and products (78 cycles for each of 16
-// instructions), and two tiles fill an SM's issue slots and tensor cores by turns.
+// (their own rounding) to 2.2e-4 - 2.9e-4. Bound by the exponentials (16 per clock
+// and SM against 4,096 multiply-adds) and the tensor cores about equally at d = 128:
+// a tile's step is a chain of softmax (about 2,350 cycles) and products (78 cycles
+// for each of 16 instructions), and two tiles fill an SM's issue slots and tensor
+// cores by turns.
 // The 8,192-token prompt takes 496 us in bursts, 1,100 TFLOP/s or 65 % of a dense
 // product's rate, and 574 in a loop of seconds, 960 TFLOP/s, 68 % of the sustained rate.
 // Steps of 64 keys (723 us), two threads per row (513) and exponentials that do
